@@ -13,8 +13,9 @@ from . import evaluate
 from . import search
 from . import gallery
 from . import align
+from . import adapter
 
 __all__ = ["get_network", "load_model", "get_transform", "extract_features", "extract_batch_embeddings",
-           "compare_faces", "compute_similarity", "embed_images", "cosine_pairs", "evaluate", "search", "gallery", "align",
+           "compare_faces", "compute_similarity", "embed_images", "cosine_pairs", "evaluate", "search", "gallery", "align", "adapter",
            "HipBackbone", "MobileNetV1", "MobileNetV2", "mobilenet_v3_large", "mobilenet_v3_small",
            "sphere20", "sphere36", "sphere64", "default_precision"]

@@ -12,6 +12,11 @@ FR_PREC_BF16, FR_PREC_F32, FR_PREC_F24 = 0, 1, 2
 FR_PLAN_NO_FUSE = 0x100
 FR_OP_CONV, FR_OP_SE, FR_OP_LINEAR = 0, 1, 2
 FR_ACT_NONE, FR_ACT_PRELU, FR_ACT_HSWISH, FR_ACT_RELU, FR_ACT_HSIGMOID = 0, 1, 2, 3, 4
+FR_ACT_GELU, FR_ACT_SILU = 5, 6
+FR_TYPE_F32, FR_TYPE_BF16, FR_TYPE_F16 = 0, 1, 2
+FR_NORM_NONE, FR_NORM_RMS, FR_NORM_LAYER, FR_NORM_L2 = 0, 1, 2, 3
+FR_GATE_NONE, FR_GATE_SIGMOID, FR_GATE_TANH = 0, 1, 2
+FR_SCORE_SOFTMAX, FR_SCORE_SIGMOID = 0, 1
 PRECISIONS = {"bf16": FR_PREC_BF16, "f32": FR_PREC_F32, "f24": FR_PREC_F24}
 
 _fp = C.POINTER(C.c_float)
@@ -65,6 +70,21 @@ _SIGS = {
     "fr_topk_merge": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int64, C.c_int, C.c_void_p, C.c_void_p,
                                 C.c_void_p]),
     "fr_topk_merge_packed": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "fr_linear_workspace_bytes": (C.c_int, [C.c_int64, C.c_int, C.c_int, C.c_int, C.POINTER(C.c_size_t)]),
+    "fr_linear": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p,
+                            C.c_int64, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int,
+                            C.c_void_p, C.c_size_t, C.c_void_p]),
+    "fr_block_norm": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_int64, C.c_int,
+                                C.c_int, C.c_void_p, C.c_void_p, C.c_float,
+                                C.c_void_p, C.c_int, C.c_int64, C.c_int, C.c_int, C.c_float,
+                                C.c_void_p, C.c_int, C.c_void_p, C.c_int,
+                                C.c_int, C.c_void_p, C.c_void_p, C.c_float, C.c_void_p, C.c_int, C.c_void_p]),
+    "fr_route_workspace_bytes": (C.c_int, [C.c_int64, C.c_int, C.c_int, C.POINTER(C.c_size_t)]),
+    "fr_route": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_int, C.c_int, C.c_int,
+                           C.c_float, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "fr_expert_linear": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
+                                   C.c_int, C.c_int64, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int,
+                                   C.c_void_p]),
 }
 EXPORTS = tuple(_SIGS)
 

@@ -1,0 +1,97 @@
+// Element types, raw vector access and activations shared by the adapter kernels (k_linear, k_norm, k_route).
+#pragma once
+#include "kernels.h"
+
+typedef _Float16 f16;
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
+typedef __attribute__((ext_vector_type(2))) unsigned int u32x2;
+
+static inline bool type_ok(int t) { return t == FR_TYPE_F32 || t == FR_TYPE_BF16 || t == FR_TYPE_F16; }
+static inline int type_bytes(int t) { return t == FR_TYPE_F32 ? 4 : 2; }
+
+// Vectors at an element's own alignment: gfx950 global loads and stores of 4..16 bytes take any address.
+typedef u32x4 __attribute__((aligned(2), may_alias)) u32x4_any;
+typedef u32x2 __attribute__((aligned(2), may_alias)) u32x2_any;
+
+// Eight consecutive elements as they lie in memory (fp32: 32 bytes, 16-bit types: 16 bytes in `a`).
+struct Raw8 { u32x4 a, b; };
+
+template <bool ALIGNED>
+FR_DEV Raw8 raw_load8(const void* base, long i, int type) {
+    Raw8 r;
+    if (type == FR_TYPE_F32) {
+        const float* p = reinterpret_cast<const float*>(base) + i;
+        if constexpr (ALIGNED) { r.a = reinterpret_cast<const u32x4*>(p)[0]; r.b = reinterpret_cast<const u32x4*>(p)[1]; }
+        else { r.a = reinterpret_cast<const u32x4_any*>(p)[0]; r.b = reinterpret_cast<const u32x4_any*>(p + 4)[0]; }
+    } else {
+        const unsigned short* p = reinterpret_cast<const unsigned short*>(base) + i;
+        if constexpr (ALIGNED) r.a = *reinterpret_cast<const u32x4*>(p);
+        else r.a = *reinterpret_cast<const u32x4_any*>(p);
+        r.b = u32x4{0, 0, 0, 0};
+    }
+    return r;
+}
+FR_DEV float f16bits_to_f(unsigned short v) { return (float)__builtin_bit_cast(f16, v); }
+FR_DEV Vec8f raw_to_f(const Raw8& r, int type) {
+    Vec8f o;
+    if (type == FR_TYPE_F32) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { o.v[i] = __uint_as_float(r.a[i]); o.v[4 + i] = __uint_as_float(r.b[i]); }
+    } else if (type == FR_TYPE_BF16) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { o.v[2 * i] = __uint_as_float(r.a[i] << 16); o.v[2 * i + 1] = __uint_as_float(r.a[i] & 0xFFFF0000u); }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { o.v[2 * i] = f16bits_to_f((unsigned short)r.a[i]); o.v[2 * i + 1] = f16bits_to_f((unsigned short)(r.a[i] >> 16)); }
+    }
+    return o;
+}
+FR_DEV float load1(const void* base, long i, int type) {
+    if (type == FR_TYPE_F32) return reinterpret_cast<const float*>(base)[i];
+    const unsigned short v = reinterpret_cast<const unsigned short*>(base)[i];
+    return type == FR_TYPE_BF16 ? bfbits_to_f(v) : f16bits_to_f(v);
+}
+FR_DEV unsigned pack2(float lo, float hi, int type) {
+    if (type == FR_TYPE_BF16) return pack2bf(lo, hi);
+    return (unsigned)__builtin_bit_cast(unsigned short, (f16)lo) | ((unsigned)__builtin_bit_cast(unsigned short, (f16)hi) << 16);
+}
+FR_DEV void store1(void* base, long i, int type, float v) {
+    if (type == FR_TYPE_F32) reinterpret_cast<float*>(base)[i] = v;
+    else reinterpret_cast<unsigned short*>(base)[i] = (unsigned short)pack2(v, 0.f, type);
+}
+template <bool ALIGNED>
+FR_DEV void store8t(void* base, long i, int type, const Vec8f& x) {
+    if (type == FR_TYPE_F32) {
+        float* p = reinterpret_cast<float*>(base) + i;
+        u32x4 a, b;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { a[j] = __float_as_uint(x.v[j]); b[j] = __float_as_uint(x.v[4 + j]); }
+        if constexpr (ALIGNED) { reinterpret_cast<u32x4*>(p)[0] = a; reinterpret_cast<u32x4*>(p)[1] = b; }
+        else { reinterpret_cast<u32x4_any*>(p)[0] = a; reinterpret_cast<u32x4_any*>(p + 4)[0] = b; }
+    } else {
+        unsigned short* p = reinterpret_cast<unsigned short*>(base) + i;
+        u32x4 a;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) a[j] = pack2(x.v[2 * j], x.v[2 * j + 1], type);
+        if constexpr (ALIGNED) *reinterpret_cast<u32x4*>(p) = a;
+        else *reinterpret_cast<u32x4_any*>(p) = a;
+    }
+}
+
+// act(v) of the adapter products.  GELU is the erf form v * Phi(v); SiLU v * sigmoid(v).
+FR_DEV float adapter_act(float v, int act, float slope) {
+    switch (act) {
+        case FR_ACT_PRELU: return v >= 0.f ? v : v * slope;
+        case FR_ACT_HSWISH: return v * fminf(fmaxf(fmaf(v, 1.f / 6.f, 0.5f), 0.f), 1.f);
+        case FR_ACT_RELU: return v > 0.f ? v : (v != v ? v : 0.f);
+        case FR_ACT_HSIGMOID: return fminf(fmaxf(fmaf(v, 1.f / 6.f, 0.5f), 0.f), 1.f);
+        case FR_ACT_GELU: return 0.5f * v * erfcf(-0.70710678118654752f * v);
+        case FR_ACT_SILU: {
+            // sigmoid(v) = 1 / (1 + e^2) or e^2 / (1 + e^2) with e = exp(-|v| / 2): no overflow, and v e e keeps results
+            // whose sigmoid alone is below the normal numbers
+            const float e = expf(-0.5f * fabsf(v)), r = 1.f / fmaf(e, e, 1.f);
+            return v >= 0.f ? v * r : (v * e) * (e * r);
+        }
+        default: return v;
+    }
+}

@@ -210,6 +210,7 @@ int build_layer(fr_plan* pl, const fr_layer_desc& d, int idx, Layer& L) {
     if (d.src < 0) { L.inC = pl->in_c; L.inH = pl->in_h; L.inW = pl->in_w; L.in_f32 = af32; L.in_fmt = afmt; }
     else { const Layer& s = pl->layers[d.src]; L.inC = s.C; L.inH = s.H; L.inW = s.W; L.in_f32 = s.out_f32; L.in_fmt = s.out_fmt; }
     if (d.act == FR_ACT_PRELU && !d.prelu) FR_FAIL(FR_ERR_ARG, std::string(where) + "PReLU without slopes");
+    if (d.act == FR_ACT_GELU || d.act == FR_ACT_SILU) FR_FAIL(FR_ERR_UNSUPPORTED, std::string(where) + "GELU / SiLU are activations of the adapter products only");
     if (!d.weight) FR_FAIL(FR_ERR_ARG, std::string(where) + "missing weight");
 
     if (d.op == FR_OP_CONV) {

@@ -239,13 +239,19 @@ def export_json(gallery: Gallery, json_path: str, chunk: int = 65536) -> None:
 
 
 def build_from_images(model, device, ids: Sequence[str], images: Sequence[np.ndarray], out_dir: str,
-                      batch_size: int = 1024, shard_rows: int = 1 << 20) -> Gallery:
+                      batch_size: int = 1024, shard_rows: int = 1 << 20, adapter=None) -> Gallery:
     """Batched replacement for the per-file loop of ``extract_batch_embeddings`` (inference.py:150-153) at
-    gallery scale: uint8 [112,112,3] faces -> fr_embed_u8 -> fr_l2norm_bf16 -> shard files."""
+    gallery scale: uint8 [112,112,3] faces -> fr_embed_u8 -> fr_l2norm_bf16 -> shard files.  With an ``adapter`` (a block of
+    the adapter module) the embeddings go through it, and its last norm writes the unit rows (``adapter.rows``): queries
+    have to take the same way."""
     from .inference import embed_images
     if len(ids) != len(images):
         raise ValueError(f"{len(ids)} ids for {len(images)} images")
     with GalleryWriter(out_dir, 512, shard_rows) as w:
         for i in range(0, len(images), batch_size):
-            w.add(ids[i:i + batch_size], embed_images(model, device, images[i:i + batch_size], batch_size))
+            emb = embed_images(model, device, images[i:i + batch_size], batch_size)
+            if adapter is None:
+                w.add(ids[i:i + batch_size], emb)
+            else:
+                w.add_normalized(ids[i:i + batch_size], adapter.rows(emb))
     return Gallery(out_dir)

@@ -87,9 +87,10 @@ def extract_features(model, device, img_path: str) -> np.ndarray:
 _STAGING: Dict[Tuple[int, bool], List[torch.Tensor]] = {}
 
 
-def embed_images(model, device, images: Sequence[np.ndarray], batch_size: int = 1024) -> torch.Tensor:
+def embed_images(model, device, images: Sequence[np.ndarray], batch_size: int = 1024, adapter=None) -> torch.Tensor:
     """Batched extraction: uint8 [112,112,3] arrays -> fp32 [n,512] on
-    ``device``.  Same arithmetic as extract_features per image, large batches on the GPU."""
+    ``device``.  Same arithmetic as extract_features per image, large batches on the GPU.
+    ``adapter``: a block of the adapter module that every batch of embeddings goes through."""
     outs: List[torch.Tensor] = []
     n = len(images)
     if n == 0:
@@ -121,7 +122,8 @@ def embed_images(model, device, images: Sequence[np.ndarray], batch_size: int = 
             if pinned:
                 done[k] = torch.cuda.Event()
                 done[k].record(torch.cuda.current_stream(dev))
-            outs.append(model.forward_u8(x))
+            emb = model.forward_u8(x)
+            outs.append(emb if adapter is None else adapter(emb))
     return torch.cat(outs) if len(outs) > 1 else outs[0]
 
 

@@ -32,6 +32,14 @@ _defs.define("cosine_pairs(Tensor a, Tensor b, float eps, float threshold) -> (T
 _defs.define("l2norm_bf16(Tensor x) -> Tensor")
 _defs.define("topk_search(Tensor q, Tensor g, int k, int idx_offset) -> (Tensor, Tensor)")
 _defs.define("topk_merge(Tensor scores, Tensor idx, int k) -> (Tensor, Tensor)")
+_defs.define("linear(Tensor x, Tensor weight, Tensor? bias, Tensor? slope, Tensor? residual, str act, ScalarType? out_dtype) -> Tensor")
+_defs.define("block_norm(Tensor x, Tensor? residual, Tensor? slot_weights, str norm, Tensor? weight, Tensor? bias, float eps, "
+             "Tensor? gate, str gate_act, float scale, str next_norm, Tensor? next_weight, Tensor? next_bias, float next_eps, "
+             "ScalarType? out_dtype, ScalarType? next_dtype) -> (Tensor, Tensor)")
+_defs.define("route(Tensor logits, int k, str score, Tensor? bias, int groups, int top_groups, bool renormalise, float scale) "
+             "-> (Tensor, Tensor, Tensor, Tensor)")
+_defs.define("expert_linear(Tensor x, Tensor weight, Tensor order, Tensor offsets, int k, Tensor? bias, str act, Tensor? slope, "
+             "str rows, str out, ScalarType? out_dtype) -> Tensor")
 _impl = torch.library.Library(_NS, "IMPL", "CUDA")
 _meta = torch.library.Library(_NS, "IMPL", "Meta")
 
@@ -174,12 +182,265 @@ def _topk_merge(scores, idx, k):
     return out_s, out_i
 
 
+# ---- adapter blocks (adapter.py) ---------------------------------------------------------------------------------------
+# Scratch is allocated per call: a call captured into a graph gets memory of the graph's own pool, so two graphs, or a graph
+# and the eager program, never write to the same workspace.
+_TYPES = {torch.float32: _lib.FR_TYPE_F32, torch.bfloat16: _lib.FR_TYPE_BF16, torch.float16: _lib.FR_TYPE_F16}
+_ACTS = {"none": _lib.FR_ACT_NONE, "prelu": _lib.FR_ACT_PRELU, "hswish": _lib.FR_ACT_HSWISH, "relu": _lib.FR_ACT_RELU,
+         "hsigmoid": _lib.FR_ACT_HSIGMOID, "gelu": _lib.FR_ACT_GELU, "silu": _lib.FR_ACT_SILU}
+_NORMS = {"none": _lib.FR_NORM_NONE, "rms": _lib.FR_NORM_RMS, "layer": _lib.FR_NORM_LAYER, "l2": _lib.FR_NORM_L2}
+_GATE_ACTS = {"none": _lib.FR_GATE_NONE, "sigmoid": _lib.FR_GATE_SIGMOID, "tanh": _lib.FR_GATE_TANH}
+_SCORES = {"softmax": _lib.FR_SCORE_SOFTMAX, "sigmoid": _lib.FR_SCORE_SIGMOID}
+
+
+def _fail(op, what):
+    raise RuntimeError(f"fr_hip::{op}: {what}")
+
+
+def _name(op, table, key, what):
+    code = table.get(key)
+    if code is None:
+        _fail(op, f"{what} is one of {', '.join(table)}: got {key!r}")
+    return code
+
+
+def _type(op, what, dtype):
+    code = _TYPES.get(dtype)
+    if code is None:
+        _fail(op, f"{what} is float32, bfloat16 or float16: got {dtype}")
+    return code
+
+
+def _check_tensors(op, first, *others):
+    """One device, and no gradient asked for: the kernels have no backward pass, and a result that silently cuts the graph
+    would be a wrong one."""
+    grad = torch.is_grad_enabled()
+    if grad and first.requires_grad:
+        _fail(op, "inference only: call it under torch.no_grad() or on detached tensors")
+    dev = first.device
+    for t in others:
+        if t is not None:
+            if t.device != dev:
+                _fail(op, f"all tensors on {dev}: got one on {t.device}")
+            if grad and t.requires_grad:
+                _fail(op, "inference only: call it under torch.no_grad() or on detached tensors")
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _call(name, dev, *args):
+    fn = getattr(_lib.lib(), name)
+    if torch.cuda.current_device() == dev.index:
+        _lib.check(fn(*args, _stream(dev)), name)
+    else:
+        with torch.cuda.device(dev):
+            _lib.check(fn(*args, _stream(dev)), name)
+
+
+def _rows(t, width):
+    """``t`` [..., width] as rows: (tensor, row stride).  A matrix whose rows are whole but apart is taken as it lies."""
+    if t.dim() == 2 and (t.stride(1) == 1 or width == 1) and t.stride(0) >= 0:
+        return t, t.stride(0)
+    return t.contiguous(), width
+
+
+def _vector(op, what, t, n, dtypes):
+    if t is None:
+        return None
+    if t.shape != (n,) or t.dtype not in dtypes:
+        _fail(op, f"{what} is [{n}] of {' or '.join(str(d)[6:] for d in dtypes)}: got {t.dtype} {tuple(t.shape)}")
+    return t.contiguous()
+
+
+def _linear_shape(op, x, weight, residual, out_dtype):
+    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1] or weight.shape[1] < 1 or weight.shape[0] < 1:
+        _fail(op, f"expected x [..., K] and weight [N, K]: got {tuple(x.shape)} and {tuple(weight.shape)}")
+    shape = x.shape[:-1] + (weight.shape[0],)
+    if residual is not None and residual.shape != shape:
+        _fail(op, f"residual is {tuple(shape)}: got {tuple(residual.shape)}")
+    return shape
+
+
+def _linear(x, weight, bias, slope, residual, act, out_dtype):
+    op = "linear"
+    _check_tensors(op, x, weight, bias, slope, residual)
+    shape = _linear_shape(op, x, weight, residual, out_dtype)
+    N, K = weight.shape
+    kind = _type(op, "x", x.dtype)
+    if weight.dtype != x.dtype:
+        _fail(op, f"x and weight have one type: got {x.dtype} and {weight.dtype}")
+    act = _name(op, _ACTS, act, "act")
+    if (slope is not None) != (act == _lib.FR_ACT_PRELU):
+        _fail(op, "slope belongs to act='prelu', and only to it")
+    bias = _vector(op, "bias", bias, N, (x.dtype, torch.float32))
+    slope = _vector(op, "slope", slope, N, (torch.float32,))
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    out_type = _type(op, "out_dtype", out_dtype)
+    res_type = kind if residual is None else _type(op, "residual", residual.dtype)
+    out = torch.empty(shape, dtype=out_dtype, device=x.device)
+    M = out.numel() // N
+    if M == 0:
+        return out
+    x, ldx = _rows(x, K)
+    residual, ldr = (None, 0) if residual is None else _rows(residual, N)
+    weight = weight.contiguous()
+    need = C.c_size_t()
+    _lib.check(_lib.lib().fr_linear_workspace_bytes(M, N, K, kind, C.byref(need)), "fr_linear_workspace_bytes")
+    ws = torch.empty(need.value, dtype=torch.uint8, device=x.device) if need.value else None
+    _call("fr_linear", x.device, x.data_ptr(), ldx, weight.data_ptr(), _ptr(bias), _ptr(slope), _ptr(residual), ldr, out.data_ptr(),
+          M, N, K, kind, kind if bias is None else _TYPES[bias.dtype], res_type, out_type, act, _ptr(ws), need.value)
+    return out
+
+
+def _block_norm_shape(op, x, slot_weights):
+    least = 1 if slot_weights is None else 2
+    if x.dim() < least or x.shape[-1] < 1:
+        _fail(op, f"expected x [..., d], or [..., slots, d] with slot_weights: got {tuple(x.shape)}")
+    if slot_weights is None:
+        return x.shape
+    if slot_weights.shape != x.shape[:-1] or slot_weights.dtype != torch.float32 or x.shape[-2] < 1:
+        _fail(op, f"slot_weights is float32 {tuple(x.shape[:-1])}: got {slot_weights.dtype} {tuple(slot_weights.shape)}")
+    return x.shape[:-2] + x.shape[-1:]
+
+
+def _block_norm(x, residual, slot_weights, norm, weight, bias, eps, gate, gate_act, scale, next_norm, next_weight, next_bias,
+                next_eps, out_dtype, next_dtype):
+    op = "block_norm"
+    _check_tensors(op, x, residual, slot_weights, weight, bias, gate, next_weight, next_bias)
+    shape = _block_norm_shape(op, x, slot_weights)
+    d = x.shape[-1]
+    norm, next_norm = _name(op, _NORMS, norm, "norm"), _name(op, _NORMS, next_norm, "next_norm")
+    f32 = (torch.float32,)
+    for n, w, b, what in ((norm, weight, bias, ""), (next_norm, next_weight, next_bias, "next_")):
+        if (w is not None or b is not None) and n not in (_lib.FR_NORM_RMS, _lib.FR_NORM_LAYER):
+            _fail(op, f"{what}weight and {what}bias belong to the rms and layer norms")
+    weight, bias = _vector(op, "weight", weight, d, f32), _vector(op, "bias", bias, d, f32)
+    next_weight, next_bias = _vector(op, "next_weight", next_weight, d, f32), _vector(op, "next_bias", next_bias, d, f32)
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    next_dtype = out_dtype if next_dtype is None else next_dtype
+    out_type, next_type, x_type = _type(op, "out_dtype", out_dtype), _type(op, "next_dtype", next_dtype), _type(op, "x", x.dtype)
+    res_type = gate_type = gate_ldt = gate_ldc = 0
+    if residual is not None:
+        if residual.shape != shape:
+            _fail(op, f"residual is {tuple(shape)}: got {tuple(residual.shape)}")
+        res_type, residual = _type(op, "residual", residual.dtype), residual.contiguous()
+    if gate is not None:
+        gate_type = _type(op, "gate", gate.dtype)
+        if gate.shape == (d,):
+            gate, gate_ldc = gate.contiguous(), 1
+        elif gate.shape == shape:
+            gate, gate_ldt, gate_ldc = gate.contiguous(), d, 1
+        elif gate.shape == shape[:-1] + (1,):
+            gate, gate_ldt = gate.contiguous(), 1
+        else:
+            _fail(op, f"gate is [{d}], {tuple(shape[:-1]) + (1,)} or {tuple(shape)}: got {tuple(gate.shape)}")
+    gate_act = _name(op, _GATE_ACTS, gate_act, "gate_act")
+    out = torch.empty(shape, dtype=out_dtype, device=x.device)
+    nxt = torch.empty(shape if next_norm else 0, dtype=next_dtype, device=x.device)
+    T = out.numel() // d
+    if T == 0:
+        return out, nxt
+    slots = 0 if slot_weights is None else x.shape[-2]
+    x = x.contiguous()
+    slot_weights = None if slot_weights is None else slot_weights.contiguous()
+    _call("fr_block_norm", x.device, x.data_ptr(), x_type, slots, _ptr(slot_weights), T, d, norm, _ptr(weight), _ptr(bias), eps,
+          _ptr(gate), gate_type, gate_ldt, gate_ldc, gate_act, scale, _ptr(residual), res_type, out.data_ptr(), out_type,
+          next_norm, _ptr(next_weight), _ptr(next_bias), next_eps, nxt.data_ptr() if next_norm else None, next_type)
+    return out, nxt
+
+
+def _route_shape(op, logits, k):
+    if logits.dim() != 2 or logits.shape[1] < 1:
+        _fail(op, f"expected logits [T, E]: got {tuple(logits.shape)}")
+    T, E = logits.shape
+    if not 1 <= k <= E:
+        _fail(op, f"1 <= k <= {E} experts: got {k}")
+    return T, E
+
+
+def _route_empty(logits, k):
+    T, E = logits.shape
+    i32 = dict(dtype=torch.int32, device=logits.device)
+    return (torch.empty((T, k), dtype=torch.float32, device=logits.device), torch.empty((T, k), **i32),
+            torch.empty(T * k, **i32), torch.empty(E + 1, **i32))
+
+
+def _route(logits, k, score, bias, groups, top_groups, renormalise, scale):
+    op = "route"
+    _check_tensors(op, logits, bias)
+    T, E = _route_shape(op, logits, k)
+    kind = _type(op, "logits", logits.dtype)
+    score = _name(op, _SCORES, score, "score")
+    bias = _vector(op, "bias", bias, E, (torch.float32,))
+    logits = logits.contiguous()
+    need = C.c_size_t()
+    _lib.check(_lib.lib().fr_route_workspace_bytes(T, E, k, C.byref(need)), "fr_route_workspace_bytes")
+    out = _route_empty(logits, k)
+    ws = torch.empty(need.value, dtype=torch.uint8, device=logits.device)
+    weights, experts, order, offsets = (t.data_ptr() or ws.data_ptr() for t in out)      # T = 0: empty tensors have no address
+    _call("fr_route", logits.device, logits.data_ptr(), kind, T, E, k, score, _ptr(bias), groups, top_groups, renormalise, scale,
+          weights, experts, order, offsets, ws.data_ptr(), need.value)
+    return out
+
+
+def _expert_shape(op, x, weight, order, offsets, k, rows, out):
+    if x.dim() != 2 or weight.dim() != 3 or x.shape[1] != weight.shape[2] or min(weight.shape) < 1:
+        _fail(op, f"expected x [rows, K] and weight [E, N, K]: got {tuple(x.shape)} and {tuple(weight.shape)}")
+    if rows not in ("tokens", "sorted") or out not in ("sorted", "slots"):
+        _fail(op, f"rows is 'tokens' or 'sorted', out 'sorted' or 'slots': got {rows!r}, {out!r}")
+    if order.dtype != torch.int32 or offsets.dtype != torch.int32 or order.dim() != 1 or offsets.shape != (weight.shape[0] + 1,):
+        _fail(op, f"expected int32 order [T*k] and offsets [{weight.shape[0] + 1}] as route returns them")
+    if k < 1 or order.shape[0] % k:
+        _fail(op, f"{order.shape[0]} slots are no multiple of k = {k}")
+    T = order.shape[0] // k
+    if x.shape[0] != (T if rows == "tokens" else T * k):
+        _fail(op, f"rows={rows!r} takes {T if rows == 'tokens' else T * k} rows of x: got {x.shape[0]}")
+    return T, (T * k, weight.shape[1]) if out == "sorted" else (T, k, weight.shape[1])
+
+
+def _expert_linear(x, weight, order, offsets, k, bias, act, slope, rows, out, out_dtype):
+    op = "expert_linear"
+    _check_tensors(op, x, weight, order, offsets, bias, slope)
+    T, shape = _expert_shape(op, x, weight, order, offsets, k, rows, out)
+    E, N, K = weight.shape
+    kind = _type(op, "x", x.dtype)
+    if weight.dtype != x.dtype:
+        _fail(op, f"x and weight have one type: got {x.dtype} and {weight.dtype}")
+    act = _name(op, _ACTS, act, "act")
+    if (slope is not None) != (act == _lib.FR_ACT_PRELU):
+        _fail(op, "slope belongs to act='prelu', and only to it")
+    if bias is not None:
+        if bias.shape != (E, N) or bias.dtype not in (x.dtype, torch.float32):
+            _fail(op, f"bias is [{E}, {N}] of x's type or float32: got {bias.dtype} {tuple(bias.shape)}")
+        bias = bias.contiguous()
+    if slope is not None:
+        if slope.shape != (E, N) or slope.dtype != torch.float32:
+            _fail(op, f"slope is float32 [{E}, {N}]: got {slope.dtype} {tuple(slope.shape)}")
+        slope = slope.contiguous()
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    y = torch.empty(shape, dtype=out_dtype, device=x.device)
+    out_type = _type(op, "out_dtype", out_dtype)
+    if T == 0:
+        return y
+    x, weight, order, offsets = x.contiguous(), weight.contiguous(), order.contiguous(), offsets.contiguous()
+    _call("fr_expert_linear", x.device, x.data_ptr(), int(rows == "sorted"), weight.data_ptr(), _ptr(bias), _ptr(slope), order.data_ptr(),
+          offsets.data_ptr(), y.data_ptr(), int(out == "slots"), T, k, E, N, K, kind, kind if bias is None else _TYPES[bias.dtype],
+          out_type, act)
+    return y
+
+
 _impl.impl("embed", _embed)
 _impl.impl("embed_u8", _embed_u8)
 _impl.impl("cosine_pairs", _cosine_pairs)
 _impl.impl("l2norm_bf16", _l2norm_bf16)
 _impl.impl("topk_search", _topk_search)
 _impl.impl("topk_merge", _topk_merge)
+_impl.impl("linear", _linear)
+_impl.impl("block_norm", _block_norm)
+_impl.impl("route", _route)
+_impl.impl("expert_linear", _expert_linear)
 
 # shape functions (tracing / torch.export)
 _meta.impl("embed", lambda x, plan, c, h, w: x.new_empty(_out_shape(x.shape[0], c, h, w), dtype=torch.float32))
@@ -191,3 +452,28 @@ _meta.impl("topk_search", lambda q, g, k, off: (q.new_empty((q.shape[0], k), dty
                                                 q.new_empty((q.shape[0], k), dtype=torch.int64)))
 _meta.impl("topk_merge", lambda s, i, k: (s.new_empty((s.shape[1], k), dtype=torch.float32),
                                           s.new_empty((s.shape[1], k), dtype=torch.int64)))
+
+
+def _meta_linear(x, weight, bias, slope, residual, act, out_dtype):
+    return x.new_empty(_linear_shape("linear", x, weight, residual, out_dtype), dtype=out_dtype or x.dtype)
+
+
+def _meta_block_norm(x, residual, slot_weights, norm, weight, bias, eps, gate, gate_act, scale, next_norm, next_weight, next_bias,
+                     next_eps, out_dtype, next_dtype):
+    shape, out_dtype = _block_norm_shape("block_norm", x, slot_weights), out_dtype or x.dtype
+    return x.new_empty(shape, dtype=out_dtype), x.new_empty(shape if next_norm != "none" else 0, dtype=next_dtype or out_dtype)
+
+
+def _meta_route(logits, k, score, bias, groups, top_groups, renormalise, scale):
+    _route_shape("route", logits, k)
+    return _route_empty(logits, k)
+
+
+def _meta_expert_linear(x, weight, order, offsets, k, bias, act, slope, rows, out, out_dtype):
+    return x.new_empty(_expert_shape("expert_linear", x, weight, order, offsets, k, rows, out)[1], dtype=out_dtype or x.dtype)
+
+
+_meta.impl("linear", _meta_linear)
+_meta.impl("block_norm", _meta_block_norm)
+_meta.impl("route", _meta_route)
+_meta.impl("expert_linear", _meta_expert_linear)

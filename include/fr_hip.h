@@ -46,7 +46,10 @@ typedef enum fr_precision { FR_PREC_BF16 = 0, FR_PREC_F32 = 1, FR_PREC_F24 = 2 }
 
 typedef enum fr_op { FR_OP_CONV = 0, FR_OP_SE = 1, FR_OP_LINEAR = 2 } fr_op;
 typedef enum fr_act { FR_ACT_NONE = 0, FR_ACT_PRELU = 1, FR_ACT_HSWISH = 2,
-                      FR_ACT_RELU = 3, FR_ACT_HSIGMOID = 4 } fr_act;
+                      FR_ACT_RELU = 3, FR_ACT_HSIGMOID = 4,
+                      FR_ACT_GELU = 5, FR_ACT_SILU = 6 } fr_act;   /* 5, 6: fr_linear / fr_expert_linear only */
+/* Element types of the adapter operators' tensors (their x_type / out_type / ... arguments). */
+typedef enum fr_type { FR_TYPE_F32 = 0, FR_TYPE_BF16 = 1, FR_TYPE_F16 = 2 } fr_type;
 
 /* One reference layer group, described with HOST pointers to the fp32 tensors exactly as they sit
  * in the reference state_dict (no folding, no re-layout on the caller's side).
@@ -217,6 +220,64 @@ int fr_topk_merge(const float* scores, const int64_t* idx, int P, int64_t Q, int
  * (face-recognition_amd/search.py: packed_bytes, exchange_topk_chunks). */
 int fr_topk_merge_packed(const void* packed, int P, int64_t Q, int k,
                          float* out_scores, int64_t* out_idx, void* stream);
+
+/* ---- adapter operators (no counterpart in the reference) ------------------------------------------------------------
+ * A residual block over embedding rows: products with their epilogue, norms fused with gate, scale and residual, and the
+ * mixture form of both (a router and its experts' products).  Inference only.  All row-major; matrices may start at any
+ * address their element type allows; statistics, sums and epilogues are fp32, results are rounded once. */
+
+/* out[m][n] = act(sum_k x[m][k] w[n][k] + bias[n]) + residual[m][n].
+ * x [M][K] (row stride ldx), w [N][K] contiguous, both of type `type` (fp32 products are exact fp32 MFMA, not split);
+ * bias [N] of bias_type (`type` or fp32) or NULL; slope fp32 [N] for FR_ACT_PRELU; residual [M][N] (row stride ldr) of
+ * res_type or NULL; out [M][N] contiguous of out_type.  residual may be `out` itself.
+ * workspace: fr_linear_workspace_bytes of the same M, N, K, type (0 for most shapes; then workspace may be NULL). */
+int fr_linear_workspace_bytes(int64_t M, int N, int K, int type, size_t* out_bytes);
+int fr_linear(const void* x, int64_t ldx, const void* w, const void* bias, const float* slope,
+              const void* residual, int64_t ldr, void* out, int64_t M, int N, int K,
+              int type, int bias_type, int res_type, int out_type, int act,
+              void* workspace, size_t workspace_bytes, void* stream);
+
+/* out = residual + scale * g(gate) * norm(y), next = next_norm(out before its rounding), y = x or sum_j slot_weights[t][j] x[t][j].
+ * x [T][d], or [T][slots][d] with slot_weights fp32 [T][slots] (slots >= 1; slots = 0: no slot dimension).  A slot whose
+ * weight is 0 is not read into the sum, whatever it holds.  Norms: FR_NORM_NONE; FR_NORM_RMS y / sqrt(mean(y^2) + eps) * weight;
+ * FR_NORM_LAYER (y - mean) / sqrt(var + eps) * weight + bias; FR_NORM_L2 y / ||y|| (a zero row stays zero; no weight).
+ * weight / bias / next_weight / next_bias: fp32 [d] or NULL (= 1 / 0).  gate of gate_type or NULL, element (t, c) at
+ * gate[t * gate_ldt + c * gate_ldc] (strides 0 = broadcast; gate_ldc 0 or 1); g by gate_act (FR_GATE_*).  residual [T][d] of
+ * res_type (row stride d) or NULL.  out [T][d] of out_type or NULL (not wanted); next_out [T][d] of next_type, or NULL
+ * with FR_NORM_NONE as next_norm.  d <= 16384.  out and next_out may not overlap each other; residual may be `out`. */
+typedef enum fr_norm { FR_NORM_NONE = 0, FR_NORM_RMS = 1, FR_NORM_LAYER = 2, FR_NORM_L2 = 3 } fr_norm;
+typedef enum fr_gate_act { FR_GATE_NONE = 0, FR_GATE_SIGMOID = 1, FR_GATE_TANH = 2 } fr_gate_act;
+int fr_block_norm(const void* x, int x_type, int slots, const float* slot_weights, int64_t T, int d,
+                  int norm, const float* weight, const float* bias, float eps,
+                  const void* gate, int gate_type, int64_t gate_ldt, int gate_ldc, int gate_act, float scale,
+                  const void* residual, int res_type, void* out, int out_type,
+                  int next_norm, const float* next_weight, const float* next_bias, float next_eps,
+                  void* next_out, int next_type, void* stream);
+
+/* Routing of T rows to k of E experts, from logits [T][E] of logits_type.
+ * score = softmax over the row (FR_SCORE_SOFTMAX) or sigmoid (FR_SCORE_SIGMOID); key = score + bias[e] (fp32 or NULL; the
+ * bias moves the choice, not the weights).  groups > 1: experts in `groups` equal runs, a group's key = the sum of its best
+ * two keys (its one key where groups == E), only the best top_groups groups stay.  Then the best k keys, ties to the lower
+ * index; keys are ordered as exact scores are (decided in 64 bits where 32 cannot tell them apart).  A logit (or bias) that
+ * is -inf or NaN masks its expert; slots that find no expert get expert -1 and weight 0.
+ * weights [T][k] fp32: the chosen scores, divided by their sum if renormalise, times scale.  experts [T][k] int32, best first.
+ * order [T*k] int32: slot numbers t*k + j sorted by expert, stable; the slots without an expert come last.
+ * offsets [E+1] int32: expert e's slots are order[offsets[e] .. offsets[e+1]).
+ * E <= 512, k <= min(16, E), groups <= 64 dividing E, T*k < 2^31. */
+typedef enum fr_score { FR_SCORE_SOFTMAX = 0, FR_SCORE_SIGMOID = 1 } fr_score;
+int fr_route_workspace_bytes(int64_t T, int E, int k, size_t* out_bytes);
+int fr_route(const void* logits, int logits_type, int64_t T, int E, int k, int score, const float* bias,
+             int groups, int top_groups, int renormalise, float scale,
+             float* weights, int32_t* experts, int32_t* order, int32_t* offsets,
+             void* workspace, size_t workspace_bytes, void* stream);
+
+/* out = act(row x w[e]^T + bias[e]) for every routed slot, e the slot's expert; order / offsets as fr_route writes them for T*k slots.
+ * w [E][N][K], bias [E][N] or NULL, slope fp32 [E][N] for FR_ACT_PRELU.  rows_sorted 0: x [T][K], slot s takes row s / k;
+ * rows_sorted 1: x [T*k][K], position p of the order takes row p.  out_slots 0: out [T*k][N] in the order's positions;
+ * out_slots 1: out row = slot number.  Slots without an expert get zero rows.  An order entry outside [0, T*k) is skipped. */
+int fr_expert_linear(const void* x, int rows_sorted, const void* w, const void* bias, const float* slope,
+                     const int32_t* order, const int32_t* offsets, void* out, int out_slots,
+                     int64_t T, int k, int E, int N, int K, int type, int bias_type, int out_type, int act, void* stream);
 
 #ifdef __cplusplus
 }
