@@ -78,20 +78,34 @@ FR_DEV void store8t(void* base, long i, int type, const Vec8f& x) {
     }
 }
 
-// act(v) of the adapter products.  GELU is the erf form v * Phi(v); SiLU v * sigmoid(v).
+// act(v) of the adapter products.  GELU is the erf form v Phi(v), SiLU v sigmoid(v).
+// exp2 and reciprocal are the hardware's (1 ulp).  Phi(-a) = erfc(a / sqrt 2) / 2 = t P(t) exp(-a^2 / 2) with
+// t = 1 / (1 + 0.3 a / sqrt 2): P is a minimax fit of erfcx(z) / t over t in (0.23, 1], 2.0e-8 relative, so small values of
+// either tail keep their digits.  SiLU is 0 below -88.7, where e^-v leaves fp32's range and |v sigmoid(v)| < 2.7e-37: the
+// epilogue of a wide product is bound by its vector instructions, and a form that keeps those values costs five more.
+FR_DEV float gelu(float v) {
+    const float t = __builtin_amdgcn_rcpf(fmaf(fabsf(v), 0.3f * 0.70710678118654752f, 1.f));
+    float p = -0.12955585f;
+    p = fmaf(p, t, 0.48573610f);
+    p = fmaf(p, t, -0.51266706f);
+    p = fmaf(p, t, 0.54820925f);
+    p = fmaf(p, t, -0.095026374f);
+    p = fmaf(p, t, 0.21510610f);
+    p = fmaf(p, t, 0.14828666f);
+    p = fmaf(p, t, 0.17072374f);
+    p = fmaf(p, t, 0.16918743f);
+    const float tail = 0.5f * (t * p) * __builtin_amdgcn_exp2f((v * v) * -0.72134752044448170f);
+    return v * (v < 0.f ? tail : 1.f - tail);
+}
+FR_DEV float silu(float v) { return v * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(v * -1.4426950408889634f)); }
 FR_DEV float adapter_act(float v, int act, float slope) {
     switch (act) {
         case FR_ACT_PRELU: return v >= 0.f ? v : v * slope;
-        case FR_ACT_HSWISH: return v * fminf(fmaxf(fmaf(v, 1.f / 6.f, 0.5f), 0.f), 1.f);
-        case FR_ACT_RELU: return v > 0.f ? v : (v != v ? v : 0.f);
-        case FR_ACT_HSIGMOID: return fminf(fmaxf(fmaf(v, 1.f / 6.f, 0.5f), 0.f), 1.f);
-        case FR_ACT_GELU: return 0.5f * v * erfcf(-0.70710678118654752f * v);
-        case FR_ACT_SILU: {
-            // sigmoid(v) = 1 / (1 + e^2) or e^2 / (1 + e^2) with e = exp(-|v| / 2): no overflow, and v e e keeps results
-            // whose sigmoid alone is below the normal numbers
-            const float e = expf(-0.5f * fabsf(v)), r = 1.f / fmaf(e, e, 1.f);
-            return v >= 0.f ? v * r : (v * e) * (e * r);
-        }
+        case FR_ACT_HSWISH: return v * __builtin_amdgcn_fmed3f(fmaf(v, 1.f / 6.f, 0.5f), 0.f, 1.f);
+        case FR_ACT_RELU: return v < 0.f ? 0.f : v;
+        case FR_ACT_HSIGMOID: return v != v ? v : __builtin_amdgcn_fmed3f(fmaf(v, 1.f / 6.f, 0.5f), 0.f, 1.f);
+        case FR_ACT_GELU: return gelu(v);
+        case FR_ACT_SILU: return silu(v);
         default: return v;
     }
 }

@@ -5,6 +5,8 @@
 // one row and stores vectors.  A "chunk" is 16 bytes of a row: 8 elements of 16 bits, one lane's share of
 // v_mfma_f32_16x16x32, or 4 floats, one each for four v_mfma_f32_16x16x4_f32 (the same k order in both operands, so any
 // assignment of chunks to lanes gives the product).
+#include <math.h>
+
 #include "adapter.h"
 
 namespace {
@@ -97,31 +99,84 @@ FR_DEV Vec8f get8n(const void* base, long i, int n, int type) {
     for (int j = 0; j < 8; ++j) o.v[j] = j < n ? load1(base, i + j, type) : 0.f;
     return o;
 }
-// Eight outputs n0 .. n0+7 (as many as N has) of row `row`.
-FR_DEV void finish8(const GemmArgs& a, long row, int n0, long nbase, Vec8f v) {
-    const int n = min(8, a.N - n0);
-    if (n <= 0) return;
-    if (a.bias) {
-        const Vec8f b = get8n(a.bias, nbase + n0, n, a.bias_type);
+template <int ACT>
+FR_DEV void act8c(Vec8f& v, const Vec8f& slope) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v.v[j] += b.v[j];
+    for (int j = 0; j < 8; ++j) v.v[j] = adapter_act(v.v[j], ACT, slope.v[j]);
+}
+FR_DEV void put8n(void* base, long i, int n, int type, const Vec8f& v) {
+    if (n == 8) { store8t<false>(base, i, type, v); return; }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) if (j < n) store1(base, i + j, type, v.v[j]);
+}
+// Bias and slopes of eight output columns, `have` of which exist.
+struct Columns { Vec8f bias, slope; };
+FR_DEV Columns columns(const GemmArgs& a, int n, int have, long nbase, bool none) {
+    Columns c{};
+    if (none || have <= 0) return c;
+    if (a.bias) c.bias = get8n(a.bias, nbase + n, have, a.bias_type);
+    if (a.act == FR_ACT_PRELU) c.slope = get8n(a.slope, nbase + n, have, FR_TYPE_F32);
+    return c;
+}
+FR_DEV void activate(const GemmArgs& a, Vec8f& v, const Columns& c) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v.v[j] += c.bias.v[j];
+    switch (a.act) {
+        case FR_ACT_PRELU: act8c<FR_ACT_PRELU>(v, c.slope); break;
+        case FR_ACT_HSWISH: act8c<FR_ACT_HSWISH>(v, c.slope); break;
+        case FR_ACT_RELU: act8c<FR_ACT_RELU>(v, c.slope); break;
+        case FR_ACT_HSIGMOID: act8c<FR_ACT_HSIGMOID>(v, c.slope); break;
+        case FR_ACT_GELU: act8c<FR_ACT_GELU>(v, c.slope); break;
+        case FR_ACT_SILU: act8c<FR_ACT_SILU>(v, c.slope); break;
+        default: break;
     }
-    if (a.act != FR_ACT_NONE) {
-        Vec8f s{};
-        if (a.act == FR_ACT_PRELU) s = get8n(a.slope, nbase + n0, n, FR_TYPE_F32);
+}
+// Eight outputs n .. n+7 (as many as N has) of row `row`; `none`: of a slot without an expert, zeros.
+FR_DEV void finish8(const GemmArgs& a, long row, int n, const Columns& c, Vec8f v, bool none) {
+    const int have = min(8, a.N - n);
+    if (have <= 0) return;
+    if (!none) {
+        activate(a, v, c);
+        if (a.res) {
+            const Vec8f r = get8n(a.res, row * a.ldr + n, have, a.res_type);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v.v[j] = adapter_act(v.v[j], a.act, s.v[j]);
+            for (int j = 0; j < 8; ++j) v.v[j] += r.v[j];
+        }
     }
-    if (a.res) {
-        const Vec8f r = get8n(a.res, row * a.ldr + n0, n, a.res_type);
+    put8n(a.out, row * a.N + n, have, a.out_type, v);
+}
+// The same for IT rows RPI apart, from position p0, their sums in LDS `PITCH` bytes a row apart; four rows at a time.
+template <int RPI, int IT, int PITCH>
+FR_DEV void finish_rows(const GemmArgs& a, long p0, long r1, int n, int have, const Columns& c, const unsigned char* at, bool none) {
+    constexpr int Q = IT < 4 ? IT : 4;
+#pragma unroll 1
+    for (int k = 0; k < IT; k += Q) {
+        if (p0 + k * RPI >= r1) break;
+        long row[Q];
+        Raw8 res[Q];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v.v[j] += r.v[j];
-    }
-    const long o = row * a.N + n0;
-    if (n == 8) store8t<false>(a.out, o, a.out_type, v);
-    else {
+        for (int e = 0; e < Q; ++e) {
+            const long p = p0 + (k + e) * RPI;
+            row[e] = p < r1 ? out_row(a, p) : -1;
+            if (a.res && have == 8) res[e] = raw_load8<false>(a.res, max(row[e], 0l) * a.ldr + n, a.res_type);
+        }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) if (j < n) store1(a.out, o + j, a.out_type, v.v[j]);
+        for (int e = 0; e < Q; ++e) {
+            Vec8f v;
+            const f32x4 lo = *reinterpret_cast<const f32x4*>(at + (k + e) * RPI * PITCH), hi = *reinterpret_cast<const f32x4*>(at + (k + e) * RPI * PITCH + 16);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { v.v[j] = lo[j]; v.v[4 + j] = hi[j]; }
+            if (row[e] < 0) continue;
+            if (!none) {
+                activate(a, v, c);
+                if (a.res) {
+                    const Vec8f r = have == 8 ? raw_to_f(res[e], a.res_type) : get8n(a.res, row[e] * a.ldr + n, have, a.res_type);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v.v[j] += r.v[j];
+                }
+            }
+            put8n(a.out, row[e] * a.N + n, have, a.out_type, v);
+        }
     }
 }
 
@@ -134,6 +189,193 @@ FR_DEV u32x4 chunk_at(const unsigned char* row, long at, long len) {
     for (int j = 0; j < 8; ++j)
         if (at + 2 * j < len) c.h[j] = *reinterpret_cast<const unsigned short*>(row + at + 2 * j);
     return c.v;
+}
+
+// ---- the staged kernel --------------------------------------------------------------------------------------------------
+typedef __attribute__((address_space(3))) void* lds_ptr_t;
+typedef const __attribute__((address_space(1))) void* glb_ptr_t;
+__device__ const u32x4 g_zero16 = {0, 0, 0, 0};            // source of the pieces behind a row's end
+
+// s_waitcnt as the compiler knows it (its own waits take it into account): at most VM vector loads and LGKM LDS reads open.
+template <int VM, int LGKM> FR_DEV void wait_counts() {
+    __builtin_amdgcn_s_waitcnt((VM & 15) | (7 << 4) | (LGKM << 8) | ((VM >> 4) << 14));
+    asm volatile("" ::: "memory");
+}
+FR_DEV void block_barrier() {                              // without the waits of __syncthreads
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// LDS written by other lanes of this wave is read behind it (a wave's LDS accesses are carried out in order).
+FR_DEV void wave_lds_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); __builtin_amdgcn_wave_barrier(); }
+
+// Number of row tiles of all experts and of the slots without one.
+FR_DEV int expert_tiles(const GemmArgs& a, int bm) {
+    const int lane = threadIdx.x & 63, P = (int)a.M;
+    int n = 0;
+    for (int e = lane; e <= a.E; e += 64) {
+        const int lo = min(max(a.offsets[e], 0), P);
+        const int hi = e < a.E ? min(max(a.offsets[e + 1], lo), P) : P;
+        n += (hi - lo + bm - 1) / bm;
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
+    return __builtin_amdgcn_readfirstlane(n);
+}
+
+// Block -> output tile.  Blocks go to the 8 XCDs in turn and each XCD has its own L2: a contiguous run of tiles for each,
+// walked in groups of 4 row tiles by every n tile, so that the blocks of an XCD that run at the same time share their operands
+// (groups of 8: 4 % slower at 16384 x 2048 x 8192, equal at 8192 cubed; of 16: 15 % slower there).
+FR_DEV void tile_of_block(int block, int mtiles, int ntiles, int& mt, int& nt) {
+    const int total = mtiles * ntiles, xcd = block & 7, q = total >> 3, r = total & 7;
+    const int t = xcd * q + min(xcd, r) + (block >> 3);
+    const int per = 4 * ntiles, g = t / per, in = t - g * per, rows = min(4, mtiles - g * 4);
+    nt = in / rows;
+    mt = g * 4 + (in - nt * rows);
+}
+
+// BM x BN outputs a block of WM x WN waves; slices of 128 bytes of K through a ring of ST buffers in LDS, brought by LDS-DMA
+// (16 bytes a lane, 8 rows an instruction: whole lines of 128 bytes; with rows of 64 bytes the DMA alone was slower, 24
+// against 43 bytes a clock and CU).  Rows are 16-byte aligned whole chunks.  LDS row r keeps its piece p at
+// p ^ ((r >> 1) & 7), so that the 16 rows of a fragment read fall on 16 different bank groups.
+// A slice is two halves of 64 bytes, their fragments in two register sets: while one set is multiplied the other is read.
+// The one barrier of a slice stands between its halves: there its last fragments have been read and the next slice has
+// landed, and behind it the DMA of slice s + ST goes into its buffer, spread over the second half's products (in one
+// burst it held up the waves that issue it).
+template <typename T, int BM, int BN, int WM, int WN, int ST>
+__global__ __launch_bounds__(64 * WM * WN, 2) void gemm_tile_kernel(GemmArgs a) {
+    constexpr int NW = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16, XB = BM * 128, BUF = (BM + BN) * 128;
+    constexpr int XI = BM / 8 / NW, WI = BN / 8 / NW, DMA = XI + WI, DPG = DMA / TM;     // DMA instructions a wave and slice
+    static_assert(XI == WI && DMA % TM == 0 && TN <= TM && NW % 2 == 0, "the interleaving below");
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int li = lane & 15, lg = lane >> 4, wm = wave / WN, wn = wave % WN;
+    int mtiles = (int)((a.M + BM - 1) / BM), mt, nt, expert = 0;
+    if (a.order) mtiles = expert_tiles(a, BM);
+    if ((int)blockIdx.x >= mtiles * a.n_tiles) return;
+    tile_of_block(blockIdx.x, mtiles, a.n_tiles, mt, nt);
+    long r0 = (long)mt * BM, r1 = min(r0 + BM, a.M);
+    if (a.order && !expert_tile(a, mt, BM, expert, r0, r1)) return;
+    const bool none = a.order && expert == a.E;
+    const int n0 = nt * BN;
+    const long nbase = (long)expert * a.N, rowb = (long)a.K * Elem<T>::BYTES;
+    const int full = none ? 0 : (int)(rowb / 128), slices = none ? 0 : (int)((rowb + 127) / 128);
+
+    // this lane's sources: row 8 (wave + NW j) + lane / 8, chunk (lane % 8) ^ key of the slice, as 32-bit offsets from the
+    // tile's first row (the matrix's where rows are gathered)
+    const int kx = ((lane & 7) ^ (((8 * wave + (lane >> 3)) >> 1) & 7)) * 16;    // the same for every j: NW is even
+    const bool gather = a.order && !a.rows_sorted;
+    const unsigned char* xbase = reinterpret_cast<const unsigned char*>(a.x) + (gather ? 0 : r0 * a.ldx * Elem<T>::BYTES);
+    const unsigned char* wbase = reinterpret_cast<const unsigned char*>(a.w) + (none ? 0 : (nbase + n0) * rowb);
+    unsigned off[DMA];
+#pragma unroll
+    for (int j = 0; j < XI; ++j) {
+        const long p = min(r0 + 8 * (wave + NW * j) + (lane >> 3), r1 - 1);
+        off[2 * j] = (unsigned)((gather ? x_row(a, p) : p - r0) * a.ldx * Elem<T>::BYTES) + kx;
+        off[2 * j + 1] = (unsigned)(min(8 * (wave + NW * j) + (lane >> 3), a.N - 1 - n0) * rowb) + kx;
+    }
+    // instruction d of the slice whose x and w columns start at xs and ws: even d x rows, odd d weight rows
+    auto dma = [&](const unsigned char* xs, const unsigned char* ws, int into, int d) __attribute__((always_inline)) {
+        __builtin_amdgcn_global_load_lds((glb_ptr_t)((d & 1 ? ws : xs) + off[d]), (lds_ptr_t)(smem + into + (d & 1 ? XB : 0) + (wave + NW * (d >> 1)) * 1024), 16, 0, 0);
+    };
+    auto stage = [&](int s, int into) {                      // a whole slice; K may end inside it: chunks behind it come from a zero
+        const unsigned lo = (long)s * 128 + kx >= rowb ? 0u : ~0u;
+        const unsigned long long m = ((unsigned long long)lo << 32) | lo, zero = (unsigned long long)&g_zero16 & ~m;
+#pragma unroll
+        for (int d = 0; d < DMA; ++d) {
+            const unsigned long long u = (unsigned long long)((d & 1 ? wbase : xbase) + (long)s * 128 + off[d]);
+            __builtin_amdgcn_global_load_lds((glb_ptr_t)((u & m) | zero), (lds_ptr_t)(smem + into + (d & 1 ? XB : 0) + (wave + NW * (d >> 1)) * 1024), 16, 0, 0);
+        }
+    };
+
+    // fragments: rows 16 t + li of the wave's part, piece (4 h + lg) ^ key; the key is that of li
+    const int fo = ((lg ^ ((li >> 1) & 7)) << 4) + li * 128;
+    const int xo = wm * TM * 2048 + fo, wo = XB + wn * TN * 2048 + fo;
+    f32x4 acc[TN][TM];
+#pragma unroll
+    for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int j = 0; j < TM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    u32x4 wf[2][TN], xf[2][TM];
+    auto fetch = [&](int from, int h, int q) __attribute__((always_inline)) {    // fragment q of half h: weights, then x
+        if (q < TN) wf[h][q] = *reinterpret_cast<const u32x4*>(smem + from + (wo ^ (h << 6)) + q * 2048);
+        else if (q < TN + TM) xf[h][q - TN] = *reinterpret_cast<const u32x4*>(smem + from + (xo ^ (h << 6)) + (q - TN) * 2048);
+    };
+    constexpr int FPG = TM == 8 ? 2 : TM == 4 ? 3 : 4;       // fragment reads a group of products: done before the last groups
+    static_assert(FPG * TM >= TM + TN, "every fragment has its place");
+    int cur = 0;                                             // offset of slice s's buffer
+    auto slice = [&](int s, bool fast) __attribute__((always_inline)) {
+        wait_counts<63, 0>();                                // the first half's fragments
+#pragma unroll
+        for (int j = 0; j < TM; ++j) {
+#pragma unroll
+            for (int q = 0; q < FPG; ++q) fetch(cur, 1, j * FPG + q);
+            if constexpr (BM == 256) __builtin_amdgcn_s_setprio(1);    // products before the other waves' reads (2 % there; smaller tiles lose by it)
+#pragma unroll
+            for (int i = 0; i < TN; ++i) Elem<T>::mma(acc[i][j], wf[0][i], xf[0][j]);
+            if constexpr (BM == 256) __builtin_amdgcn_s_setprio(0);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        // all but the DMA of the last ST - 2 slices asked for has landed (near the end: all of it), fragments are read
+        if (fast || s + ST - 1 < slices) wait_counts<DMA * (ST - 2), 0>();
+        else wait_counts<0, 0>();
+        block_barrier();
+        if (!fast && s + ST < slices) stage(s + ST, cur);
+        const unsigned char *xs = xbase + (long)(s + ST) * 128, *ws = wbase + (long)(s + ST) * 128;
+        asm("" : "+s"(xs), "+s"(ws));                        // scalar bases: the lanes add their 32-bit offsets
+        const int free = cur;
+        cur = cur + BUF == ST * BUF ? 0 : cur + BUF;
+#pragma unroll
+        for (int j = 0; j < TM; ++j) {
+#pragma unroll
+            for (int q = 0; q < FPG; ++q) fetch(cur, 0, j * FPG + q);      // behind the last slice: whatever that buffer holds, unused
+            if (fast)
+#pragma unroll
+                for (int d = 0; d < DPG; ++d) dma(xs, ws, free, j * DPG + d);
+            if constexpr (BM == 256) __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+            for (int i = 0; i < TN; ++i) Elem<T>::mma(acc[i][j], wf[1][i], xf[1][j]);
+            if constexpr (BM == 256) __builtin_amdgcn_s_setprio(0);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    if (slices) {
+        for (int s = 0; s < ST && s < slices; ++s) stage(s, s * BUF);
+        if (slices >= ST) wait_counts<DMA * (ST - 1), 15>();
+        else wait_counts<0, 15>();
+        block_barrier();
+#pragma unroll
+        for (int q = 0; q < TM + TN; ++q) fetch(0, 0, q);
+        int s = 0;
+        for (; s + ST < full; ++s) slice(s, true);
+        for (; s < slices; ++s) slice(s, false);
+    }
+
+    // epilogue: up to 64 x 64 of the wave's outputs at a time through its part of LDS (rows 16 bytes more than a multiple of
+    // 128: writes of 16 rows fall on different banks), then 8 outputs a lane, whole lines.  A lane keeps its columns, so bias
+    // and slopes are loaded once; residuals of four rows are asked for together.
+    constexpr int EM = TM < 4 ? TM : 4, EN = TN < 4 ? TN : 4, PITCH = EN * 64 + 16, LPR = EN * 2, RPI = 64 / LPR, IT = EM * 16 / RPI;
+    unsigned char* part = smem + wave * EM * 16 * PITCH;
+    __syncthreads();                                         // the ring is read
+#pragma unroll
+    for (int q = 0; q < TN / EN; ++q) {
+        const int n = n0 + (wn * TN + EN * q) * 16 + (lane % LPR) * 8, have = min(8, a.N - n);
+        const Columns col = columns(a, n, have, nbase, none);
+#pragma unroll
+        for (int u = 0; u < TM / EM; ++u) {
+#pragma unroll
+            for (int j = 0; j < EM; ++j)
+#pragma unroll
+                for (int i = 0; i < EN; ++i) *reinterpret_cast<f32x4*>(part + (16 * j + li) * PITCH + i * 64 + lg * 16) = acc[EN * q + i][EM * u + j];
+            wave_lds_fence();
+            const long p0 = r0 + (wm * TM + EM * u) * 16 + lane / LPR;
+            const unsigned char* at = part + (lane / LPR) * PITCH + (lane % LPR) * 32;
+            if (have > 0) finish_rows<RPI, IT, PITCH>(a, p0, r1, n, have, col, at, none);
+            wave_lds_fence();
+        }
+    }
 }
 
 // Any shape, any alignment: 64 x 64 outputs a block, 4 waves of 32 x 32, slices of 128 bytes of K through registers into
@@ -211,14 +453,48 @@ __global__ __launch_bounds__(256) void gemm_any_kernel(GemmArgs a) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) { v.v[r] = acc[0][j][r]; v.v[4 + r] = acc[1][j][r]; }
         const int n = n0 + wn * 32 + lg * 8;
-        if (none) {
-            for (int q = 0; q < 8; ++q) if (n + q < a.N) store1(a.out, row * a.N + n + q, a.out_type, 0.f);
-        } else finish8(a, row, n, nbase, v);
+        finish8(a, row, n, columns(a, n, min(8, a.N - n), nbase, none), v, none);
     }
+}
+
+template <typename T, int BM, int BN, int WM, int WN, int ST>
+int launch_tile(GemmArgs a, hipStream_t st) {
+    const long mt = a.order ? a.M / BM + std::min<long>(a.M, a.E + 1) : (a.M + BM - 1) / BM;
+    a.n_tiles = (a.N + BN - 1) / BN;
+    if (mt * a.n_tiles > 0x7FFFFFFFll) FR_FAIL(FR_ERR_UNSUPPORTED, "adapter product: more than 2^31 output tiles");
+    const int lds = std::max(ST * (BM + BN) * 128, WM * WN * std::min(64, BM / WM) * (std::min(64, BN / WN) * 4 + 16));    // the ring; the epilogue's rows
+    FR_BIG_LDS_ONCE((gemm_tile_kernel<T, BM, BN, WM, WN, ST>), lds);
+    hipLaunchKernelGGL((gemm_tile_kernel<T, BM, BN, WM, WN, ST>), dim3((unsigned)(mt * a.n_tiles)), dim3(64 * WM * WN), lds, st, a);
+    FR_LAUNCH_CHECK("gemm_tile_kernel");
+    return FR_OK;
+}
+
+// Time of a slice of 128 bytes of K with as many tiles on the fullest CU as this shape gives it, in us, measured on one
+// card: 256-tiles one after the other, 128-tiles two, 64-tiles three at a time; a tile alone on its CU waits for memory.
+// fp32 is bound by its matrix instructions whatever the tile: there only the rounding to whole tiles differs.
+template <typename T, int B>
+double slice_cost(const GemmArgs& a) {
+    const double rows = a.order ? (double)a.M / B + 0.5 * std::min<long>(a.M, a.E) : (double)((a.M + B - 1) / B);
+    const double on_cu = ceil(rows * ((a.N + B - 1) / B) / 256.0);
+    constexpr bool f32 = std::is_same<T, float>::value;
+    const double alone = B == 256 ? (f32 ? 6.8 : 1.33) : B == 128 ? (f32 ? 1.9 : 0.75) : (f32 ? 0.6 : 0.32);
+    const double each = B == 256 ? (f32 ? 6.8 : 1.55) : B == 128 ? (f32 ? 1.72 : 0.475) : (f32 ? 0.44 : 0.19);
+    return on_cu <= 1 ? alone : std::max(alone, on_cu * each);
 }
 
 template <typename T>
 int launch_gemm(GemmArgs a, hipStream_t st) {
+    const long rowb = (long)a.K * Elem<T>::BYTES, ldxb = a.ldx * Elem<T>::BYTES;
+    const bool gather = a.order && !a.rows_sorted;
+    const bool whole = rowb % 16 == 0 && ldxb % 16 == 0 && ((uintptr_t)a.x & 15) == 0 && ((uintptr_t)a.w & 15) == 0;
+    // the staged kernel adds 32-bit offsets to its tile's (gathered rows: the matrix's) first row
+    const bool near = std::max(rowb, ldxb) < (1l << 23) && (!gather || a.M / a.k * ldxb < (1l << 32));
+    if (whole && near) {
+        const double c256 = slice_cost<T, 256>(a), c128 = slice_cost<T, 128>(a), c64 = slice_cost<T, 64>(a);
+        if (c256 <= c128 && c256 <= c64) return launch_tile<T, 256, 256, 2, 4, 2>(a, st);
+        if (c128 <= c64) return launch_tile<T, 128, 128, 2, 2, 2>(a, st);
+        return launch_tile<T, 64, 64, 2, 2, 3>(a, st);
+    }
     const long mt = a.order ? a.M / 64 + std::min<long>(a.M, a.E + 1) : (a.M + 63) / 64;
     a.n_tiles = (a.N + 63) / 64;
     if (mt * a.n_tiles > 0x7FFFFFFFll) FR_FAIL(FR_ERR_UNSUPPORTED, "adapter product: more than 2^31 output tiles");

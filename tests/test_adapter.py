@@ -310,8 +310,11 @@ def test_linear_extremes_of_activations():
     w = torch.ones(1, 1, device="cuda")
     for act in ("hswish", "relu", "hsigmoid", "gelu", "silu"):
         want = oa.act(x, act)
-        # expf(y) is off by U of y's rounding times |y| <= 88 in its exponent: 100 U covers it; erfcf the same way, of v^2 / 2
-        close(adapter.linear(x, w, act=act), want, 200 * U * want.abs() + 2.0 ** -126, act)
+        # exp2(y) is off by U of y's rounding times |y| <= 128 in its exponent (89 U), and that of v^2 by as much again: 200 U
+        # covers both.  e^88.73 is the last in f32's range: below that SiLU is 0 where |v| e^v < 88.73 * 2^-128 < 2^-121.
+        close(adapter.linear(x, w, act=act), want, 200 * U * want.abs() + 2.0 ** -121, act)
+        ends = torch.tensor([math.inf, -math.inf, math.nan], device="cuda")[:, None]
+        close(adapter.linear(ends, w, act=act), oa.act(ends, act), torch.zeros((), dtype=torch.float64, device="cuda"), act)
 
 
 @pytest.mark.gpu
