@@ -1,5 +1,6 @@
 // Routing of rows to experts: scores, balance bias, group limit, the best k, weights, and the slots sorted by expert.
-// Three launches: choose (and count a chunk's slots per expert), scan the chunks' counts, place every slot.
+// Three launches: choose (and count a chunk's slots per expert), scan the chunks' counts, place every slot; one for up to
+// 64 rows, a single chunk.
 #include "adapter.h"
 
 namespace {
@@ -11,191 +12,196 @@ constexpr int RT_EMAX = 512, RT_KMAX = 16;
 struct RouteArgs {
     const void* logits; const float* bias;
     float* weights; int* experts; int* order; int* offsets;
-    int* counts;                         // [chunks][E + 1]: slots of a chunk per expert (E: none), then their first places
+    int* counts;                         // [E + 1][chunks]: slots of a chunk per expert (E: none), then those of earlier chunks
     int* totals;                         // [E + 1]
     long T;
     int type, E, k, score, groups, top_groups, renormalise, chunks;
     float scale;
 };
 
-template <typename V>
-FR_DEV void best_of_wave(V& key, int& idx) {                 // greatest key, ties to the lower index, in every lane
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const V k2 = __shfl_xor(key, o, 64);
-        const int i2 = __shfl_xor(idx, o, 64);
-        if (k2 > key || (k2 == key && i2 < idx)) { key = k2; idx = i2; }
-    }
-}
-
-FR_DEV float wave_sum_k(float v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-    return v;
-}
-
 // LDS written by other lanes of this wave is read behind it.
 FR_DEV void wave_lds_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); __builtin_amdgcn_wave_barrier(); }
 
-// One row per wave at a time; lane l holds experts l, l + 64, ...  Keys are doubles: exact scores differ by less than a
-// float's step often enough to matter, and their order is what the choice is.
+// ---- sums and maxima over the LPR lanes of a row, in every lane of it (all lanes of the wave take part) -----------------
+template <int CTRL> FR_DEV unsigned dpp(unsigned v) { return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true); }
+template <int LPR, typename F>
+FR_DEV unsigned row_fold(unsigned v, F f) {
+    v = f(v, dpp<0xB1>(v));                                  // lane ^ 1, lane ^ 2, the other half of 8, of 16
+    v = f(v, dpp<0x4E>(v));
+    v = f(v, dpp<0x141>(v));
+    if constexpr (LPR >= 16) v = f(v, dpp<0x140>(v));
+    if constexpr (LPR >= 32) v = f(v, (unsigned)__shfl_xor((int)v, 16, 64));
+    if constexpr (LPR >= 64) v = f(v, (unsigned)__shfl_xor((int)v, 32, 64));
+    return v;
+}
+template <int LPR> FR_DEV unsigned row_maxu(unsigned v) { return row_fold<LPR>(v, [](unsigned x, unsigned y) { return max(x, y); }); }
+template <int LPR> FR_DEV float row_max(float v) {
+    return __uint_as_float(row_fold<LPR>(__float_as_uint(v), [](unsigned x, unsigned y) { return __float_as_uint(fmaxf(__uint_as_float(x), __uint_as_float(y))); }));
+}
+template <int LPR> FR_DEV float row_sum(float v) {
+    return __uint_as_float(row_fold<LPR>(__float_as_uint(v), [](unsigned x, unsigned y) { return __float_as_uint(__uint_as_float(x) + __uint_as_float(y)); }));
+}
+
+// The weight of a chosen expert with logit l, `top` the greatest chosen logit, m and z the row's greatest and its sum of
+// exp(l - m).  What renormalising divides by comes after.
+FR_DEV float raw_weight(const RouteArgs& a, float l, float top, float m, float z) {
+    if (a.score == FR_SCORE_SOFTMAX) {
+        const float against = a.renormalise ? top : m;
+        const float w = l == against ? 1.f : expf(l - against);
+        return a.renormalise ? w : w / z;
+    }
+    if (a.renormalise && top < -20.f) return expf(l - top);  // sigmoid(l) = e^l to 2e-9 there
+    return 1.f / (1.f + expf(-l));
+}
+
+FR_DEV double dpp_step(double v, int ctrl) {                // ctrl is a constant at every call
+    const unsigned long long u = __builtin_bit_cast(unsigned long long, v);
+    unsigned lo, hi;
+    switch (ctrl) {
+        case 0: lo = dpp<0xB1>((unsigned)u); hi = dpp<0xB1>((unsigned)(u >> 32)); break;
+        case 1: lo = dpp<0x4E>((unsigned)u); hi = dpp<0x4E>((unsigned)(u >> 32)); break;
+        case 2: lo = dpp<0x141>((unsigned)u); hi = dpp<0x141>((unsigned)(u >> 32)); break;
+        default: lo = dpp<0x140>((unsigned)u); hi = dpp<0x140>((unsigned)(u >> 32)); break;
+    }
+    return __builtin_bit_cast(double, ((unsigned long long)hi << 32) | lo);
+}
+FR_DEV double lane_of(double v, int lane) {
+    const unsigned long long u = __builtin_bit_cast(unsigned long long, v);
+    const unsigned lo = (unsigned)__builtin_amdgcn_readlane((int)(unsigned)u, lane), hi = (unsigned)__builtin_amdgcn_readlane((int)(unsigned)(u >> 32), lane);
+    return __builtin_bit_cast(double, ((unsigned long long)hi << 32) | lo);
+}
+FR_DEV double wave_max(double v) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v = fmax(v, dpp_step(v, i));
+    return fmax(fmax(lane_of(v, 0), lane_of(v, 16)), fmax(lane_of(v, 32), lane_of(v, 48)));
+}
+FR_DEV double wave_sum(double v) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v += dpp_step(v, i);
+    return (lane_of(v, 0) + lane_of(v, 16)) + (lane_of(v, 32) + lane_of(v, 48));
+}
+FR_DEV unsigned wave_minu(unsigned v) {
+    v = row_fold<16>(v, [](unsigned x, unsigned y) { return min(x, y); });
+    const unsigned a = (unsigned)__builtin_amdgcn_readlane((int)v, 0), b = (unsigned)__builtin_amdgcn_readlane((int)v, 16),
+                   c = (unsigned)__builtin_amdgcn_readlane((int)v, 32), d = (unsigned)__builtin_amdgcn_readlane((int)v, 48);
+    return min(min(a, b), min(c, d));
+}
+
+// One row by a whole wave, decided in doubles: lane l holds experts l, l + 64, ...  Lane j < k returns the j-th choice
+// (-1: none) and its weight.  Few rows come here, but a wave that has one holds up its block, and its time is that of fetching
+// code that no wave nearby has run, then of the chain of dependent steps: loops stay rolled, maxima take DPP steps.
+// (Unrolled over the experts, or with LDS shuffles for every step of a maximum, a row took 30 to 40 us.)
 template <int NE>
-__global__ __launch_bounds__(64 * RT_WAVES) void route_choose_kernel(RouteArgs a) {
-    __shared__ int count[RT_EMAX + 1];
-    __shared__ double keys[RT_WAVES][NE * 64];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    for (int e = threadIdx.x; e <= a.E; e += blockDim.x) count[e] = 0;
-    __syncthreads();
+FR_DEV void choose_exact(const RouteArgs& a, long row, double* keys, int& mine, float& weight) {
+    const int lane = threadIdx.x & 63;
     const double NONE = -INFINITY;
-    const bool scored = a.bias != nullptr || a.groups > 1;
-    for (int r = wave; r < RT_ROWS; r += RT_WAVES) {
-        const long row = (long)blockIdx.x * RT_ROWS + r;
-        if (row >= a.T) break;
+    const bool scored = a.bias != nullptr || a.groups > 1, soft = a.score == FR_SCORE_SOFTMAX;
+    float m = -INFINITY;
+    {
         float l[NE];
-        double key[NE];
-        float m = -INFINITY;
+#pragma unroll
+        for (int q = 0; q < NE; ++q) l[q] = lane + 64 * q < a.E ? load1(a.logits, row * a.E + lane + 64 * q, a.type) : -INFINITY;
 #pragma unroll
         for (int q = 0; q < NE; ++q) {
-            const int e = lane + 64 * q;
-            l[q] = e < a.E ? load1(a.logits, row * a.E + e, a.type) : -INFINITY;
-            if (!(l[q] > -INFINITY)) l[q] = -INFINITY;       // NaN masks too
+            l[q] = l[q] > -INFINITY ? l[q] : -INFINITY;      // NaN masks too
             m = fmaxf(m, l[q]);
+            keys[lane + 64 * q] = l[q];
         }
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-        float z = 0.f;
-        double z64 = 0.0;
-        if (a.score == FR_SCORE_SOFTMAX) {
-#pragma unroll
-            for (int q = 0; q < NE; ++q) {
-                const double p = l[q] == m ? 1.0 : exp((double)l[q] - (double)m);
-                key[q] = l[q] > -INFINITY ? p : 0.0;
-                z64 += key[q];
+    }
+    m = row_max<64>(m);
+    double z = 0.0;
+    if (scored || soft) {
+#pragma unroll 1
+        for (int e = lane; e < 64 * NE; e += 64) {
+            const double l = keys[e], x = l == (double)m && soft ? 1.0 : exp(soft ? l - (double)m : -l);
+            const double s = !(l > NONE) ? 0.0 : soft ? x : 1.0 / (1.0 + x);
+            z += s;
+            if (scored) keys[e] = l > NONE ? s : NONE;
+        }
+        if (soft) z = wave_sum(z);
+    }
+    if (scored) {
+        const double rz = soft ? z : 1.0;
+#pragma unroll 1
+        for (int e = lane; e < a.E; e += 64) {
+            const float b = a.bias ? a.bias[e] : 0.f;
+            const double s = keys[e];
+            keys[e] = s > NONE && b > -INFINITY ? s / rz + (double)b : NONE;
+        }
+    }
+    wave_lds_fence();
+    if (a.groups > 1) {
+        // 64 / groups lanes a group, each its part of it; the first of them joins the parts
+        const int per = a.E / a.groups, n = 64 / a.groups, g = lane / n;
+        double b1 = NONE, b2 = NONE;
+        if (g < a.groups) {
+#pragma unroll 1
+            for (int i = lane - g * n; i < per; i += n) {
+                const double v = keys[g * per + i];
+                b2 = fmax(b2, fmin(b1, v));
+                b1 = fmax(b1, v);
             }
-#pragma unroll
-            for (int o = 32; o > 0; o >>= 1) z64 += __shfl_xor(z64, o, 64);
-            z = (float)z64;
         }
+        double g1 = b1, g2 = b2;
+#pragma unroll 1
+        for (int p = 1; p < n; ++p) {
+            const double o1 = __shfl(b1, (lane + p) & 63, 64), o2 = __shfl(b2, (lane + p) & 63, 64);
+            g2 = fmax(fmin(g1, o1), fmax(g2, o2));
+            g1 = fmax(g1, o1);
+        }
+        const double sum = per > 1 ? g1 + g2 : g1;           // right in the first lane of each group
+        int rank = 0;
+#pragma unroll 1
+        for (int o = 0; o < a.groups; ++o) {
+            const double v = lane_of(sum, o * n);
+            if (v > sum || (v == sum && o < g)) ++rank;
+        }
+        const bool drop = g < a.groups && __shfl(rank, g * n, 64) >= a.top_groups;
+        if (drop) {
+#pragma unroll 1
+            for (int i = lane - g * n; i < per; i += n) keys[g * per + i] = NONE;
+        }
+        wave_lds_fence();
+    }
+    mine = -1;
+#pragma unroll 1
+    for (int j = 0; j < a.k; ++j) {
+        double own = NONE;
+        unsigned at = RT_EMAX;
 #pragma unroll
         for (int q = 0; q < NE; ++q) {
-            const int e = lane + 64 * q;
-            if (!scored) key[q] = l[q];
-            else {
-                const double s = a.score == FR_SCORE_SOFTMAX ? key[q] / z64 : 1.0 / (1.0 + exp(-(double)l[q]));
-                const float b = a.bias && e < a.E ? a.bias[e] : 0.f;
-                key[q] = l[q] > -INFINITY && b > -INFINITY ? s + (double)b : NONE;
-            }
+            const double v = keys[lane + 64 * q];
+            if (v > own) { own = v; at = lane + 64 * q; }
         }
-        if (a.groups > 1) {
-            const int per = a.E / a.groups;
-#pragma unroll
-            for (int q = 0; q < NE; ++q) keys[wave][lane + 64 * q] = key[q];
-            wave_lds_fence();
-            double g = NONE;
-            if (lane < a.groups) {
-                double b1 = NONE, b2 = NONE;
-                for (int i = 0; i < per; ++i) {
-                    const double v = keys[wave][lane * per + i];
-                    if (v > b1) { b2 = b1; b1 = v; } else if (v > b2) b2 = v;
-                }
-                g = per > 1 ? b1 + b2 : b1;
-            }
-            wave_lds_fence();
-            int rank = 0;
-            for (int o = 0; o < a.groups; ++o) {
-                const double v = __shfl(g, o, 64);
-                if (v > g || (v == g && o < lane)) ++rank;
-            }
-            const unsigned long long keep = __ballot(lane < a.groups && rank < a.top_groups);
-#pragma unroll
-            for (int q = 0; q < NE; ++q) {
-                const int e = lane + 64 * q;
-                if (e >= a.E || !((keep >> (e / per)) & 1)) key[q] = NONE;
-            }
-        }
-        int mine = -1;                                       // lane j < k: the j-th choice
-        float mine_l = -INFINITY;
-        for (int j = 0; j < a.k; ++j) {
-            double b = NONE;
-            int bi = RT_EMAX;
-            float bl = -INFINITY;
-#pragma unroll
-            for (int q = 0; q < NE; ++q)
-                if (key[q] > b) { b = key[q]; bi = lane + 64 * q; }
-            best_of_wave(b, bi);
-            if (b == NONE) break;
-#pragma unroll
-            for (int q = 0; q < NE; ++q)
-                if (lane + 64 * q == bi) { key[q] = NONE; bl = l[q]; }
-            bl = __shfl(bl, bi & 63, 64);
-            if (lane == j) { mine = bi; mine_l = bl; }
-        }
-        float top = mine_l;
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-        float w = 0.f;
-        if (mine >= 0) {
-            if (a.score == FR_SCORE_SOFTMAX) {
-                const float against = a.renormalise ? top : m;
-                w = mine_l == against ? 1.f : expf(mine_l - against);
-                if (!a.renormalise) w /= z;
-            } else if (a.renormalise && top < -20.f) w = expf(mine_l - top);   // sigmoid(l) = e^l to 2e-9 there
-            else w = 1.f / (1.f + expf(-mine_l));
-        }
-        if (a.renormalise) {
-            const float sum = wave_sum_k(w);
-            if (sum > 0.f) w /= sum;
-        }
-        if (lane < a.k) {
-            a.weights[row * a.k + lane] = w * a.scale;
-            a.experts[row * a.k + lane] = mine;
-            atomicAdd(&count[mine >= 0 ? mine : a.E], 1);     // whole numbers: any order gives the same
-        }
+        const double best = wave_max(own);
+        if (best == NONE) break;
+        at = wave_minu(own == best ? at : RT_EMAX);
+        if (lane == (int)(at & 63)) keys[at] = NONE;
+        if (lane == j) mine = (int)at;
+        wave_lds_fence();
     }
-    __syncthreads();
-    for (int e = threadIdx.x; e <= a.E; e += blockDim.x) a.counts[(long)blockIdx.x * (a.E + 1) + e] = count[e];
+    const float mine_l = mine >= 0 ? load1(a.logits, row * a.E + mine, a.type) : -INFINITY, top = row_max<64>(mine_l);
+    weight = mine >= 0 ? raw_weight(a, mine_l, top, m, (float)z) : 0.f;
+    if (a.renormalise) {
+        const float sum = row_sum<64>(weight);
+        if (sum > 0.f) weight /= sum;
+    }
+    weight *= a.scale;
+    wave_lds_fence();
 }
 
-// counts[c][e] -> number of e's slots in the chunks before c; totals[e].  One wave per expert.
-__global__ __launch_bounds__(64) void route_scan_kernel(RouteArgs a) {
-    const int e = blockIdx.x, lane = threadIdx.x;
-    int before = 0;
-    for (int c0 = 0; c0 < a.chunks; c0 += 64) {
-        const int c = c0 + lane;
-        const int n = c < a.chunks ? a.counts[(long)c * (a.E + 1) + e] : 0;
-        int s = n;
+// Places of one chunk's slots, by one wave: next[e] is the place of expert e's first slot here (E: none).  Equal experts
+// among 64 slots find each other by the bits of their number.
+FR_DEV void place_slots(const RouteArgs& a, int* next, const int* experts, int n, long slot0) {
+    const int lane = threadIdx.x & 63;
+    int ex[RT_KMAX];                                         // 64 rows * k slots: k a lane, all asked for before the first is used
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) { const int t = __shfl_up(s, o, 64); if (lane >= o) s += t; }
-        if (c < a.chunks) a.counts[(long)c * (a.E + 1) + e] = before + s - n;
-        before += __shfl(s, 63, 64);
-    }
-    if (lane == 0) a.totals[e] = before;
-}
-
-// Places of a chunk's slots: first place of the expert + its slots in earlier chunks + earlier in this chunk.
-__global__ __launch_bounds__(64) void route_place_kernel(RouteArgs a) {
-    __shared__ int next[RT_EMAX + 1];
-    const int lane = threadIdx.x;
-    int before = 0;
-    for (int e0 = 0; e0 <= a.E; e0 += 64) {
-        const int e = e0 + lane;
-        const int n = e <= a.E ? a.totals[e] : 0;
-        int s = n;
+    for (int j = 0; j < RT_KMAX; ++j) ex[j] = j * 64 + lane < n ? experts[j * 64 + lane] : 0;
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) { const int t = __shfl_up(s, o, 64); if (lane >= o) s += t; }
-        if (e <= a.E) {
-            next[e] = before + s - n + (a.chunks ? a.counts[(long)blockIdx.x * (a.E + 1) + e] : 0);
-            if (blockIdx.x == 0) a.offsets[e] = before + s - n;
-        }
-        before += __shfl(s, 63, 64);
-    }
-    __syncthreads();
-    const long s0 = (long)blockIdx.x * RT_ROWS * a.k, s1 = min(s0 + (long)RT_ROWS * a.k, a.T * a.k);
-    for (long b = s0; b < s1; b += 64) {
-        const long s = b + lane;
-        const bool on = s < s1;
-        const int ex = on ? a.experts[s] : -1;
-        const int e = ex < 0 ? a.E : ex;
+    for (int j = 0; j < RT_KMAX; ++j) {
+        if (j * 64 >= n) break;
+        const bool on = j * 64 + lane < n;
+        const int e = ex[j] < 0 ? a.E : ex[j];
         unsigned long long same = __ballot(on);              // lanes with this lane's expert
         for (int bit = 0; (1 << bit) <= a.E; ++bit) {
             const bool set = (e >> bit) & 1;
@@ -203,11 +209,260 @@ __global__ __launch_bounds__(64) void route_place_kernel(RouteArgs a) {
             same &= set ? with : ~with;
         }
         const int rank = __popcll(same & ((1ull << lane) - 1));
-        if (on) a.order[next[e] + rank] = (int)s;
-        __syncthreads();
-        if (on && rank == 0) next[e] += __popcll(same);
-        __syncthreads();
+        int base = 0;
+        if (on) base = next[e];
+        wave_lds_fence();
+        if (on) a.order[base + rank] = (int)(slot0 + j * 64 + lane);
+        if (on && rank == 0) next[e] = base + __popcll(same);
+        wave_lds_fence();
     }
+}
+// next[e] = sum of n[0 .. e) for e <= E, by one wave; n(e) gives a count, also written to a.offsets if `write`.
+template <typename F>
+FR_DEV void first_places(const RouteArgs& a, int* next, bool write, F n) {
+    const int lane = threadIdx.x & 63;
+    int before = 0;
+    for (int e0 = 0; e0 <= a.E; e0 += 64) {
+        const int e = e0 + lane, c = e <= a.E ? n(e) : 0;
+        int s = c;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) { const int t = __shfl_up(s, o, 64); if (lane >= o) s += t; }
+        if (e <= a.E) {
+            next[e] = before + s - c;
+            if (write) a.offsets[e] = before + s - c;
+        }
+        before += __shfl(s, 63, 64);
+    }
+}
+
+// A row takes LPR lanes, a lane up to V experts of one group, in index order over the lanes.  The k best come from k maxima
+// over the row of keys that are unique in their lane: f32 in unsigned order, the low NB bits replaced by an index (greater for lower
+// ones).  Unscored rows (no bias, one group) order by the logits themselves and put the expert's number there: unique in
+// the row, ties need no care, and with 16-bit logits nothing is lost.  Scored rows put the place in the lane there, 4 bits.
+// A row is done again by the whole wave in doubles where f32 cannot vouch for the choice: where two neighbours in the order
+// (or the groups on either side of the cut) are no further apart than the bits dropped and the error of their scores, which
+// is at most 4 steps of 2^-24 for a sigmoid (exp2's argument and result, the sum, the reciprocal) and 32 for a softmax
+// (the row's sum of up to 512 besides).  At 65536 x 256, biased sigmoids, 8 of 256 in 4 of 8 groups, one row in 500 goes
+// that way; with the expert's number in the scored keys too it was one in 50, which took more time than all the rest.
+template <int V, int LPR, int NE, int NB, bool SCORED>
+__global__ __launch_bounds__(64 * RT_WAVES) void route_choose_kernel(RouteArgs a) {
+    __shared__ int count[RT_EMAX + 1];
+    __shared__ int chosen[RT_ROWS * RT_KMAX];
+    __shared__ double keys[RT_WAVES][NE * 64];
+    constexpr unsigned MASK = (1u << NB) - 1;
+    constexpr int RPW = 64 / LPR;
+    constexpr float L2E = 1.4426950408889634f, DROP = 1.f / (float)(1u << (23 - NB));
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, rl = lane % LPR, base = lane - rl;
+    for (int e = threadIdx.x; e <= a.E; e += blockDim.x) count[e] = 0;
+    __syncthreads();
+    static_assert(!SCORED || V <= 1 << NB, "a lane's keys are unique");
+    const bool need_z = SCORED || !a.renormalise;
+    const int per = a.E / a.groups, LG = (per + V - 1) / V, g = rl / LG, part = rl - g * LG;
+    const float slack = a.score == FR_SCORE_SOFTMAX ? 0x1p-18f : 0x1p-21f;
+    const int e0 = g * per + part * V, cnt = g < a.groups ? min(V, per - part * V) : 0;
+    float b[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) b[v] = a.bias && v < cnt ? a.bias[e0 + v] : 0.f;
+#pragma unroll 1
+    for (int it = wave; it * RPW < RT_ROWS; it += RT_WAVES) {
+        const int r = it * RPW + lane / LPR;
+        const long row = (long)blockIdx.x * RT_ROWS + r;
+        const int have = row < a.T ? cnt : 0;
+        float l[V];
+#pragma unroll
+        for (int c = 0; c < V; c += 8) {
+            Vec8f x;
+            if (have - c >= 8) x = raw_to_f(raw_load8<false>(a.logits, row * a.E + e0 + c, a.type), a.type);
+            else {
+#pragma unroll
+                for (int v = 0; v < 8; ++v) x.v[v] = c + v < have ? load1(a.logits, row * a.E + e0 + c + v, a.type) : -INFINITY;
+            }
+#pragma unroll
+            for (int v = 0; v < 8; ++v) l[c + v] = x.v[v] > -INFINITY ? x.v[v] : -INFINITY;      // NaN masks too
+        }
+        float m = 0.f, z = 1.f;
+        if (a.score == FR_SCORE_SOFTMAX && need_z) {
+            m = l[0];
+#pragma unroll
+            for (int v = 1; v < V; ++v) m = fmaxf(m, l[v]);
+            m = row_max<LPR>(m);
+        }
+        float f[V];                                          // keys: logits or scores + bias; -inf: masked
+        if (a.score == FR_SCORE_SOFTMAX && need_z) {
+            z = 0.f;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                f[v] = l[v] == m ? 1.f : __builtin_amdgcn_exp2f((l[v] - m) * L2E);
+                z += l[v] > -INFINITY ? f[v] : 0.f;
+            }
+            z = row_sum<LPR>(z);
+        }
+        if constexpr (SCORED) {
+            const float rz = __builtin_amdgcn_rcpf(z);
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const float s = a.score == FR_SCORE_SOFTMAX ? f[v] * rz : __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-l[v] * L2E));
+                f[v] = l[v] > -INFINITY && b[v] > -INFINITY ? s + b[v] : -INFINITY;
+            }
+        } else {
+#pragma unroll
+            for (int v = 0; v < V; ++v) f[v] = l[v] + 0.f;   // -0 is 0
+        }
+        bool doubt = false, kept = true;
+        if (SCORED && a.groups > 1) {
+            float b1 = -INFINITY, b2 = -INFINITY;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                b2 = __builtin_amdgcn_fmed3f(b1, b2, f[v]);
+                b1 = fmaxf(b1, f[v]);
+            }
+            float g1 = b1, g2 = b2;
+            for (int p = 1; p < LG; ++p) {
+                const int from = base + g * LG + (part + p >= LG ? part + p - LG : part + p);
+                const float o1 = __shfl(b1, from, 64), o2 = __shfl(b2, from, 64);
+                g2 = fmaxf(fminf(g1, o1), fmaxf(g2, o2));
+                g1 = fmaxf(g1, o1);
+            }
+            const float sum = per > 1 ? g1 + g2 : g1;
+            int rank = 0;
+            for (int o = 0; o < a.groups; ++o) {
+                const float v = __shfl(sum, base + o * LG, 64);
+                if (v > sum || (v == sum && o < g)) ++rank;
+            }
+            kept = g < a.groups && rank < a.top_groups;
+            if (a.top_groups < a.groups) {                   // sums of two: twice the error
+                const float least = -row_max<LPR>(kept ? -sum : -INFINITY), most = row_max<LPR>(!kept && g < a.groups ? sum : -INFINITY);
+                doubt = !(least - most > 2.f * slack * fmaxf(1.f, fabsf(least)));
+            }
+        }
+        unsigned key[V];                                     // 0: not to be chosen
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            unsigned u = __float_as_uint(f[v]);
+            u ^= (unsigned)((int)u >> 31) | 0x80000000u;
+            key[v] = kept && f[v] > -INFINITY ? (u & ~MASK) | (MASK - (unsigned)(SCORED ? v : e0 + v)) : 0u;
+        }
+        if (SCORED && a.groups > 1) {                        // a row without any eligible expert needs no second look
+            unsigned live = 0;
+#pragma unroll
+            for (int v = 0; v < V; ++v) live |= f[v] > -INFINITY ? 1u : 0u;
+            doubt = doubt && row_maxu<LPR>(live);
+        }
+        unsigned mine = 0, last = 0;
+        if (SCORED && rl < a.k) chosen[r * a.k + rl] = -1;
+        wave_lds_fence();
+        for (int j = 0; j <= a.k; ++j) {
+            unsigned own = key[0];
+#pragma unroll
+            for (int v = 1; v < V; ++v) own = max(own, key[v]);
+            const unsigned top = row_maxu<LPR>(own);
+            if (j > 0 && top) {
+                const unsigned x = last & ~MASK, y = top & ~MASK;
+                if constexpr (!SCORED) doubt |= a.type == FR_TYPE_F32 && x == y;
+                else {
+                    const float fx = __uint_as_float(x & 0x80000000u ? x ^ 0x80000000u : ~x), fy = __uint_as_float(y & 0x80000000u ? y ^ 0x80000000u : ~y);
+                    doubt |= !(fx - fy > slack * fmaxf(1.f, fabsf(fx)) + 2.f * DROP * fmaxf(fabsf(fx), fabsf(fy)));
+                }
+            }
+            if (j == a.k) break;
+            last = top;
+            if constexpr (SCORED) {
+                const bool here = own == top && top;
+                if (here) chosen[r * a.k + j] = e0 + (int)(MASK - (top & MASK));
+                const unsigned long long who = (__ballot(here) >> base) & (LPR == 64 ? ~0ull : (1ull << (LPR & 63)) - 1);
+                doubt |= __popcll(who) > 1;                  // equal keys of two lanes
+            } else if (rl == j) mine = top;
+#pragma unroll
+            for (int v = 0; v < V; ++v) key[v] = key[v] == top ? 0u : key[v];
+        }
+        // lane j < k of the row: its j-th choice
+        wave_lds_fence();
+        int pick = mine ? (int)(MASK - (mine & MASK)) : -1;
+        if (SCORED) pick = rl < a.k ? chosen[r * a.k + rl] : -1;
+        const float pl = pick >= 0 ? load1(a.logits, row * a.E + pick, a.type) : -INFINITY;
+        const float best = row_max<LPR>(pl);
+        float w = pick >= 0 ? raw_weight(a, pl, best, m, z) : 0.f;
+        if (a.renormalise) {
+            const float sum = row_sum<LPR>(w);
+            if (sum > 0.f) w /= sum;
+        }
+        const bool sure = row < a.T && !doubt;
+        if (sure && rl < a.k) {
+            a.weights[row * a.k + rl] = w * a.scale;
+            a.experts[row * a.k + rl] = pick;
+            chosen[r * a.k + rl] = pick;
+            atomicAdd(&count[pick >= 0 ? pick : a.E], 1);    // whole numbers: any order gives the same
+        }
+        unsigned long long again = __ballot(doubt && row < a.T && rl == 0);
+        while (again) {
+            const int at = __ffsll(again) - 1, rr = it * RPW + at / LPR;
+            again &= again - 1;
+            const long row2 = (long)blockIdx.x * RT_ROWS + rr;
+            int pick2;
+            float w2;
+            choose_exact<NE>(a, row2, keys[wave], pick2, w2);
+            if (lane < a.k) {
+                a.weights[row2 * a.k + lane] = w2;
+                a.experts[row2 * a.k + lane] = pick2;
+                chosen[rr * a.k + lane] = pick2;
+                atomicAdd(&count[pick2 >= 0 ? pick2 : a.E], 1);
+            }
+        }
+    }
+    __syncthreads();
+    if (a.chunks > 1) {
+        for (int e = threadIdx.x; e <= a.E; e += blockDim.x) a.counts[(long)e * a.chunks + blockIdx.x] = count[e];
+    } else if (wave == 0) {                                  // one chunk is all: order it here, one launch in place of three
+        first_places(a, count, true, [&](int e) { return count[e]; });
+        wave_lds_fence();
+        place_slots(a, count, chosen, (int)(a.T * a.k), 0);
+    }
+}
+
+// counts[e][c] -> number of e's slots in the chunks before c; totals[e].  One block per expert, four chunks a thread.
+__global__ __launch_bounds__(256) void route_scan_kernel(RouteArgs a) {
+    __shared__ int part[2][4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int* row = a.counts + (long)blockIdx.x * a.chunks;
+    int before = 0, turn = 0;
+    for (int c0 = 0; c0 < a.chunks; c0 += 1024, ++turn) {
+        const int c = c0 + threadIdx.x * 4;
+        int n[4], t = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { n[j] = c + j < a.chunks ? row[c + j] : 0; t += n[j]; }
+        int s = t;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) { const int u = __shfl_up(s, o, 64); if (lane >= o) s += u; }
+        int* p = part[turn & 1];
+        if (lane == 63) p[wave] = s;
+        __syncthreads();
+        int at = before + s - t;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) { if (w < wave) at += p[w]; before += p[w]; }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (c + j < a.chunks) row[c + j] = at;
+            at += n[j];
+        }
+    }
+    if (threadIdx.x == 0) a.totals[blockIdx.x] = before;
+}
+
+// Places of a chunk's slots: first place of the expert + its slots in earlier chunks + earlier in this chunk.
+__global__ __launch_bounds__(64) void route_place_kernel(RouteArgs a) {
+    __shared__ int next[RT_EMAX + 1];
+    first_places(a, next, blockIdx.x == 0, [&](int e) { return a.totals[e]; });
+    wave_lds_fence();
+    for (int e = threadIdx.x; e <= a.E; e += 64) next[e] += a.counts[(long)e * a.chunks + blockIdx.x];
+    wave_lds_fence();
+    const long s0 = (long)blockIdx.x * RT_ROWS * a.k;
+    place_slots(a, next, a.experts + s0, (int)min((long)RT_ROWS * a.k, a.T * a.k - s0), s0);
+}
+
+template <int V, int LPR, int NE, int NB>
+void launch_choose(const RouteArgs& a, hipStream_t st) {
+    if (a.bias || a.groups > 1) hipLaunchKernelGGL((route_choose_kernel<V, LPR, NE, 4, true>), dim3(a.chunks), dim3(64 * RT_WAVES), 0, st, a);
+    else hipLaunchKernelGGL((route_choose_kernel<V, LPR, NE, NB, false>), dim3(a.chunks), dim3(64 * RT_WAVES), 0, st, a);
 }
 
 }  // namespace
@@ -237,17 +492,20 @@ extern "C" int fr_route(const void* logits, int logits_type, int64_t T, int E, i
     RouteArgs a{logits, bias, weights, experts, order, offsets, (int*)workspace + E + 1, (int*)workspace, T,
                 logits_type, E, k, score, groups, top_groups, renormalise, (int)((T + RT_ROWS - 1) / RT_ROWS), scale};
     hipStream_t st = (hipStream_t)stream;
-    if (a.chunks) {
-        const dim3 grid(a.chunks), block(64 * RT_WAVES);
-        if (E <= 64) hipLaunchKernelGGL((route_choose_kernel<1>), grid, block, 0, st, a);
-        else if (E <= 128) hipLaunchKernelGGL((route_choose_kernel<2>), grid, block, 0, st, a);
-        else if (E <= 256) hipLaunchKernelGGL((route_choose_kernel<4>), grid, block, 0, st, a);
-        else hipLaunchKernelGGL((route_choose_kernel<8>), grid, block, 0, st, a);
-        FR_LAUNCH_CHECK("route_choose_kernel");
+    if (a.chunks == 0) a.chunks = 1;                          // no rows: the offsets are written all the same
+    // lanes a row takes: every group a whole number of them, and one for each of the k choices
+    const int V = E <= 64 && groups == 1 ? 8 : 16, per = E / groups, lanes = std::max(groups * ((per + V - 1) / V), k);
+    if (V == 8 && lanes <= 8) launch_choose<8, 8, 1, 6>(a, st);
+    else if (lanes <= 8 && E <= 128) launch_choose<16, 8, 2, 8>(a, st);
+    else if (lanes <= 16 && E <= 256) launch_choose<16, 16, 4, 8>(a, st);
+    else if (lanes <= 32) launch_choose<16, 32, 8, 9>(a, st);
+    else launch_choose<16, 64, 8, 9>(a, st);
+    FR_LAUNCH_CHECK("route_choose_kernel");
+    if (a.chunks > 1) {
+        hipLaunchKernelGGL(route_scan_kernel, dim3(E + 1), dim3(256), 0, st, a);
+        FR_LAUNCH_CHECK("route_scan_kernel");
+        hipLaunchKernelGGL(route_place_kernel, dim3(a.chunks), dim3(64), 0, st, a);
+        FR_LAUNCH_CHECK("route_place_kernel");
     }
-    hipLaunchKernelGGL(route_scan_kernel, dim3(E + 1), dim3(64), 0, st, a);
-    FR_LAUNCH_CHECK("route_scan_kernel");
-    hipLaunchKernelGGL(route_place_kernel, dim3(std::max(1, a.chunks)), dim3(64), 0, st, a);
-    FR_LAUNCH_CHECK("route_place_kernel");
     return FR_OK;
 }

@@ -18,6 +18,7 @@ call replaces).
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from typing import Dict, Tuple
 
 import torch
@@ -231,12 +232,25 @@ def _ptr(t):
 
 
 def _call(name, dev, *args):
+    """One C-ABI call on the device's current stream.  A call on one row takes a few microseconds on the GPU, so the host's
+    share counts: no Stream object, no device switch where none is needed."""
+    index = dev.index
     fn = getattr(_lib.lib(), name)
-    if torch.cuda.current_device() == dev.index:
-        _lib.check(fn(*args, _stream(dev)), name)
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(dev):
-            _lib.check(fn(*args, _stream(dev)), name)
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        _lib.check(rc, name)
+
+
+@functools.lru_cache(maxsize=1024)
+def _scratch_bytes(name, *shape):
+    """Workspace of a shape, by shape alone (the rules behind it are the library's, fixed for the process)."""
+    need = C.c_size_t()
+    _lib.check(getattr(_lib.lib(), name)(*shape, C.byref(need)), name)
+    return need.value
 
 
 def _rows(t, width):
@@ -254,7 +268,7 @@ def _vector(op, what, t, n, dtypes):
     return t.contiguous()
 
 
-def _linear_shape(op, x, weight, residual, out_dtype):
+def _linear_shape(op, x, weight, residual):
     if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1] or weight.shape[1] < 1 or weight.shape[0] < 1:
         _fail(op, f"expected x [..., K] and weight [N, K]: got {tuple(x.shape)} and {tuple(weight.shape)}")
     shape = x.shape[:-1] + (weight.shape[0],)
@@ -266,7 +280,7 @@ def _linear_shape(op, x, weight, residual, out_dtype):
 def _linear(x, weight, bias, slope, residual, act, out_dtype):
     op = "linear"
     _check_tensors(op, x, weight, bias, slope, residual)
-    shape = _linear_shape(op, x, weight, residual, out_dtype)
+    shape = _linear_shape(op, x, weight, residual)
     N, K = weight.shape
     kind = _type(op, "x", x.dtype)
     if weight.dtype != x.dtype:
@@ -279,18 +293,17 @@ def _linear(x, weight, bias, slope, residual, act, out_dtype):
     out_dtype = x.dtype if out_dtype is None else out_dtype
     out_type = _type(op, "out_dtype", out_dtype)
     res_type = kind if residual is None else _type(op, "residual", residual.dtype)
-    out = torch.empty(shape, dtype=out_dtype, device=x.device)
+    out = x.new_empty(shape, dtype=out_dtype)
     M = out.numel() // N
     if M == 0:
         return out
     x, ldx = _rows(x, K)
     residual, ldr = (None, 0) if residual is None else _rows(residual, N)
     weight = weight.contiguous()
-    need = C.c_size_t()
-    _lib.check(_lib.lib().fr_linear_workspace_bytes(M, N, K, kind, C.byref(need)), "fr_linear_workspace_bytes")
-    ws = torch.empty(need.value, dtype=torch.uint8, device=x.device) if need.value else None
+    need = _scratch_bytes("fr_linear_workspace_bytes", M, N, K, kind)
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
     _call("fr_linear", x.device, x.data_ptr(), ldx, weight.data_ptr(), _ptr(bias), _ptr(slope), _ptr(residual), ldr, out.data_ptr(),
-          M, N, K, kind, kind if bias is None else _TYPES[bias.dtype], res_type, out_type, act, _ptr(ws), need.value)
+          M, N, K, kind, kind if bias is None else _TYPES[bias.dtype], res_type, out_type, act, _ptr(ws), need)
     return out
 
 
@@ -337,8 +350,8 @@ def _block_norm(x, residual, slot_weights, norm, weight, bias, eps, gate, gate_a
         else:
             _fail(op, f"gate is [{d}], {tuple(shape[:-1]) + (1,)} or {tuple(shape)}: got {tuple(gate.shape)}")
     gate_act = _name(op, _GATE_ACTS, gate_act, "gate_act")
-    out = torch.empty(shape, dtype=out_dtype, device=x.device)
-    nxt = torch.empty(shape if next_norm else 0, dtype=next_dtype, device=x.device)
+    out = x.new_empty(shape, dtype=out_dtype)
+    nxt = x.new_empty(shape if next_norm else 0, dtype=next_dtype)
     T = out.numel() // d
     if T == 0:
         return out, nxt
@@ -362,9 +375,9 @@ def _route_shape(op, logits, k):
 
 def _route_empty(logits, k):
     T, E = logits.shape
-    i32 = dict(dtype=torch.int32, device=logits.device)
-    return (torch.empty((T, k), dtype=torch.float32, device=logits.device), torch.empty((T, k), **i32),
-            torch.empty(T * k, **i32), torch.empty(E + 1, **i32))
+    i32 = torch.int32
+    return (logits.new_empty((T, k), dtype=torch.float32), logits.new_empty((T, k), dtype=i32), logits.new_empty(T * k, dtype=i32),
+            logits.new_empty(E + 1, dtype=i32))
 
 
 def _route(logits, k, score, bias, groups, top_groups, renormalise, scale):
@@ -375,13 +388,12 @@ def _route(logits, k, score, bias, groups, top_groups, renormalise, scale):
     score = _name(op, _SCORES, score, "score")
     bias = _vector(op, "bias", bias, E, (torch.float32,))
     logits = logits.contiguous()
-    need = C.c_size_t()
-    _lib.check(_lib.lib().fr_route_workspace_bytes(T, E, k, C.byref(need)), "fr_route_workspace_bytes")
+    need = _scratch_bytes("fr_route_workspace_bytes", T, E, k)
     out = _route_empty(logits, k)
-    ws = torch.empty(need.value, dtype=torch.uint8, device=logits.device)
+    ws = logits.new_empty(need, dtype=torch.uint8)
     weights, experts, order, offsets = (t.data_ptr() or ws.data_ptr() for t in out)      # T = 0: empty tensors have no address
     _call("fr_route", logits.device, logits.data_ptr(), kind, T, E, k, score, _ptr(bias), groups, top_groups, renormalise, scale,
-          weights, experts, order, offsets, ws.data_ptr(), need.value)
+          weights, experts, order, offsets, ws.data_ptr(), need)
     return out
 
 
@@ -420,7 +432,7 @@ def _expert_linear(x, weight, order, offsets, k, bias, act, slope, rows, out, ou
             _fail(op, f"slope is float32 [{E}, {N}]: got {slope.dtype} {tuple(slope.shape)}")
         slope = slope.contiguous()
     out_dtype = x.dtype if out_dtype is None else out_dtype
-    y = torch.empty(shape, dtype=out_dtype, device=x.device)
+    y = x.new_empty(shape, dtype=out_dtype)
     out_type = _type(op, "out_dtype", out_dtype)
     if T == 0:
         return y
@@ -455,7 +467,7 @@ _meta.impl("topk_merge", lambda s, i, k: (s.new_empty((s.shape[1], k), dtype=tor
 
 
 def _meta_linear(x, weight, bias, slope, residual, act, out_dtype):
-    return x.new_empty(_linear_shape("linear", x, weight, residual, out_dtype), dtype=out_dtype or x.dtype)
+    return x.new_empty(_linear_shape("linear", x, weight, residual), dtype=out_dtype or x.dtype)
 
 
 def _meta_block_norm(x, residual, slot_weights, norm, weight, bias, eps, gate, gate_act, scale, next_norm, next_weight, next_bias,
