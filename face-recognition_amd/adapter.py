@@ -26,6 +26,14 @@ import torch
 from . import ops as _ops
 
 
+def _op(name: str, x: torch.Tensor):
+    """The operator for a call on ``x``: its implementation itself for an eager call on a plain tensor (the dispatcher takes
+    as long as the smallest kernels run), ``torch.ops.fr_hip`` for whatever traces or stands in for one."""
+    if (type(x) is torch.Tensor or type(x) is torch.nn.Parameter) and not torch.compiler.is_compiling():
+        return getattr(_ops, "_" + name)
+    return getattr(torch.ops.fr_hip, name)
+
+
 def _need_gpu(x: torch.Tensor, what: str) -> None:
     if not x.is_cuda:
         raise RuntimeError(f"{what} needs GPU tensors: the hot path has no CPU fallback")
@@ -38,7 +46,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     type or f32, residual [..., N] of any of the three.  act: none, prelu (slope f32 [N]), hswish, relu, hsigmoid, gelu
     (erf form), silu.  Accumulation and epilogue in f32, rounded once to ``out_dtype`` (x's type by default)."""
     _need_gpu(x, "linear")
-    return torch.ops.fr_hip.linear(x, weight, bias, slope, residual, act, out_dtype)
+    return _op("linear", x)(x, weight, bias, slope, residual, act, out_dtype)
 
 
 def block_norm(x: torch.Tensor, residual: Optional[torch.Tensor] = None, *, slot_weights: Optional[torch.Tensor] = None,
@@ -53,7 +61,7 @@ def block_norm(x: torch.Tensor, residual: Optional[torch.Tensor] = None, *, slot
     weight / bias f32 [d] for rms and layer.  gate: [d], [..., 1] or [..., d]; gate_act none, sigmoid, tanh.  d <= 16384.
     Returns out, or (out, next)."""
     _need_gpu(x, "block_norm")
-    out, nxt = torch.ops.fr_hip.block_norm(x, residual, slot_weights, norm, weight, bias, eps, gate, gate_act, scale,
+    out, nxt = _op("block_norm", x)(x, residual, slot_weights, norm, weight, bias, eps, gate, gate_act, scale,
                                            next_norm or "none", next_weight, next_bias, next_eps, out_dtype, next_dtype)
     return (out, nxt) if next_norm not in (None, "none") else out
 
@@ -74,7 +82,7 @@ def route(logits: torch.Tensor, k: int, *, score: str = "softmax", bias: Optiona
     ``renormalise``, times ``scale``.  Logits (or biases) that are -inf or NaN mask their expert; a row whose mask leaves
     fewer than k has slots of expert -1 and weight 0.  E <= 512, k <= 16, groups <= 64."""
     _need_gpu(logits, "route")
-    return Routing(*torch.ops.fr_hip.route(logits, k, score, bias, groups, top_groups, renormalise, scale))
+    return Routing(*_op("route", logits)(logits, k, score, bias, groups, top_groups, renormalise, scale))
 
 
 def expert_linear(x: torch.Tensor, weight: torch.Tensor, routing: Routing, bias: Optional[torch.Tensor] = None, *,
@@ -85,7 +93,7 @@ def expert_linear(x: torch.Tensor, weight: torch.Tensor, routing: Routing, bias:
     out="sorted" answers [T * k, N] in those positions, out="slots" [T, k, N] by slot, ready for ``block_norm``'s
     slot_weights.  Slots without an expert get zero rows."""
     _need_gpu(x, "expert_linear")
-    return torch.ops.fr_hip.expert_linear(x, weight, routing.order, routing.offsets, routing.experts.shape[1], bias, act, slope,
+    return _op("expert_linear", x)(x, weight, routing.order, routing.offsets, routing.experts.shape[1], bias, act, slope,
                                           rows, out, out_dtype)
 
 

@@ -20,6 +20,8 @@ struct GemmArgs {
     const int* order; const int* offsets;
     int E, k, rows_sorted, out_slots;
     int n_tiles;
+    int splits, split_slices;            // K in `splits` parts of split_slices slices each, their sums in `partial` [splits][M][N]
+    float* partial;
 };
 
 template <typename T> struct Elem;       // BYTES, mma over one chunk of both operands
@@ -254,27 +256,29 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_tile_kernel(GemmArgs a) 
     const int li = lane & 15, lg = lane >> 4, wm = wave / WN, wn = wave % WN;
     int mtiles = (int)((a.M + BM - 1) / BM), mt, nt, expert = 0;
     if (a.order) mtiles = expert_tiles(a, BM);
-    if ((int)blockIdx.x >= mtiles * a.n_tiles) return;
-    tile_of_block(blockIdx.x, mtiles, a.n_tiles, mt, nt);
+    const int tiles = mtiles * a.n_tiles, split = a.splits > 1 ? blockIdx.x / tiles : 0;
+    if ((int)blockIdx.x - split * tiles >= tiles || split >= a.splits) return;     // experts: the grid is an upper bound
+    tile_of_block(blockIdx.x - split * tiles, mtiles, a.n_tiles, mt, nt);
     long r0 = (long)mt * BM, r1 = min(r0 + BM, a.M);
     if (a.order && !expert_tile(a, mt, BM, expert, r0, r1)) return;
     const bool none = a.order && expert == a.E;
     const int n0 = nt * BN;
-    const long nbase = (long)expert * a.N, rowb = (long)a.K * Elem<T>::BYTES;
+    const long nbase = (long)expert * a.N, pitch = (long)a.K * Elem<T>::BYTES, k0 = (long)split * a.split_slices * 128;
+    const long rowb = a.splits > 1 ? min(pitch - k0, (long)a.split_slices * 128) : pitch;     // bytes of a row in this part of K
     const int full = none ? 0 : (int)(rowb / 128), slices = none ? 0 : (int)((rowb + 127) / 128);
 
     // this lane's sources: row 8 (wave + NW j) + lane / 8, chunk (lane % 8) ^ key of the slice, as 32-bit offsets from the
     // tile's first row (the matrix's where rows are gathered)
     const int kx = ((lane & 7) ^ (((8 * wave + (lane >> 3)) >> 1) & 7)) * 16;    // the same for every j: NW is even
     const bool gather = a.order && !a.rows_sorted;
-    const unsigned char* xbase = reinterpret_cast<const unsigned char*>(a.x) + (gather ? 0 : r0 * a.ldx * Elem<T>::BYTES);
-    const unsigned char* wbase = reinterpret_cast<const unsigned char*>(a.w) + (none ? 0 : (nbase + n0) * rowb);
+    const unsigned char* xbase = reinterpret_cast<const unsigned char*>(a.x) + (gather ? 0 : r0 * a.ldx * Elem<T>::BYTES) + k0;
+    const unsigned char* wbase = reinterpret_cast<const unsigned char*>(a.w) + (none ? 0 : (nbase + n0) * pitch) + k0;
     unsigned off[DMA];
 #pragma unroll
     for (int j = 0; j < XI; ++j) {
         const long p = min(r0 + 8 * (wave + NW * j) + (lane >> 3), r1 - 1);
         off[2 * j] = (unsigned)((gather ? x_row(a, p) : p - r0) * a.ldx * Elem<T>::BYTES) + kx;
-        off[2 * j + 1] = (unsigned)(min(8 * (wave + NW * j) + (lane >> 3), a.N - 1 - n0) * rowb) + kx;
+        off[2 * j + 1] = (unsigned)(min(8 * (wave + NW * j) + (lane >> 3), a.N - 1 - n0) * pitch) + kx;
     }
     // instruction d of the slice whose x and w columns start at xs and ws: even d x rows, odd d weight rows
     auto dma = [&](const unsigned char* xs, const unsigned char* ws, int into, int d) __attribute__((always_inline)) {
@@ -358,11 +362,16 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_tile_kernel(GemmArgs a) 
     // and slopes are loaded once; residuals of four rows are asked for together.
     constexpr int EM = TM < 4 ? TM : 4, EN = TN < 4 ? TN : 4, PITCH = EN * 64 + 16, LPR = EN * 2, RPI = 64 / LPR, IT = EM * 16 / RPI;
     unsigned char* part = smem + wave * EM * 16 * PITCH;
+    GemmArgs o = a;
+    if (a.splits > 1) {                                      // a part's plain sums; gemm_join_kernel does the rest
+        o.bias = o.res = nullptr; o.act = FR_ACT_NONE; o.out_type = FR_TYPE_F32;
+        o.out = a.partial + (long)split * a.M * a.N;
+    }
     __syncthreads();                                         // the ring is read
 #pragma unroll
     for (int q = 0; q < TN / EN; ++q) {
         const int n = n0 + (wn * TN + EN * q) * 16 + (lane % LPR) * 8, have = min(8, a.N - n);
-        const Columns col = columns(a, n, have, nbase, none);
+        const Columns col = columns(o, n, have, nbase, none);
 #pragma unroll
         for (int u = 0; u < TM / EM; ++u) {
 #pragma unroll
@@ -372,10 +381,32 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_tile_kernel(GemmArgs a) 
             wave_lds_fence();
             const long p0 = r0 + (wm * TM + EM * u) * 16 + lane / LPR;
             const unsigned char* at = part + (lane / LPR) * PITCH + (lane % LPR) * 32;
-            if (have > 0) finish_rows<RPI, IT, PITCH>(a, p0, r1, n, have, col, at, none);
+            if (have > 0) finish_rows<RPI, IT, PITCH>(o, p0, r1, n, have, col, at, none);
             wave_lds_fence();
         }
     }
+}
+
+// The parts of a split K added in their order, then the epilogue: 8 outputs a thread.
+__global__ __launch_bounds__(256) void gemm_join_kernel(GemmArgs a) {
+    const int vecs = (a.N + 7) / 8;
+    const long i = blockIdx.x * 256l + threadIdx.x, row = i / vecs;
+    if (row >= a.M) return;
+    const int n = (int)(i - row * vecs) * 8, have = min(8, a.N - n);
+    Vec8f v{};
+    for (int s0 = 0; s0 < a.splits; s0 += 4) {
+        Vec8f p[4];
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+            if (s0 + s < a.splits) p[s] = get8n(a.partial, ((s0 + s) * a.M + row) * a.N + n, have, FR_TYPE_F32);
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+            if (s0 + s < a.splits) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v.v[j] += p[s].v[j];
+            }
+    }
+    finish8(a, row, n, columns(a, n, have, 0, false), v, false);
 }
 
 // Any shape, any alignment: 64 x 64 outputs a block, 4 waves of 32 x 32, slices of 128 bytes of K through registers into
@@ -464,7 +495,7 @@ int launch_tile(GemmArgs a, hipStream_t st) {
     if (mt * a.n_tiles > 0x7FFFFFFFll) FR_FAIL(FR_ERR_UNSUPPORTED, "adapter product: more than 2^31 output tiles");
     const int lds = std::max(ST * (BM + BN) * 128, WM * WN * std::min(64, BM / WM) * (std::min(64, BN / WN) * 4 + 16));    // the ring; the epilogue's rows
     FR_BIG_LDS_ONCE((gemm_tile_kernel<T, BM, BN, WM, WN, ST>), lds);
-    hipLaunchKernelGGL((gemm_tile_kernel<T, BM, BN, WM, WN, ST>), dim3((unsigned)(mt * a.n_tiles)), dim3(64 * WM * WN), lds, st, a);
+    hipLaunchKernelGGL((gemm_tile_kernel<T, BM, BN, WM, WN, ST>), dim3((unsigned)(mt * a.n_tiles * a.splits)), dim3(64 * WM * WN), lds, st, a);
     FR_LAUNCH_CHECK("gemm_tile_kernel");
     return FR_OK;
 }
@@ -482,6 +513,14 @@ double slice_cost(const GemmArgs& a) {
     return on_cu <= 1 ? alone : std::max(alone, on_cu * each);
 }
 
+// K of a product whose 64-tiles leave most of the card idle is split into parts of at least 4 slices, up to two blocks a CU.
+// 24 x 4096 x 4096 f16: 20.3 us in one part; below 6 us saved (K of fewer than 16 slices) the second launch eats it up.
+int split_count(int64_t M, int N, int K, int type) {
+    const long slices = ((long)K * type_bytes(type) + 127) / 128, tiles = ((M + 63) / 64) * ((N + 63) / 64);
+    if (tiles > 160 || slices < 16) return 1;
+    return (int)std::max(1l, std::min(std::min(slices / 4, 512 / tiles), 16l));
+}
+
 template <typename T>
 int launch_gemm(GemmArgs a, hipStream_t st) {
     const long rowb = (long)a.K * Elem<T>::BYTES, ldxb = a.ldx * Elem<T>::BYTES;
@@ -489,7 +528,19 @@ int launch_gemm(GemmArgs a, hipStream_t st) {
     const bool whole = rowb % 16 == 0 && ldxb % 16 == 0 && ((uintptr_t)a.x & 15) == 0 && ((uintptr_t)a.w & 15) == 0;
     // the staged kernel adds 32-bit offsets to its tile's (gathered rows: the matrix's) first row
     const bool near = std::max(rowb, ldxb) < (1l << 23) && (!gather || a.M / a.k * ldxb < (1l << 32));
+    a.splits = 1;
     if (whole && near) {
+        const int splits = a.partial ? split_count(a.M, a.N, a.K, Elem<T>::BYTES == 4 ? FR_TYPE_F32 : FR_TYPE_BF16) : 1;
+        if (splits > 1) {
+            const long slices = (rowb + 127) / 128;
+            a.split_slices = (int)((slices + splits - 1) / splits);
+            a.splits = (int)((slices + a.split_slices - 1) / a.split_slices);
+            const int rc = launch_tile<T, 64, 64, 2, 2, 3>(a, st);
+            if (rc) return rc;
+            hipLaunchKernelGGL(gemm_join_kernel, dim3((unsigned)((a.M * ((a.N + 7) / 8) + 255) / 256)), dim3(256), 0, st, a);
+            FR_LAUNCH_CHECK("gemm_join_kernel");
+            return FR_OK;
+        }
         const double c256 = slice_cost<T, 256>(a), c128 = slice_cost<T, 128>(a), c64 = slice_cost<T, 64>(a);
         if (c256 <= c128 && c256 <= c64) return launch_tile<T, 256, 256, 2, 4, 2>(a, st);
         if (c128 <= c64) return launch_tile<T, 128, 128, 2, 2, 2>(a, st);
@@ -512,7 +563,8 @@ int launch_type(int type, const GemmArgs& a, hipStream_t st) {
 
 extern "C" int fr_linear_workspace_bytes(int64_t M, int N, int K, int type, size_t* out_bytes) {
     if (!out_bytes || M < 0 || N <= 0 || K <= 0 || !type_ok(type)) FR_FAIL(FR_ERR_ARG, "fr_linear_workspace_bytes: bad shape or type");
-    *out_bytes = 0;
+    const int splits = split_count(M, N, K, type);
+    *out_bytes = splits > 1 ? (size_t)splits * M * N * 4 : 0;
     return FR_OK;
 }
 
@@ -527,7 +579,10 @@ extern "C" int fr_linear(const void* x, int64_t ldx, const void* w, const void* 
     if (act == FR_ACT_PRELU && !slope) FR_FAIL(FR_ERR_ARG, "fr_linear: PReLU without slopes");
     if (M == 0) return FR_OK;
     if (!x || !w || !out) FR_FAIL(FR_ERR_ARG, "fr_linear: NULL tensor");
+    const int splits = split_count(M, N, K, type);
+    if (splits > 1 && (!workspace || workspace_bytes < (size_t)splits * M * N * 4)) FR_FAIL(FR_ERR_WORKSPACE, "fr_linear: workspace too small");
     GemmArgs a{};
+    a.partial = splits > 1 ? (float*)workspace : nullptr;
     a.x = x; a.w = w; a.bias = bias; a.slope = slope; a.res = residual; a.out = out;
     a.M = M; a.ldx = ldx; a.ldr = ldr; a.N = N; a.K = K;
     a.bias_type = bias_type; a.res_type = res_type; a.out_type = out_type; a.act = act;

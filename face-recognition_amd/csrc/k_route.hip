@@ -470,7 +470,7 @@ void launch_choose(const RouteArgs& a, hipStream_t st) {
 extern "C" int fr_route_workspace_bytes(int64_t T, int E, int k, size_t* out_bytes) {
     if (!out_bytes || T < 0 || E <= 0 || E > RT_EMAX || k <= 0 || k > RT_KMAX || k > E) FR_FAIL(FR_ERR_ARG, "fr_route_workspace_bytes: bad shape (E <= 512, k <= min(16, E))");
     const size_t chunks = (size_t)((T + RT_ROWS - 1) / RT_ROWS);
-    *out_bytes = align_up((chunks + 1) * (E + 1) * 4, 16);
+    *out_bytes = chunks > 1 ? align_up((chunks + 1) * (E + 1) * 4, 16) : 0;
     return FR_OK;
 }
 
@@ -487,8 +487,8 @@ extern "C" int fr_route(const void* logits, int logits_type, int64_t T, int E, i
     size_t need = 0;
     const int rc = fr_route_workspace_bytes(T, E, k, &need);
     if (rc) return rc;
-    if (!weights || !experts || !order || !offsets || (T && !logits)) FR_FAIL(FR_ERR_ARG, "fr_route: NULL tensor");
-    if (workspace_bytes < need || !workspace) FR_FAIL(FR_ERR_WORKSPACE, "fr_route: workspace too small");
+    if (!offsets || (T && (!weights || !experts || !order || !logits))) FR_FAIL(FR_ERR_ARG, "fr_route: NULL tensor");
+    if (workspace_bytes < need || (need && !workspace)) FR_FAIL(FR_ERR_WORKSPACE, "fr_route: workspace too small");
     RouteArgs a{logits, bias, weights, experts, order, offsets, (int*)workspace + E + 1, (int*)workspace, T,
                 logits_type, E, k, score, groups, top_groups, renormalise, (int)((T + RT_ROWS - 1) / RT_ROWS), scale};
     hipStream_t st = (hipStream_t)stream;

@@ -215,16 +215,13 @@ def _type(op, what, dtype):
 def _check_tensors(op, first, *others):
     """One device, and no gradient asked for: the kernels have no backward pass, and a result that silently cuts the graph
     would be a wrong one."""
-    grad = torch.is_grad_enabled()
-    if grad and first.requires_grad:
-        _fail(op, "inference only: call it under torch.no_grad() or on detached tensors")
     dev = first.device
     for t in others:
-        if t is not None:
-            if t.device != dev:
-                _fail(op, f"all tensors on {dev}: got one on {t.device}")
-            if grad and t.requires_grad:
-                _fail(op, "inference only: call it under torch.no_grad() or on detached tensors")
+        if t is not None and t.device != dev:
+            _fail(op, f"all tensors on {dev}: got one on {t.device}")
+    if torch.is_grad_enabled() and (first.requires_grad or any(t is not None and t.requires_grad for t in others)):
+        _fail(op, "inference only: call it under torch.no_grad() or on detached tensors")
+    return dev
 
 
 def _ptr(t):
@@ -235,14 +232,19 @@ def _call(name, dev, *args):
     """One C-ABI call on the device's current stream.  A call on one row takes a few microseconds on the GPU, so the host's
     share counts: no Stream object, no device switch where none is needed."""
     index = dev.index
-    fn = getattr(_lib.lib(), name)
-    if torch.cuda.current_device() == index:
+    fn = _entry(name)
+    if torch._C._cuda_getDevice() == index:
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(dev):
             rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     if rc:
         _lib.check(rc, name)
+
+
+@functools.lru_cache(maxsize=None)
+def _entry(name):
+    return getattr(_lib.lib(), name)
 
 
 @functools.lru_cache(maxsize=1024)
@@ -269,9 +271,10 @@ def _vector(op, what, t, n, dtypes):
 
 
 def _linear_shape(op, x, weight, residual):
-    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1] or weight.shape[1] < 1 or weight.shape[0] < 1:
-        _fail(op, f"expected x [..., K] and weight [N, K]: got {tuple(x.shape)} and {tuple(weight.shape)}")
-    shape = x.shape[:-1] + (weight.shape[0],)
+    xs, ws = x.shape, weight.shape
+    if len(xs) < 1 or len(ws) != 2 or xs[-1] != ws[1] or ws[1] < 1 or ws[0] < 1:
+        _fail(op, f"expected x [..., K] and weight [N, K]: got {tuple(xs)} and {tuple(ws)}")
+    shape = xs[:-1] + ws[:1]
     if residual is not None and residual.shape != shape:
         _fail(op, f"residual is {tuple(shape)}: got {tuple(residual.shape)}")
     return shape
@@ -279,31 +282,44 @@ def _linear_shape(op, x, weight, residual):
 
 def _linear(x, weight, bias, slope, residual, act, out_dtype):
     op = "linear"
-    _check_tensors(op, x, weight, bias, slope, residual)
+    dev = _check_tensors(op, x, weight, bias, slope, residual)
     shape = _linear_shape(op, x, weight, residual)
     N, K = weight.shape
-    kind = _type(op, "x", x.dtype)
-    if weight.dtype != x.dtype:
-        _fail(op, f"x and weight have one type: got {x.dtype} and {weight.dtype}")
-    act = _name(op, _ACTS, act, "act")
-    if (slope is not None) != (act == _lib.FR_ACT_PRELU):
+    dtype = x.dtype
+    kind = _type(op, "x", dtype)
+    if weight.dtype != dtype:
+        _fail(op, f"x and weight have one type: got {dtype} and {weight.dtype}")
+    code = _name(op, _ACTS, act, "act")
+    if (slope is not None) != (act == "prelu"):
         _fail(op, "slope belongs to act='prelu', and only to it")
-    bias = _vector(op, "bias", bias, N, (x.dtype, torch.float32))
-    slope = _vector(op, "slope", slope, N, (torch.float32,))
-    out_dtype = x.dtype if out_dtype is None else out_dtype
-    out_type = _type(op, "out_dtype", out_dtype)
-    res_type = kind if residual is None else _type(op, "residual", residual.dtype)
-    out = x.new_empty(shape, dtype=out_dtype)
+    bias_type, res_type, ldr = kind, kind, 0
+    bias_ptr = slope_ptr = res_ptr = ws_ptr = None
+    if bias is not None:
+        bias = _vector(op, "bias", bias, N, (dtype, torch.float32))
+        bias_type, bias_ptr = _TYPES[bias.dtype], bias.data_ptr()
+    if slope is not None:
+        slope = _vector(op, "slope", slope, N, (torch.float32,))
+        slope_ptr = slope.data_ptr()
+    if out_dtype is None or out_dtype == dtype:
+        out, out_type = x.new_empty(shape), kind
+    else:
+        out_type = _type(op, "out_dtype", out_dtype)
+        out = x.new_empty(shape, dtype=out_dtype)
+    if residual is not None:
+        res_type = _type(op, "residual", residual.dtype)
+        residual, ldr = _rows(residual, N)
+        res_ptr = residual.data_ptr()
     M = out.numel() // N
     if M == 0:
         return out
     x, ldx = _rows(x, K)
-    residual, ldr = (None, 0) if residual is None else _rows(residual, N)
     weight = weight.contiguous()
     need = _scratch_bytes("fr_linear_workspace_bytes", M, N, K, kind)
-    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-    _call("fr_linear", x.device, x.data_ptr(), ldx, weight.data_ptr(), _ptr(bias), _ptr(slope), _ptr(residual), ldr, out.data_ptr(),
-          M, N, K, kind, kind if bias is None else _TYPES[bias.dtype], res_type, out_type, act, _ptr(ws), need)
+    if need:
+        ws = x.new_empty(need, dtype=torch.uint8)
+        ws_ptr = ws.data_ptr()
+    _call("fr_linear", dev, x.data_ptr(), ldx, weight.data_ptr(), bias_ptr, slope_ptr, res_ptr, ldr, out.data_ptr(),
+          M, N, K, kind, bias_type, res_type, out_type, code, ws_ptr, need)
     return out
 
 
@@ -321,7 +337,7 @@ def _block_norm_shape(op, x, slot_weights):
 def _block_norm(x, residual, slot_weights, norm, weight, bias, eps, gate, gate_act, scale, next_norm, next_weight, next_bias,
                 next_eps, out_dtype, next_dtype):
     op = "block_norm"
-    _check_tensors(op, x, residual, slot_weights, weight, bias, gate, next_weight, next_bias)
+    dev = _check_tensors(op, x, residual, slot_weights, weight, bias, gate, next_weight, next_bias)
     shape = _block_norm_shape(op, x, slot_weights)
     d = x.shape[-1]
     norm, next_norm = _name(op, _NORMS, norm, "norm"), _name(op, _NORMS, next_norm, "next_norm")
@@ -351,14 +367,14 @@ def _block_norm(x, residual, slot_weights, norm, weight, bias, eps, gate, gate_a
             _fail(op, f"gate is [{d}], {tuple(shape[:-1]) + (1,)} or {tuple(shape)}: got {tuple(gate.shape)}")
     gate_act = _name(op, _GATE_ACTS, gate_act, "gate_act")
     out = x.new_empty(shape, dtype=out_dtype)
-    nxt = x.new_empty(shape if next_norm else 0, dtype=next_dtype)
+    nxt = x.new_empty(shape if next_norm else 0, dtype=next_dtype)      # without next_norm: empty, as the op's schema has two results
     T = out.numel() // d
     if T == 0:
         return out, nxt
     slots = 0 if slot_weights is None else x.shape[-2]
     x = x.contiguous()
     slot_weights = None if slot_weights is None else slot_weights.contiguous()
-    _call("fr_block_norm", x.device, x.data_ptr(), x_type, slots, _ptr(slot_weights), T, d, norm, _ptr(weight), _ptr(bias), eps,
+    _call("fr_block_norm", dev, x.data_ptr(), x_type, slots, _ptr(slot_weights), T, d, norm, _ptr(weight), _ptr(bias), eps,
           _ptr(gate), gate_type, gate_ldt, gate_ldc, gate_act, scale, _ptr(residual), res_type, out.data_ptr(), out_type,
           next_norm, _ptr(next_weight), _ptr(next_bias), next_eps, nxt.data_ptr() if next_norm else None, next_type)
     return out, nxt
@@ -382,7 +398,7 @@ def _route_empty(logits, k):
 
 def _route(logits, k, score, bias, groups, top_groups, renormalise, scale):
     op = "route"
-    _check_tensors(op, logits, bias)
+    dev = _check_tensors(op, logits, bias)
     T, E = _route_shape(op, logits, k)
     kind = _type(op, "logits", logits.dtype)
     score = _name(op, _SCORES, score, "score")
@@ -390,10 +406,9 @@ def _route(logits, k, score, bias, groups, top_groups, renormalise, scale):
     logits = logits.contiguous()
     need = _scratch_bytes("fr_route_workspace_bytes", T, E, k)
     out = _route_empty(logits, k)
-    ws = logits.new_empty(need, dtype=torch.uint8)
-    weights, experts, order, offsets = (t.data_ptr() or ws.data_ptr() for t in out)      # T = 0: empty tensors have no address
-    _call("fr_route", logits.device, logits.data_ptr(), kind, T, E, k, score, _ptr(bias), groups, top_groups, renormalise, scale,
-          weights, experts, order, offsets, ws.data_ptr(), need)
+    ws = logits.new_empty(need, dtype=torch.uint8) if need else None
+    _call("fr_route", dev, logits.data_ptr(), kind, T, E, k, score, _ptr(bias), groups, top_groups, renormalise, scale,
+          out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(), out[3].data_ptr(), _ptr(ws), need)
     return out
 
 
@@ -414,7 +429,7 @@ def _expert_shape(op, x, weight, order, offsets, k, rows, out):
 
 def _expert_linear(x, weight, order, offsets, k, bias, act, slope, rows, out, out_dtype):
     op = "expert_linear"
-    _check_tensors(op, x, weight, order, offsets, bias, slope)
+    dev = _check_tensors(op, x, weight, order, offsets, bias, slope)
     T, shape = _expert_shape(op, x, weight, order, offsets, k, rows, out)
     E, N, K = weight.shape
     kind = _type(op, "x", x.dtype)
@@ -437,7 +452,7 @@ def _expert_linear(x, weight, order, offsets, k, bias, act, slope, rows, out, ou
     if T == 0:
         return y
     x, weight, order, offsets = x.contiguous(), weight.contiguous(), order.contiguous(), offsets.contiguous()
-    _call("fr_expert_linear", x.device, x.data_ptr(), int(rows == "sorted"), weight.data_ptr(), _ptr(bias), _ptr(slope), order.data_ptr(),
+    _call("fr_expert_linear", dev, x.data_ptr(), int(rows == "sorted"), weight.data_ptr(), _ptr(bias), _ptr(slope), order.data_ptr(),
           offsets.data_ptr(), y.data_ptr(), int(out == "slots"), T, k, E, N, K, kind, kind if bias is None else _TYPES[bias.dtype],
           out_type, act)
     return y

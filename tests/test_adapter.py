@@ -186,8 +186,8 @@ def test_c_entries_refuse_before_they_launch():
     refused(route(groups=3), -1, "groups")
     refused(route(groups=4, top=5), -1, "groups")
     refused(route(groups=8, top=1), -1, "fewer than k")
-    refused(route(wsb=8), -4, "workspace")
-    refused(route(ws=None), -4, "workspace")
+    refused(route(T=1000, wsb=8), -4, "workspace")
+    refused(route(T=1000, ws=None), -4, "workspace")
 
     def expert(T=1, k=2, E=4, N=8, K=8, kind=1, act=0, order=one):
         return lib.fr_expert_linear(one, 0, one, None, None, order, one, one, 0, T, k, E, N, K, kind, kind, kind, act, None)
