@@ -409,6 +409,117 @@ __global__ __launch_bounds__(256) void gemm_join_kernel(GemmArgs a) {
     finish8(a, row, n, columns(a, n, have, 0, false), v, false);
 }
 
+// Few rows: the weights are read once and are nearly all there is to read.  A block takes 16 weight rows and up to 16 MT rows
+// of x; its NW waves take the slices of K in turn, each with a ring of R slices of its own in LDS, so that nothing waits but
+// a wave for its own oldest slice; the waves' sums meet in LDS, in their order, and one launch does it all.
+// The ring is filled by LDS-DMA in whole lines of 128 bytes: fragments straight from memory take 64 bytes of 16 rows an
+// instruction, which the address path carries at half the rate (16 x 4096 x 4096: 12 us).  Rows that are not whole 16-byte
+// chunks (WHOLE false) go through registers instead.
+template <typename T, int MT, int NW, int R, bool WHOLE>
+__global__ __launch_bounds__(64 * NW) void gemm_rows_kernel(GemmArgs a) {
+    constexpr int ROWS = 16 + 16 * MT, DPS = ROWS / 8, SLOT = ROWS * 128;
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int li = lane & 15, lg = lane >> 4;
+    const int nt = blockIdx.x % a.n_tiles, mt = blockIdx.x / a.n_tiles, n0 = nt * 16;
+    long r0 = (long)mt * 16 * MT, r1 = min(r0 + 16 * MT, a.M);
+    int expert = 0;
+    if (a.order && !expert_tile(a, mt, 16 * MT, expert, r0, r1)) return;
+    const bool none = a.order && expert == a.E;
+    const long nbase = (long)expert * a.N, rowb = (long)a.K * Elem<T>::BYTES;
+    f32x4 acc[MT];
+#pragma unroll
+    for (int j = 0; j < MT; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    unsigned char* ring = smem + wave * R * SLOT;
+    if (!none) {
+        // this lane's sources: row 8 d + lane / 8 of the 16 weight rows and then those of x, chunk (lane % 8) ^ key
+        const unsigned char* src[DPS];
+        int kx[2];                                           // the key of row r is that of r + 16
+#pragma unroll
+        for (int d = 0; d < 2; ++d) kx[d] = ((lane & 7) ^ (((8 * d + (lane >> 3)) >> 1) & 7)) * 16;
+#pragma unroll
+        for (int d = 0; d < DPS; ++d) {
+            const int r = 8 * d + (lane >> 3);
+            src[d] = (d < 2 ? reinterpret_cast<const unsigned char*>(a.w) + (nbase + min(n0 + r, a.N - 1)) * rowb
+                            : reinterpret_cast<const unsigned char*>(a.x) + x_row(a, min(r0 + r - 16, r1 - 1)) * a.ldx * Elem<T>::BYTES) + kx[d & 1];
+        }
+        const int slices = (int)((rowb + 127) / 128), mine = (slices - wave + NW - 1) / NW;    // <= 0: more waves than slices
+        auto multiply = [&](const unsigned char* slot) __attribute__((always_inline)) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int at = li * 128 + (((4 * h + lg) ^ ((li >> 1) & 7)) << 4);
+                const u32x4 w = *reinterpret_cast<const u32x4*>(slot + at);
+                u32x4 x[MT];
+#pragma unroll
+                for (int j = 0; j < MT; ++j) x[j] = *reinterpret_cast<const u32x4*>(slot + (j + 1) * 2048 + at);
+#pragma unroll
+                for (int j = 0; j < MT; ++j) Elem<T>::mma(acc[j], w, x[j]);
+            }
+        };
+        if constexpr (WHOLE) {
+            auto stage = [&](int i, int slot) __attribute__((always_inline)) {
+                const long at = (long)(wave + i * NW) * 128;
+#pragma unroll
+                for (int d = 0; d < DPS; ++d) {
+                    const unsigned lo = at + kx[d & 1] >= rowb ? 0u : ~0u;       // K may end inside the slice: zeros behind it
+                    const unsigned long long m = ((unsigned long long)lo << 32) | lo;
+                    const unsigned long long u = ((unsigned long long)(src[d] + at) & m) | ((unsigned long long)&g_zero16 & ~m);
+                    __builtin_amdgcn_global_load_lds((glb_ptr_t)u, (lds_ptr_t)(ring + slot * SLOT + d * 1024), 16, 0, 0);
+                }
+            };
+#pragma unroll
+            for (int i = 0; i < R; ++i)
+                if (i < mine) stage(i, i);
+            int slot = 0;
+            for (int i = 0; i < mine; ++i) {
+                if (i + R <= mine) wait_counts<(R - 1) * DPS, 15>();
+                else wait_counts<0, 15>();
+                multiply(ring + slot * SLOT);
+                wait_counts<63, 0>();
+                if (i + R < mine) stage(i + R, slot);
+                slot = slot + 1 == R ? 0 : slot + 1;
+            }
+        } else {
+            u32x4 c[DPS];
+            auto fetch = [&](int i) __attribute__((always_inline)) {
+                const long at = (long)(wave + i * NW) * 128;
+#pragma unroll
+                for (int d = 0; d < DPS; ++d) c[d] = chunk_at(src[d], at, rowb - kx[d & 1]);
+            };
+            if (mine > 0) fetch(0);
+            for (int i = 0; i < mine; ++i) {
+#pragma unroll
+                for (int d = 0; d < DPS; ++d) *reinterpret_cast<u32x4*>(ring + d * 1024 + lane * 16) = c[d];
+                if (i + 1 < mine) fetch(i + 1);
+                wave_lds_fence();
+                multiply(ring);
+                wave_lds_fence();
+            }
+        }
+    }
+    __syncthreads();
+    f32x4* red = reinterpret_cast<f32x4*>(smem);             // [NW][MT][64], over the rings
+#pragma unroll
+    for (int j = 0; j < MT; ++j) red[(wave * MT + j) * 64 + lane] = acc[j];
+    __syncthreads();
+    if (tid >= MT * 32) return;
+    // thread: row j * 16 + i, columns 8 half .. 8 half + 7: the four of lane groups 2 half and 2 half + 1
+    const int j = tid >> 5, i = tid & 15, half = (tid >> 4) & 1;
+    Vec8f v{};
+#pragma unroll
+    for (int q = 0; q < NW; ++q) {
+        const f32x4 lo = red[(q * MT + j) * 64 + half * 32 + i], hi = red[(q * MT + j) * 64 + half * 32 + 16 + i];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { v.v[e] += lo[e]; v.v[4 + e] += hi[e]; }
+    }
+    const long p = r0 + 16 * j + i;
+    if (p >= r1) return;
+    const long row = out_row(a, p);
+    const int n = n0 + half * 8;
+    if (row < 0 || n >= a.N) return;
+    finish8(a, row, n, columns(a, n, min(8, a.N - n), nbase, none), v, none);
+}
+
 // Any shape, any alignment: 64 x 64 outputs a block, 4 waves of 32 x 32, slices of 128 bytes of K through registers into
 // LDS.  Piece p of LDS row r lies at p ^ ((r >> 1) & 7): the 16 rows of a fragment read fall on different banks.
 template <typename T>
@@ -513,11 +624,26 @@ double slice_cost(const GemmArgs& a) {
     return on_cu <= 1 ? alone : std::max(alone, on_cu * each);
 }
 
+template <typename T, int MT, int NW, int R>
+int launch_rows(GemmArgs a, bool whole, hipStream_t st) {
+    const long mt = a.order ? a.M / (16 * MT) + std::min<long>(a.M, a.E + 1) : (a.M + 16 * MT - 1) / (16 * MT);
+    a.n_tiles = (a.N + 15) / 16;
+    if (mt * a.n_tiles > 0x7FFFFFFFll) FR_FAIL(FR_ERR_UNSUPPORTED, "adapter product: more than 2^31 output tiles");
+    const int lds = NW * R * (16 + 16 * MT) * 128;
+    const dim3 grid((unsigned)(mt * a.n_tiles)), block(64 * NW);
+    if (whole) {
+        FR_BIG_LDS_ONCE((gemm_rows_kernel<T, MT, NW, R, true>), lds);
+        hipLaunchKernelGGL((gemm_rows_kernel<T, MT, NW, R, true>), grid, block, lds, st, a);
+    } else hipLaunchKernelGGL((gemm_rows_kernel<T, MT, NW, 1, false>), grid, block, lds / R, st, a);
+    FR_LAUNCH_CHECK("gemm_rows_kernel");
+    return FR_OK;
+}
+
 // K of a product whose 64-tiles leave most of the card idle is split into parts of at least 4 slices, up to two blocks a CU.
-// 24 x 4096 x 4096 f16: 20.3 us in one part; below 6 us saved (K of fewer than 16 slices) the second launch eats it up.
+// 128 x 4096 x 4096 bf16: 17 us, 20 in one part; K of fewer than 16 slices saves less than the second launch takes.
 int split_count(int64_t M, int N, int K, int type) {
     const long slices = ((long)K * type_bytes(type) + 127) / 128, tiles = ((M + 63) / 64) * ((N + 63) / 64);
-    if (tiles > 160 || slices < 16) return 1;
+    if (M <= 64 || tiles > 160 || slices < 16) return 1;        // up to 64 rows: gemm_rows_kernel
     return (int)std::max(1l, std::min(std::min(slices / 4, 512 / tiles), 16l));
 }
 
@@ -529,6 +655,14 @@ int launch_gemm(GemmArgs a, hipStream_t st) {
     // the staged kernel adds 32-bit offsets to its tile's (gathered rows: the matrix's) first row
     const bool near = std::max(rowb, ldxb) < (1l << 23) && (!gather || a.M / a.k * ldxb < (1l << 32));
     a.splits = 1;
+    if (!a.order && a.M <= 64 && (rowb >= 1024 || !whole)) {
+        // us at K = N = 4096 (16 bits) / 2048 (fp32), against 64-tiles with K split: 16 rows 10 and 14, 24 rows 10 and 15,
+        // 64 rows 13 and 18; fp32 24 rows 9 and 17, 64 rows 14 and 19 (two tiles of 32 rows there: 17 as one of 64)
+        constexpr bool f32 = std::is_same<T, float>::value;
+        if (a.M <= 16 || (f32 && a.M <= 32)) return launch_rows<T, 1, 8, 4>(a, whole, st);
+        if (a.M <= 32 || f32) return launch_rows<T, 2, 8, 3>(a, whole, st);
+        return launch_rows<T, 4, 4, 3>(a, whole, st);
+    }
     if (whole && near) {
         const int splits = a.partial ? split_count(a.M, a.N, a.K, Elem<T>::BYTES == 4 ? FR_TYPE_F32 : FR_TYPE_BF16) : 1;
         if (splits > 1) {
