@@ -249,8 +249,8 @@ FR_DEV void tile_of_block(int block, int mtiles, int ntiles, int& mt, int& nt) {
 template <typename T, int BM, int BN, int WM, int WN, int ST>
 __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_tile_kernel(GemmArgs a) {
     constexpr int NW = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16, XB = BM * 128, BUF = (BM + BN) * 128;
-    constexpr int XI = BM / 8 / NW, WI = BN / 8 / NW, DMA = XI + WI, DPG = DMA / TM;     // DMA instructions a wave and slice
-    static_assert(XI == WI && DMA % TM == 0 && TN <= TM && NW % 2 == 0, "the interleaving below");
+    constexpr int XI = BM / 8 / NW, WI = BN / 8 / NW, DMA = XI + WI, DPG = (DMA + TM - 1) / TM;     // DMA instructions a wave and slice, and a group of products
+    static_assert(TN <= TM && NW % 2 == 0, "the interleaving below");
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int li = lane & 15, lg = lane >> 4, wm = wave / WN, wn = wave % WN;
@@ -273,24 +273,28 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_tile_kernel(GemmArgs a) 
     const bool gather = a.order && !a.rows_sorted;
     const unsigned char* xbase = reinterpret_cast<const unsigned char*>(a.x) + (gather ? 0 : r0 * a.ldx * Elem<T>::BYTES) + k0;
     const unsigned char* wbase = reinterpret_cast<const unsigned char*>(a.w) + (none ? 0 : (nbase + n0) * pitch) + k0;
-    unsigned off[DMA];
+    unsigned off[DMA];                                       // x rows, then weight rows
 #pragma unroll
     for (int j = 0; j < XI; ++j) {
         const long p = min(r0 + 8 * (wave + NW * j) + (lane >> 3), r1 - 1);
-        off[2 * j] = (unsigned)((gather ? x_row(a, p) : p - r0) * a.ldx * Elem<T>::BYTES) + kx;
-        off[2 * j + 1] = (unsigned)(min(8 * (wave + NW * j) + (lane >> 3), a.N - 1 - n0) * pitch) + kx;
+        off[j] = (unsigned)((gather ? x_row(a, p) : p - r0) * a.ldx * Elem<T>::BYTES) + kx;
     }
-    // instruction d of the slice whose x and w columns start at xs and ws: even d x rows, odd d weight rows
+#pragma unroll
+    for (int j = 0; j < WI; ++j) off[XI + j] = (unsigned)(min(8 * (wave + NW * j) + (lane >> 3), a.N - 1 - n0) * pitch) + kx;
+    auto place = [&](int into, int d) __attribute__((always_inline)) {          // of instruction d in LDS
+        return smem + into + (d < XI ? wave + NW * d : BM / 8 + wave + NW * (d - XI)) * 1024;
+    };
+    // instruction d of the slice whose x and w columns start at xs and ws
     auto dma = [&](const unsigned char* xs, const unsigned char* ws, int into, int d) __attribute__((always_inline)) {
-        __builtin_amdgcn_global_load_lds((glb_ptr_t)((d & 1 ? ws : xs) + off[d]), (lds_ptr_t)(smem + into + (d & 1 ? XB : 0) + (wave + NW * (d >> 1)) * 1024), 16, 0, 0);
+        __builtin_amdgcn_global_load_lds((glb_ptr_t)((d < XI ? xs : ws) + off[d]), (lds_ptr_t)place(into, d), 16, 0, 0);
     };
     auto stage = [&](int s, int into) {                      // a whole slice; K may end inside it: chunks behind it come from a zero
         const unsigned lo = (long)s * 128 + kx >= rowb ? 0u : ~0u;
         const unsigned long long m = ((unsigned long long)lo << 32) | lo, zero = (unsigned long long)&g_zero16 & ~m;
 #pragma unroll
         for (int d = 0; d < DMA; ++d) {
-            const unsigned long long u = (unsigned long long)((d & 1 ? wbase : xbase) + (long)s * 128 + off[d]);
-            __builtin_amdgcn_global_load_lds((glb_ptr_t)((u & m) | zero), (lds_ptr_t)(smem + into + (d & 1 ? XB : 0) + (wave + NW * (d >> 1)) * 1024), 16, 0, 0);
+            const unsigned long long u = (unsigned long long)((d < XI ? xbase : wbase) + (long)s * 128 + off[d]);
+            __builtin_amdgcn_global_load_lds((glb_ptr_t)((u & m) | zero), (lds_ptr_t)place(into, d), 16, 0, 0);
         }
     };
 
@@ -337,7 +341,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_tile_kernel(GemmArgs a) 
             for (int q = 0; q < FPG; ++q) fetch(cur, 0, j * FPG + q);      // behind the last slice: whatever that buffer holds, unused
             if (fast)
 #pragma unroll
-                for (int d = 0; d < DPG; ++d) dma(xs, ws, free, j * DPG + d);
+                for (int d = j * DPG; d < (j + 1) * DPG && d < DMA; ++d) dma(xs, ws, free, d);
             if constexpr (BM == 256) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int i = 0; i < TN; ++i) Elem<T>::mma(acc[i][j], wf[1][i], xf[1][j]);
