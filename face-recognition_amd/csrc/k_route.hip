@@ -87,12 +87,12 @@ FR_DEV unsigned wave_minu(unsigned v) {
     return min(min(a, b), min(c, d));
 }
 
-// One row by a whole wave, decided in doubles: lane l holds experts l, l + 64, ...  Lane j < k returns the j-th choice
-// (-1: none) and its weight.  Few rows come here, but a wave that has one holds up its block, and its time is that of fetching
+// The choices of one row by a whole wave, decided in doubles: lane l holds experts l, l + 64, ...; chosen[j] gets the j-th
+// (-1: none).  Few rows come here, but a wave that has one holds up its block, and its time is that of fetching
 // code that no wave nearby has run, then of the chain of dependent steps: loops stay rolled, maxima take DPP steps.
 // (Unrolled over the experts, or with LDS shuffles for every step of a maximum, a row took 30 to 40 us.)
 template <int NE>
-FR_DEV void choose_exact(const RouteArgs& a, long row, double* keys, int& mine, float& weight) {
+FR_DEV void choose_exact(const RouteArgs& a, long row, double* keys, int* chosen) {
     const int lane = threadIdx.x & 63;
     const double NONE = -INFINITY;
     const bool scored = a.bias != nullptr || a.groups > 1, soft = a.score == FR_SCORE_SOFTMAX;
@@ -163,9 +163,9 @@ FR_DEV void choose_exact(const RouteArgs& a, long row, double* keys, int& mine, 
         }
         wave_lds_fence();
     }
-    mine = -1;
+    int j = 0;
 #pragma unroll 1
-    for (int j = 0; j < a.k; ++j) {
+    for (; j < a.k; ++j) {
         double own = NONE;
         unsigned at = RT_EMAX;
 #pragma unroll
@@ -176,17 +176,10 @@ FR_DEV void choose_exact(const RouteArgs& a, long row, double* keys, int& mine, 
         const double best = wave_max(own);
         if (best == NONE) break;
         at = wave_minu(own == best ? at : RT_EMAX);
-        if (lane == (int)(at & 63)) keys[at] = NONE;
-        if (lane == j) mine = (int)at;
+        if (lane == (int)(at & 63)) { keys[at] = NONE; chosen[j] = (int)at; }
         wave_lds_fence();
     }
-    const float mine_l = mine >= 0 ? load1(a.logits, row * a.E + mine, a.type) : -INFINITY, top = row_max<64>(mine_l);
-    weight = mine >= 0 ? raw_weight(a, mine_l, top, m, (float)z) : 0.f;
-    if (a.renormalise) {
-        const float sum = row_sum<64>(weight);
-        if (sum > 0.f) weight /= sum;
-    }
-    weight *= a.scale;
+    if (lane >= j && lane < a.k) chosen[lane] = -1;
     wave_lds_fence();
 }
 
@@ -217,22 +210,32 @@ FR_DEV void place_slots(const RouteArgs& a, int* next, const int* experts, int n
         wave_lds_fence();
     }
 }
-// next[e] = sum of n[0 .. e) for e <= E, by one wave; n(e) gives a count, also written to a.offsets if `write`.
-template <typename F>
-FR_DEV void first_places(const RouteArgs& a, int* next, bool write, F n) {
+// next[e] = sum of n(0 .. e - 1) + more(e) for e <= E, by one wave; the sums alone also go to a.offsets if `write`.
+template <typename F, typename G>
+FR_DEV void first_places(const RouteArgs& a, int* next, bool write, F n, G more) {
     const int lane = threadIdx.x & 63;
+    int c[RT_EMAX / 64 + 1], m[RT_EMAX / 64 + 1];            // all asked for before the first is used
+#pragma unroll
+    for (int q = 0; q <= RT_EMAX / 64; ++q) {
+        const int e = q * 64 + lane;
+        c[q] = e <= a.E ? n(e) : 0;
+        m[q] = e <= a.E ? more(e) : 0;
+    }
     int before = 0;
-    for (int e0 = 0; e0 <= a.E; e0 += 64) {
-        const int e = e0 + lane, c = e <= a.E ? n(e) : 0;
-        int s = c;
+#pragma unroll
+    for (int q = 0; q <= RT_EMAX / 64; ++q) {
+        if (q * 64 > a.E) break;
+        const int e = q * 64 + lane;
+        int s = c[q];
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) { const int t = __shfl_up(s, o, 64); if (lane >= o) s += t; }
         if (e <= a.E) {
-            next[e] = before + s - c;
-            if (write) a.offsets[e] = before + s - c;
+            next[e] = before + s - c[q] + m[q];
+            if (write) a.offsets[e] = before + s - c[q];
         }
         before += __shfl(s, 63, 64);
     }
+    wave_lds_fence();
 }
 
 // A row takes LPR lanes, a lane up to V experts of one group, in index order over the lanes.  The k best come from k maxima
@@ -245,24 +248,24 @@ FR_DEV void first_places(const RouteArgs& a, int* next, bool write, F n) {
 // (the row's sum of up to 512 besides).  At 65536 x 256, biased sigmoids, 8 of 256 in 4 of 8 groups, one row in 500 goes
 // that way; with the expert's number in the scored keys too it was one in 50, which took more time than all the rest.
 template <int V, int LPR, int NE, int NB, bool SCORED>
-__global__ __launch_bounds__(64 * RT_WAVES) void route_choose_kernel(RouteArgs a) {
+__global__ __launch_bounds__(64 * RT_WAVES, 4) void route_choose_kernel(RouteArgs a) {
     __shared__ int count[RT_EMAX + 1];
     __shared__ int chosen[RT_ROWS * RT_KMAX];
+    __shared__ float bias[SCORED ? RT_EMAX + V : 1];
     __shared__ double keys[RT_WAVES][NE * 64];
     constexpr unsigned MASK = (1u << NB) - 1;
     constexpr int RPW = 64 / LPR;
     constexpr float L2E = 1.4426950408889634f, DROP = 1.f / (float)(1u << (23 - NB));
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, rl = lane % LPR, base = lane - rl;
     for (int e = threadIdx.x; e <= a.E; e += blockDim.x) count[e] = 0;
+    if constexpr (SCORED)                                    // in LDS: registers are what limits the waves a SIMD holds
+        for (int e = threadIdx.x; e < RT_EMAX + V; e += blockDim.x) bias[e] = a.bias && e < a.E ? a.bias[e] : 0.f;
     __syncthreads();
     static_assert(!SCORED || V <= 1 << NB, "a lane's keys are unique");
     const bool need_z = SCORED || !a.renormalise;
     const int per = a.E / a.groups, LG = (per + V - 1) / V, g = rl / LG, part = rl - g * LG;
     const float slack = a.score == FR_SCORE_SOFTMAX ? 0x1p-18f : 0x1p-21f;
     const int e0 = g * per + part * V, cnt = g < a.groups ? min(V, per - part * V) : 0;
-    float b[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) b[v] = a.bias && v < cnt ? a.bias[e0 + v] : 0.f;
 #pragma unroll 1
     for (int it = wave; it * RPW < RT_ROWS; it += RT_WAVES) {
         const int r = it * RPW + lane / LPR;
@@ -302,7 +305,8 @@ __global__ __launch_bounds__(64 * RT_WAVES) void route_choose_kernel(RouteArgs a
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 const float s = a.score == FR_SCORE_SOFTMAX ? f[v] * rz : __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-l[v] * L2E));
-                f[v] = l[v] > -INFINITY && b[v] > -INFINITY ? s + b[v] : -INFINITY;
+                const float b = bias[min(e0, RT_EMAX) + v];
+                f[v] = l[v] > -INFINITY && b > -INFINITY ? s + b : -INFINITY;
             }
         } else {
 #pragma unroll
@@ -376,9 +380,15 @@ __global__ __launch_bounds__(64 * RT_WAVES) void route_choose_kernel(RouteArgs a
             for (int v = 0; v < V; ++v) key[v] = key[v] == top ? 0u : key[v];
         }
         // lane j < k of the row: its j-th choice
+        if (!SCORED && rl < a.k) chosen[r * a.k + rl] = mine ? (int)(MASK - (mine & MASK)) : -1;
         wave_lds_fence();
-        int pick = mine ? (int)(MASK - (mine & MASK)) : -1;
-        if (SCORED) pick = rl < a.k ? chosen[r * a.k + rl] : -1;
+        unsigned long long again = __ballot(doubt && row < a.T && rl == 0);
+        while (again) {
+            const int rr = it * RPW + (__ffsll(again) - 1) / LPR;
+            again &= again - 1;
+            choose_exact<NE>(a, (long)blockIdx.x * RT_ROWS + rr, keys[wave], chosen + rr * a.k);
+        }
+        const int pick = rl < a.k && row < a.T ? chosen[r * a.k + rl] : -1;
         const float pl = pick >= 0 ? load1(a.logits, row * a.E + pick, a.type) : -INFINITY;
         const float best = row_max<LPR>(pl);
         float w = pick >= 0 ? raw_weight(a, pl, best, m, z) : 0.f;
@@ -386,35 +396,17 @@ __global__ __launch_bounds__(64 * RT_WAVES) void route_choose_kernel(RouteArgs a
             const float sum = row_sum<LPR>(w);
             if (sum > 0.f) w /= sum;
         }
-        const bool sure = row < a.T && !doubt;
-        if (sure && rl < a.k) {
+        if (rl < a.k && row < a.T) {
             a.weights[row * a.k + rl] = w * a.scale;
             a.experts[row * a.k + rl] = pick;
-            chosen[r * a.k + rl] = pick;
             atomicAdd(&count[pick >= 0 ? pick : a.E], 1);    // whole numbers: any order gives the same
-        }
-        unsigned long long again = __ballot(doubt && row < a.T && rl == 0);
-        while (again) {
-            const int at = __ffsll(again) - 1, rr = it * RPW + at / LPR;
-            again &= again - 1;
-            const long row2 = (long)blockIdx.x * RT_ROWS + rr;
-            int pick2;
-            float w2;
-            choose_exact<NE>(a, row2, keys[wave], pick2, w2);
-            if (lane < a.k) {
-                a.weights[row2 * a.k + lane] = w2;
-                a.experts[row2 * a.k + lane] = pick2;
-                chosen[rr * a.k + lane] = pick2;
-                atomicAdd(&count[pick2 >= 0 ? pick2 : a.E], 1);
-            }
         }
     }
     __syncthreads();
     if (a.chunks > 1) {
         for (int e = threadIdx.x; e <= a.E; e += blockDim.x) a.counts[(long)e * a.chunks + blockIdx.x] = count[e];
     } else if (wave == 0) {                                  // one chunk is all: order it here, one launch in place of three
-        first_places(a, count, true, [&](int e) { return count[e]; });
-        wave_lds_fence();
+        first_places(a, count, true, [&](int e) { return count[e]; }, [](int) { return 0; });
         place_slots(a, count, chosen, (int)(a.T * a.k), 0);
     }
 }
@@ -451,10 +443,7 @@ __global__ __launch_bounds__(256) void route_scan_kernel(RouteArgs a) {
 // Places of a chunk's slots: first place of the expert + its slots in earlier chunks + earlier in this chunk.
 __global__ __launch_bounds__(64) void route_place_kernel(RouteArgs a) {
     __shared__ int next[RT_EMAX + 1];
-    first_places(a, next, blockIdx.x == 0, [&](int e) { return a.totals[e]; });
-    wave_lds_fence();
-    for (int e = threadIdx.x; e <= a.E; e += 64) next[e] += a.counts[(long)e * a.chunks + blockIdx.x];
-    wave_lds_fence();
+    first_places(a, next, blockIdx.x == 0, [&](int e) { return a.totals[e]; }, [&](int e) { return a.counts[(long)e * a.chunks + blockIdx.x]; });
     const long s0 = (long)blockIdx.x * RT_ROWS * a.k;
     place_slots(a, next, a.experts + s0, (int)min((long)RT_ROWS * a.k, a.T * a.k - s0), s0);
 }
