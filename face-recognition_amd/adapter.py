@@ -26,11 +26,15 @@ import torch
 from . import ops as _ops
 
 
+_EAGER = {"linear": _ops._linear, "block_norm": _ops._block_norm_eager, "route": _ops._route, "expert_linear": _ops._expert_linear}
+
+
 def _op(name: str, x: torch.Tensor):
     """The operator for a call on ``x``: its implementation itself for an eager call on a plain tensor (the dispatcher takes
     as long as the smallest kernels run), ``torch.ops.fr_hip`` for whatever traces or stands in for one."""
-    if (type(x) is torch.Tensor or type(x) is torch.nn.Parameter) and not torch.compiler.is_compiling():
-        return getattr(_ops, "_" + name)
+    kind = type(x)
+    if (kind is torch.Tensor or kind is torch.nn.Parameter) and not torch.compiler.is_compiling():
+        return _EAGER[name]
     return getattr(torch.ops.fr_hip, name)
 
 

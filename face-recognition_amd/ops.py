@@ -215,11 +215,14 @@ def _type(op, what, dtype):
 def _check_tensors(op, first, *others):
     """One device, and no gradient asked for: the kernels have no backward pass, and a result that silently cuts the graph
     would be a wrong one."""
-    dev = first.device
+    dev, index = first.device, first.get_device()
+    grad = first.requires_grad
     for t in others:
-        if t is not None and t.device != dev:
-            _fail(op, f"all tensors on {dev}: got one on {t.device}")
-    if torch.is_grad_enabled() and (first.requires_grad or any(t is not None and t.requires_grad for t in others)):
+        if t is not None:
+            if t.get_device() != index or (index < 0 and t.device != dev):
+                _fail(op, f"all tensors on {dev}: got one on {t.device}")
+            grad = grad or t.requires_grad
+    if grad and torch.is_grad_enabled():
         _fail(op, "inference only: call it under torch.no_grad() or on detached tensors")
     return dev
 
@@ -257,6 +260,8 @@ def _scratch_bytes(name, *shape):
 
 def _rows(t, width):
     """``t`` [..., width] as rows: (tensor, row stride).  A matrix whose rows are whole but apart is taken as it lies."""
+    if t.is_contiguous():
+        return t, width
     if t.dim() == 2 and (t.stride(1) == 1 or width == 1) and t.stride(0) >= 0:
         return t, t.stride(0)
     return t.contiguous(), width
@@ -334,19 +339,25 @@ def _block_norm_shape(op, x, slot_weights):
     return x.shape[:-2] + x.shape[-1:]
 
 
-def _block_norm(x, residual, slot_weights, norm, weight, bias, eps, gate, gate_act, scale, next_norm, next_weight, next_bias,
-                next_eps, out_dtype, next_dtype):
+def _affine(op, what, norm, weight, bias, d):
+    if weight is None and bias is None:
+        return None, None
+    if norm not in (_lib.FR_NORM_RMS, _lib.FR_NORM_LAYER):
+        _fail(op, f"{what}weight and {what}bias belong to the rms and layer norms")
+    f32 = (torch.float32,)
+    return _vector(op, what + "weight", weight, d, f32), _vector(op, what + "bias", bias, d, f32)
+
+
+def _block_norm_eager(x, residual, slot_weights, norm, weight, bias, eps, gate, gate_act, scale, next_norm, next_weight, next_bias,
+                      next_eps, out_dtype, next_dtype):
+    """(out, next), None for a next that is not asked for."""
     op = "block_norm"
     dev = _check_tensors(op, x, residual, slot_weights, weight, bias, gate, next_weight, next_bias)
     shape = _block_norm_shape(op, x, slot_weights)
     d = x.shape[-1]
     norm, next_norm = _name(op, _NORMS, norm, "norm"), _name(op, _NORMS, next_norm, "next_norm")
-    f32 = (torch.float32,)
-    for n, w, b, what in ((norm, weight, bias, ""), (next_norm, next_weight, next_bias, "next_")):
-        if (w is not None or b is not None) and n not in (_lib.FR_NORM_RMS, _lib.FR_NORM_LAYER):
-            _fail(op, f"{what}weight and {what}bias belong to the rms and layer norms")
-    weight, bias = _vector(op, "weight", weight, d, f32), _vector(op, "bias", bias, d, f32)
-    next_weight, next_bias = _vector(op, "next_weight", next_weight, d, f32), _vector(op, "next_bias", next_bias, d, f32)
+    weight, bias = _affine(op, "", norm, weight, bias, d)
+    next_weight, next_bias = _affine(op, "next_", next_norm, next_weight, next_bias, d)
     out_dtype = x.dtype if out_dtype is None else out_dtype
     next_dtype = out_dtype if next_dtype is None else next_dtype
     out_type, next_type, x_type = _type(op, "out_dtype", out_dtype), _type(op, "next_dtype", next_dtype), _type(op, "x", x.dtype)
@@ -367,7 +378,7 @@ def _block_norm(x, residual, slot_weights, norm, weight, bias, eps, gate, gate_a
             _fail(op, f"gate is [{d}], {tuple(shape[:-1]) + (1,)} or {tuple(shape)}: got {tuple(gate.shape)}")
     gate_act = _name(op, _GATE_ACTS, gate_act, "gate_act")
     out = x.new_empty(shape, dtype=out_dtype)
-    nxt = x.new_empty(shape if next_norm else 0, dtype=next_dtype)      # without next_norm: empty, as the op's schema has two results
+    nxt = x.new_empty(shape, dtype=next_dtype) if next_norm else None
     T = out.numel() // d
     if T == 0:
         return out, nxt
@@ -376,8 +387,15 @@ def _block_norm(x, residual, slot_weights, norm, weight, bias, eps, gate, gate_a
     slot_weights = None if slot_weights is None else slot_weights.contiguous()
     _call("fr_block_norm", dev, x.data_ptr(), x_type, slots, _ptr(slot_weights), T, d, norm, _ptr(weight), _ptr(bias), eps,
           _ptr(gate), gate_type, gate_ldt, gate_ldc, gate_act, scale, _ptr(residual), res_type, out.data_ptr(), out_type,
-          next_norm, _ptr(next_weight), _ptr(next_bias), next_eps, nxt.data_ptr() if next_norm else None, next_type)
+          next_norm, _ptr(next_weight), _ptr(next_bias), next_eps, _ptr(nxt), next_type)
     return out, nxt
+
+
+def _block_norm(x, residual, slot_weights, norm, weight, bias, eps, gate, gate_act, scale, next_norm, next_weight, next_bias,
+                next_eps, out_dtype, next_dtype):
+    out, nxt = _block_norm_eager(x, residual, slot_weights, norm, weight, bias, eps, gate, gate_act, scale, next_norm, next_weight,
+                                 next_bias, next_eps, out_dtype, next_dtype)
+    return out, x.new_empty(0, dtype=next_dtype or out.dtype) if nxt is None else nxt      # the op's schema has two results
 
 
 def _route_shape(op, logits, k):
