@@ -193,6 +193,22 @@ FR_DEV u32x4 chunk_at(const unsigned char* row, long at, long len) {
     return c.v;
 }
 
+// One column of a wave's tiles.  fp32 goes through the tiles once per element of the chunk: four products into one
+// accumulator in a row would each wait for the one before.
+template <typename T, int TN, int TM>
+FR_DEV void column(f32x4 (&acc)[TN][TM], int j, const u32x4 (&w)[TN], const u32x4& x) {
+    if constexpr (std::is_same<T, float>::value) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int i = 0; i < TN; ++i)
+                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(w[i][e]), __uint_as_float(x[e]), acc[i][j], 0, 0, 0);
+    } else {
+#pragma unroll
+        for (int i = 0; i < TN; ++i) Elem<T>::mma(acc[i][j], w[i], x);
+    }
+}
+
 // ---- the staged kernel --------------------------------------------------------------------------------------------------
 typedef __attribute__((address_space(3))) void* lds_ptr_t;
 typedef const __attribute__((address_space(1))) void* glb_ptr_t;
@@ -246,11 +262,13 @@ FR_DEV void tile_of_block(int block, int mtiles, int ntiles, int& mt, int& nt) {
 // The one barrier of a slice stands between its halves: there its last fragments have been read and the next slice has
 // landed, and behind it the DMA of slice s + ST goes into its buffer, spread over the second half's products (in one
 // burst it held up the waves that issue it).
-template <typename T, int BM, int BN, int WM, int WN, int ST>
+// WHOLE false: rows of any alignment.  The chunks of slice s + ST go to registers in the second half of slice s and to LDS in
+// the first half of the next, where ST = 2 wants them by its barrier.
+template <typename T, int BM, int BN, int WM, int WN, int ST, bool WHOLE>
 __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_tile_kernel(GemmArgs a) {
     constexpr int NW = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16, XB = BM * 128, BUF = (BM + BN) * 128;
     constexpr int XI = BM / 8 / NW, WI = BN / 8 / NW, DMA = XI + WI, DPG = (DMA + TM - 1) / TM;     // DMA instructions a wave and slice, and a group of products
-    static_assert(TN <= TM && NW % 2 == 0, "the interleaving below");
+    static_assert(TN <= TM && NW % 2 == 0 && (WHOLE || ST == 2), "the interleaving below");
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int li = lane & 15, lg = lane >> 4, wm = wave / WN, wn = wave % WN;
@@ -285,16 +303,26 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_tile_kernel(GemmArgs a) 
         return smem + into + (d < XI ? wave + NW * d : BM / 8 + wave + NW * (d - XI)) * 1024;
     };
     // instruction d of the slice whose x and w columns start at xs and ws
+    u32x4 held[WHOLE ? 1 : DMA];
     auto dma = [&](const unsigned char* xs, const unsigned char* ws, int into, int d) __attribute__((always_inline)) {
-        __builtin_amdgcn_global_load_lds((glb_ptr_t)((d < XI ? xs : ws) + off[d]), (lds_ptr_t)place(into, d), 16, 0, 0);
+        const unsigned char* src = (d < XI ? xs : ws) + off[d];
+        if constexpr (WHOLE) __builtin_amdgcn_global_load_lds((glb_ptr_t)src, (lds_ptr_t)place(into, d), 16, 0, 0);
+        else held[d] = *reinterpret_cast<const u32x4_any*>(src);
     };
-    auto stage = [&](int s, int into) {                      // a whole slice; K may end inside it: chunks behind it come from a zero
-        const unsigned lo = (long)s * 128 + kx >= rowb ? 0u : ~0u;
-        const unsigned long long m = ((unsigned long long)lo << 32) | lo, zero = (unsigned long long)&g_zero16 & ~m;
+    auto stage = [&](int s, int into) {                      // a whole slice; K may end inside it: zeros behind its end
+        const long at = (long)s * 128;
+        if constexpr (WHOLE) {
+            const unsigned lo = at + kx >= rowb ? 0u : ~0u;
+            const unsigned long long m = ((unsigned long long)lo << 32) | lo, zero = (unsigned long long)&g_zero16 & ~m;
 #pragma unroll
-        for (int d = 0; d < DMA; ++d) {
-            const unsigned long long u = (unsigned long long)((d < XI ? xbase : wbase) + (long)s * 128 + off[d]);
-            __builtin_amdgcn_global_load_lds((glb_ptr_t)((u & m) | zero), (lds_ptr_t)place(into, d), 16, 0, 0);
+            for (int d = 0; d < DMA; ++d) {
+                const unsigned long long u = (unsigned long long)((d < XI ? xbase : wbase) + at + off[d]);
+                __builtin_amdgcn_global_load_lds((glb_ptr_t)((u & m) | zero), (lds_ptr_t)place(into, d), 16, 0, 0);
+            }
+        } else {
+#pragma unroll
+            for (int d = 0; d < DMA; ++d)
+                *reinterpret_cast<u32x4*>(place(into, d) + lane * 16) = chunk_at((d < XI ? xbase : wbase) + off[d], at, rowb - kx);
         }
     };
 
@@ -314,6 +342,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_tile_kernel(GemmArgs a) 
     constexpr int FPG = TM == 8 ? 2 : TM == 4 ? 3 : 4;       // fragment reads a group of products: done before the last groups
     static_assert(FPG * TM >= TM + TN, "every fragment has its place");
     int cur = 0;                                             // offset of slice s's buffer
+    bool holds = false;                                      // WHOLE false: slice s + 1 is still in `held`
     auto slice = [&](int s, bool fast) __attribute__((always_inline)) {
         wait_counts<63, 0>();                                // the first half's fragments
 #pragma unroll
@@ -321,8 +350,12 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_tile_kernel(GemmArgs a) 
 #pragma unroll
             for (int q = 0; q < FPG; ++q) fetch(cur, 1, j * FPG + q);
             if constexpr (BM == 256) __builtin_amdgcn_s_setprio(1);    // products before the other waves' reads (2 % there; smaller tiles lose by it)
+            column<T, TN, TM>(acc, j, wf[0], xf[0][j]);
+            if constexpr (!WHOLE)
+                if (j == TM / 2 && holds) {
 #pragma unroll
-            for (int i = 0; i < TN; ++i) Elem<T>::mma(acc[i][j], wf[0][i], xf[0][j]);
+                    for (int d = 0; d < DMA; ++d) *reinterpret_cast<u32x4*>(place(BUF - cur, d) + lane * 16) = held[d];
+                }
             if constexpr (BM == 256) __builtin_amdgcn_s_setprio(0);
             __builtin_amdgcn_sched_barrier(0);
         }
@@ -331,6 +364,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_tile_kernel(GemmArgs a) 
         else wait_counts<0, 0>();
         block_barrier();
         if (!fast && s + ST < slices) stage(s + ST, cur);
+        holds = fast;
         const unsigned char *xs = xbase + (long)(s + ST) * 128, *ws = wbase + (long)(s + ST) * 128;
         asm("" : "+s"(xs), "+s"(ws));                        // scalar bases: the lanes add their 32-bit offsets
         const int free = cur;
@@ -343,14 +377,14 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_tile_kernel(GemmArgs a) 
 #pragma unroll
                 for (int d = j * DPG; d < (j + 1) * DPG && d < DMA; ++d) dma(xs, ws, free, d);
             if constexpr (BM == 256) __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-            for (int i = 0; i < TN; ++i) Elem<T>::mma(acc[i][j], wf[1][i], xf[1][j]);
+            column<T, TN, TM>(acc, j, wf[1], xf[1][j]);
             if constexpr (BM == 256) __builtin_amdgcn_s_setprio(0);
             __builtin_amdgcn_sched_barrier(0);
         }
     };
     if (slices) {
         for (int s = 0; s < ST && s < slices; ++s) stage(s, s * BUF);
+        if constexpr (!WHOLE) wait_counts<0, 0>();
         if (slices >= ST) wait_counts<DMA * (ST - 1), 15>();
         else wait_counts<0, 15>();
         block_barrier();
@@ -530,8 +564,8 @@ template <typename T>
 __global__ __launch_bounds__(256) void gemm_any_kernel(GemmArgs a) {
     __shared__ __attribute__((aligned(16))) unsigned char lds[2][64 * 128];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int nt = blockIdx.x % a.n_tiles, mt = blockIdx.x / a.n_tiles;
-    const int n0 = nt * 64;
+    const int mt = blockIdx.z * 65535 + blockIdx.y, n0 = blockIdx.x * 64;
+    if (!a.order && (long)mt * 64 >= a.M) return;
     long r0 = (long)mt * 64, r1 = min(r0 + 64, a.M);
     int expert = 0;
     if (a.order && !expert_tile(a, mt, 64, expert, r0, r1)) return;
@@ -603,14 +637,14 @@ __global__ __launch_bounds__(256) void gemm_any_kernel(GemmArgs a) {
     }
 }
 
-template <typename T, int BM, int BN, int WM, int WN, int ST>
+template <typename T, int BM, int BN, int WM, int WN, int ST, bool WHOLE = true>
 int launch_tile(GemmArgs a, hipStream_t st) {
     const long mt = a.order ? a.M / BM + std::min<long>(a.M, a.E + 1) : (a.M + BM - 1) / BM;
     a.n_tiles = (a.N + BN - 1) / BN;
-    if (mt * a.n_tiles > 0x7FFFFFFFll) FR_FAIL(FR_ERR_UNSUPPORTED, "adapter product: more than 2^31 output tiles");
+    if (mt * a.n_tiles * a.splits >= (1l << 32) / (64 * WM * WN)) FR_FAIL(FR_ERR_UNSUPPORTED, "adapter product: more output tiles than a launch takes");
     const int lds = std::max(ST * (BM + BN) * 128, WM * WN * std::min(64, BM / WM) * (std::min(64, BN / WN) * 4 + 16));    // the ring; the epilogue's rows
-    FR_BIG_LDS_ONCE((gemm_tile_kernel<T, BM, BN, WM, WN, ST>), lds);
-    hipLaunchKernelGGL((gemm_tile_kernel<T, BM, BN, WM, WN, ST>), dim3((unsigned)(mt * a.n_tiles * a.splits)), dim3(64 * WM * WN), lds, st, a);
+    FR_BIG_LDS_ONCE((gemm_tile_kernel<T, BM, BN, WM, WN, ST, WHOLE>), lds);
+    hipLaunchKernelGGL((gemm_tile_kernel<T, BM, BN, WM, WN, ST, WHOLE>), dim3((unsigned)(mt * a.n_tiles * a.splits)), dim3(64 * WM * WN), lds, st, a);
     FR_LAUNCH_CHECK("gemm_tile_kernel");
     return FR_OK;
 }
@@ -632,7 +666,7 @@ template <typename T, int MT, int NW, int R>
 int launch_rows(GemmArgs a, bool whole, hipStream_t st) {
     const long mt = a.order ? a.M / (16 * MT) + std::min<long>(a.M, a.E + 1) : (a.M + 16 * MT - 1) / (16 * MT);
     a.n_tiles = (a.N + 15) / 16;
-    if (mt * a.n_tiles > 0x7FFFFFFFll) FR_FAIL(FR_ERR_UNSUPPORTED, "adapter product: more than 2^31 output tiles");
+    if (mt * a.n_tiles >= (1l << 32) / (64 * NW)) FR_FAIL(FR_ERR_UNSUPPORTED, "adapter product: more output tiles than a launch takes");
     const int lds = NW * R * (16 + 16 * MT) * 128;
     const dim3 grid((unsigned)(mt * a.n_tiles)), block(64 * NW);
     if (whole) {
@@ -667,7 +701,12 @@ int launch_gemm(GemmArgs a, hipStream_t st) {
         if (a.M <= 32 || f32) return launch_rows<T, 2, 8, 3>(a, whole, st);
         return launch_rows<T, 4, 4, 3>(a, whole, st);
     }
-    if (whole && near) {
+    // rows of any alignment, us against gemm_any_kernel: 16384 x 2048 x 4097 bf16 455 and 723, 3001 x 2047 x 2049 68 and 90;
+    // a 64-tile alone on its CU has its chunks sooner there (300 x 1001 x 1001: 18 and 15)
+    const double tiles64 = (a.order ? (double)a.M / 64 + 0.5 * std::min<long>(a.M, a.E) : (double)((a.M + 63) / 64)) * ((a.N + 63) / 64);
+    if (near && (whole || tiles64 > 256)) {
+        const double c256 = slice_cost<T, 256>(a), c128 = slice_cost<T, 128>(a), c64 = slice_cost<T, 64>(a);
+        if (!whole) return c128 <= c64 ? launch_tile<T, 128, 128, 2, 2, 2, false>(a, st) : launch_tile<T, 64, 64, 2, 2, 2, false>(a, st);
         const int splits = a.partial ? split_count(a.M, a.N, a.K, Elem<T>::BYTES == 4 ? FR_TYPE_F32 : FR_TYPE_BF16) : 1;
         if (splits > 1) {
             const long slices = (rowb + 127) / 128;
@@ -679,15 +718,14 @@ int launch_gemm(GemmArgs a, hipStream_t st) {
             FR_LAUNCH_CHECK("gemm_join_kernel");
             return FR_OK;
         }
-        const double c256 = slice_cost<T, 256>(a), c128 = slice_cost<T, 128>(a), c64 = slice_cost<T, 64>(a);
         if (c256 <= c128 && c256 <= c64) return launch_tile<T, 256, 256, 2, 4, 2>(a, st);
         if (c128 <= c64) return launch_tile<T, 128, 128, 2, 2, 2>(a, st);
         return launch_tile<T, 64, 64, 2, 2, 3>(a, st);
     }
     const long mt = a.order ? a.M / 64 + std::min<long>(a.M, a.E + 1) : (a.M + 63) / 64;
     a.n_tiles = (a.N + 63) / 64;
-    if (mt * a.n_tiles > 0x7FFFFFFFll) FR_FAIL(FR_ERR_UNSUPPORTED, "adapter product: more than 2^31 output tiles");
-    hipLaunchKernelGGL((gemm_any_kernel<T>), dim3((unsigned)(mt * a.n_tiles)), dim3(256), 0, st, a);
+    if (mt >= 1l << 24 || a.n_tiles >= 1 << 24) FR_FAIL(FR_ERR_UNSUPPORTED, "adapter product: more output tiles than a launch takes");
+    hipLaunchKernelGGL((gemm_any_kernel<T>), dim3(a.n_tiles, (unsigned)std::min(mt, 65535l), (unsigned)((mt + 65534) / 65535)), dim3(256), 0, st, a);
     FR_LAUNCH_CHECK("gemm_any_kernel");
     return FR_OK;
 }

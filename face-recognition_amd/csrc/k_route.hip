@@ -468,7 +468,7 @@ extern "C" int fr_route(const void* logits, int logits_type, int64_t T, int E, i
                         float* weights, int32_t* experts, int32_t* order, int32_t* offsets,
                         void* workspace, size_t workspace_bytes, void* stream) {
     if (T < 0 || E <= 0 || E > RT_EMAX || k <= 0 || k > RT_KMAX || k > E) FR_FAIL(FR_ERR_ARG, "fr_route: bad shape (E <= 512, k <= min(16, E))");
-    if (T * k > 0x7FFFFFFFll) FR_FAIL(FR_ERR_UNSUPPORTED, "fr_route: T * k does not fit 31 bits");
+    if (T >= 1ll << 30 || T * k > 0x7FFFFFFFll) FR_FAIL(FR_ERR_UNSUPPORTED, "fr_route: T * k does not fit 31 bits, or T 30");
     if (!type_ok(logits_type)) FR_FAIL(FR_ERR_ARG, "fr_route: unknown element type");
     if (score != FR_SCORE_SOFTMAX && score != FR_SCORE_SIGMOID) FR_FAIL(FR_ERR_ARG, "fr_route: unknown score");
     if (groups < 1 || groups > 64 || E % groups || top_groups < 1 || top_groups > groups) FR_FAIL(FR_ERR_ARG, "fr_route: groups (at most 64) must divide E, 1 <= top_groups <= groups");

@@ -263,7 +263,7 @@ int fr_block_norm(const void* x, int x_type, int slots, const float* slot_weight
  * weights [T][k] fp32: the chosen scores, divided by their sum if renormalise, times scale.  experts [T][k] int32, best first.
  * order [T*k] int32: slot numbers t*k + j sorted by expert, stable; the slots without an expert come last.
  * offsets [E+1] int32: expert e's slots are order[offsets[e] .. offsets[e+1]).
- * E <= 512, k <= min(16, E), groups <= 64 dividing E, T*k < 2^31.  workspace: fr_route_workspace_bytes (0 up to 64 rows). */
+ * E <= 512, k <= min(16, E), groups <= 64 dividing E, T < 2^30, T*k < 2^31.  workspace: fr_route_workspace_bytes (0 up to 64 rows). */
 typedef enum fr_score { FR_SCORE_SOFTMAX = 0, FR_SCORE_SIGMOID = 1 } fr_score;
 int fr_route_workspace_bytes(int64_t T, int E, int k, size_t* out_bytes);
 int fr_route(const void* logits, int logits_type, int64_t T, int E, int k, int score, const float* bias,

@@ -496,6 +496,23 @@ def test_block_norm_many_rows():
     check_norm(big[-1:], norm="rms")
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [8, 2056])
+def test_block_norm_more_rows_than_a_launch(d):
+    """2^22 rows a launch."""
+    t = 4200001 if d == 8 else 4194307
+    x = randn(gen(14), t, d, dtype=torch.bfloat16)
+    got = adapter.block_norm(x, norm="layer")
+    for at in (0, 4194296, t - 8):
+        if at < t:
+            part = x[at:at + 8]
+            want, _, tol, _ = norm_ref(part, norm="layer")
+            close(got[at:at + 8], want, tol, at)
+    # rows of every block and turn, against the same rows in a small call
+    pick = torch.randint(0, t, (5000,), generator=gen(15), device="cuda")
+    assert torch.equal(got[pick], adapter.block_norm(x[pick], norm="layer"))
+
+
 # ---- on the GPU: route -------------------------------------------------------------------------------------------------
 
 def check_route(logits, k, what="", **kw):
@@ -694,6 +711,46 @@ def test_expert_linear_tables_that_lie_are_not_followed():
     adapter.expert_linear(x, w, r._replace(offsets=offsets), out="slots")
     adapter.expert_linear(x, w, r._replace(offsets=-offsets), out="sorted")
     torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", ["tokens", "sorted"])
+def test_expert_linear_rows_beyond_32_bits(rows):
+    """x of more than 4 GiB, gathered and in the order's positions."""
+    t, e, k, d, n = 2200000, 3, 1, 1024, 40                    # 4.5 GB of bf16
+    g = gen(35)
+    x = torch.zeros(t, d, dtype=torch.bfloat16, device="cuda")
+    some = torch.tensor([0, 1, 1000000, t - 2, t - 1], device="cuda")
+    x[some] = randn(g, 5, d, dtype=torch.bfloat16)
+    ex = (torch.arange(t, device="cuda") % e).to(torch.int32)[:, None]
+    flat = torch.sort(ex.reshape(-1), stable=True)
+    r = adapter.Routing(torch.ones(t, 1, device="cuda"), ex, flat.indices.to(torch.int32),
+                        torch.searchsorted(flat.values, torch.arange(e + 1, device="cuda", dtype=torch.int32)).to(torch.int32))
+    w = randn(g, e, n, d, dtype=torch.bfloat16, scale=d ** -0.5)
+    got = adapter.expert_linear(x, w, r, rows=rows, out="slots" if rows == "tokens" else "sorted", out_dtype=torch.float32).view(t, n)
+    for i in some.tolist():
+        slot = i if rows == "tokens" else int(r.order[i])      # sorted: row i stands at position i of the order
+        m = w[int(ex[slot])]
+        want = oa.linear(x[i][None], m)
+        close(got[i][None], want, linear_tol(x[i][None], m, None, None, want, torch.float32), (rows, i))
+    keep = torch.ones(t, dtype=torch.bool, device="cuda")
+    keep[some] = False
+    assert not got[keep].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("m, k, n", [(1100, 333, 1100), (1300, 130, 1500), (2000, 65, 2000), (1500, 519, 1030)])
+def test_linear_large_rows_of_any_alignment(kind, m, k, n):
+    g, dt = gen(m + k), TYPES[kind]
+    x, w, b = randn(g, m, k, dtype=dt), randn(g, n, k, dtype=dt, scale=k ** -0.5), randn(g, n)
+    want = oa.linear(x, w, b, name="relu")
+    close(adapter.linear(x, w, b, act="relu"), want, linear_tol(x, w, b, None, want, dt), (kind, m, k, n))
+    shifted = torch.empty(m * 384 + 8, dtype=dt, device="cuda")[3:3 + m * 384].view(m, 384)      # whole chunks a row, but not at 16 bytes
+    shifted.copy_(randn(g, m, 384, dtype=dt))
+    w = randn(g, n, 384, dtype=dt, scale=0.05)
+    want = oa.linear(shifted, w)
+    close(adapter.linear(shifted, w), want, linear_tol(shifted, w, None, None, want, dt), "shifted")
 
 
 @pytest.mark.gpu
