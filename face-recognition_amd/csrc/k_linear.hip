@@ -68,8 +68,10 @@ FR_DEV bool expert_tile(const GemmArgs& a, int tile, int bm, int& expert, long& 
             const int first = before + __shfl(s - nt, f, 64);
             lo = __shfl(lo, f, 64); hi = __shfl(hi, f, 64);
             expert = __builtin_amdgcn_readfirstlane(e0 + f);
-            r0 = __builtin_amdgcn_readfirstlane(lo + (tile - first) * bm);
-            r1 = min(r0 + bm, (long)__builtin_amdgcn_readfirstlane(hi));
+            const long begin = __builtin_amdgcn_readfirstlane(lo), end = __builtin_amdgcn_readfirstlane(hi);
+            r0 = begin + (long)__builtin_amdgcn_readfirstlane(tile - first) * bm;
+            r1 = min(r0 + bm, end);
+            if (r0 < begin || r0 >= end) return false;       // only where the counts of a table that lies have overflowed
             return true;
         }
         before += __shfl(s, 63, 64);
@@ -460,79 +462,73 @@ __global__ __launch_bounds__(64 * NW) void gemm_rows_kernel(GemmArgs a) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int li = lane & 15, lg = lane >> 4;
     const int nt = blockIdx.x % a.n_tiles, mt = blockIdx.x / a.n_tiles, n0 = nt * 16;
-    long r0 = (long)mt * 16 * MT, r1 = min(r0 + 16 * MT, a.M);
-    int expert = 0;
-    if (a.order && !expert_tile(a, mt, 16 * MT, expert, r0, r1)) return;
-    const bool none = a.order && expert == a.E;
-    const long nbase = (long)expert * a.N, rowb = (long)a.K * Elem<T>::BYTES;
+    const long r0 = (long)mt * 16 * MT, r1 = min(r0 + 16 * MT, a.M), rowb = (long)a.K * Elem<T>::BYTES;
     f32x4 acc[MT];
 #pragma unroll
     for (int j = 0; j < MT; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
     unsigned char* ring = smem + wave * R * SLOT;
-    if (!none) {
-        // this lane's sources: row 8 d + lane / 8 of the 16 weight rows and then those of x, chunk (lane % 8) ^ key
-        const unsigned char* src[DPS];
-        int kx[2];                                           // the key of row r is that of r + 16
+    // this lane's sources: row 8 d + lane / 8 of the 16 weight rows and then those of x, chunk (lane % 8) ^ key
+    const unsigned char* src[DPS];
+    int kx[2];                                           // the key of row r is that of r + 16
 #pragma unroll
-        for (int d = 0; d < 2; ++d) kx[d] = ((lane & 7) ^ (((8 * d + (lane >> 3)) >> 1) & 7)) * 16;
+    for (int d = 0; d < 2; ++d) kx[d] = ((lane & 7) ^ (((8 * d + (lane >> 3)) >> 1) & 7)) * 16;
 #pragma unroll
-        for (int d = 0; d < DPS; ++d) {
-            const int r = 8 * d + (lane >> 3);
-            src[d] = (d < 2 ? reinterpret_cast<const unsigned char*>(a.w) + (nbase + min(n0 + r, a.N - 1)) * rowb
-                            : reinterpret_cast<const unsigned char*>(a.x) + x_row(a, min(r0 + r - 16, r1 - 1)) * a.ldx * Elem<T>::BYTES) + kx[d & 1];
+    for (int d = 0; d < DPS; ++d) {
+        const int r = 8 * d + (lane >> 3);
+        src[d] = (d < 2 ? reinterpret_cast<const unsigned char*>(a.w) + (long)min(n0 + r, a.N - 1) * rowb
+                        : reinterpret_cast<const unsigned char*>(a.x) + min(r0 + r - 16, r1 - 1) * a.ldx * Elem<T>::BYTES) + kx[d & 1];
+    }
+    const int slices = (int)((rowb + 127) / 128), mine = (slices - wave + NW - 1) / NW;    // <= 0: more waves than slices
+    auto multiply = [&](const unsigned char* slot) __attribute__((always_inline)) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int at = li * 128 + (((4 * h + lg) ^ ((li >> 1) & 7)) << 4);
+            const u32x4 w = *reinterpret_cast<const u32x4*>(slot + at);
+            u32x4 x[MT];
+#pragma unroll
+            for (int j = 0; j < MT; ++j) x[j] = *reinterpret_cast<const u32x4*>(slot + (j + 1) * 2048 + at);
+#pragma unroll
+            for (int j = 0; j < MT; ++j) Elem<T>::mma(acc[j], w, x[j]);
         }
-        const int slices = (int)((rowb + 127) / 128), mine = (slices - wave + NW - 1) / NW;    // <= 0: more waves than slices
-        auto multiply = [&](const unsigned char* slot) __attribute__((always_inline)) {
+    };
+    if constexpr (WHOLE) {
+        auto stage = [&](int i, int slot) __attribute__((always_inline)) {
+            const long at = (long)(wave + i * NW) * 128;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int at = li * 128 + (((4 * h + lg) ^ ((li >> 1) & 7)) << 4);
-                const u32x4 w = *reinterpret_cast<const u32x4*>(slot + at);
-                u32x4 x[MT];
-#pragma unroll
-                for (int j = 0; j < MT; ++j) x[j] = *reinterpret_cast<const u32x4*>(slot + (j + 1) * 2048 + at);
-#pragma unroll
-                for (int j = 0; j < MT; ++j) Elem<T>::mma(acc[j], w, x[j]);
+            for (int d = 0; d < DPS; ++d) {
+                const unsigned lo = at + kx[d & 1] >= rowb ? 0u : ~0u;       // K may end inside the slice: zeros behind it
+                const unsigned long long m = ((unsigned long long)lo << 32) | lo;
+                const unsigned long long u = ((unsigned long long)(src[d] + at) & m) | ((unsigned long long)&g_zero16 & ~m);
+                __builtin_amdgcn_global_load_lds((glb_ptr_t)u, (lds_ptr_t)(ring + slot * SLOT + d * 1024), 16, 0, 0);
             }
         };
-        if constexpr (WHOLE) {
-            auto stage = [&](int i, int slot) __attribute__((always_inline)) {
-                const long at = (long)(wave + i * NW) * 128;
 #pragma unroll
-                for (int d = 0; d < DPS; ++d) {
-                    const unsigned lo = at + kx[d & 1] >= rowb ? 0u : ~0u;       // K may end inside the slice: zeros behind it
-                    const unsigned long long m = ((unsigned long long)lo << 32) | lo;
-                    const unsigned long long u = ((unsigned long long)(src[d] + at) & m) | ((unsigned long long)&g_zero16 & ~m);
-                    __builtin_amdgcn_global_load_lds((glb_ptr_t)u, (lds_ptr_t)(ring + slot * SLOT + d * 1024), 16, 0, 0);
-                }
-            };
+        for (int i = 0; i < R; ++i)
+            if (i < mine) stage(i, i);
+        int slot = 0;
+        for (int i = 0; i < mine; ++i) {
+            if (i + R <= mine) wait_counts<(R - 1) * DPS, 15>();
+            else wait_counts<0, 15>();
+            multiply(ring + slot * SLOT);
+            wait_counts<63, 0>();
+            if (i + R < mine) stage(i + R, slot);
+            slot = slot + 1 == R ? 0 : slot + 1;
+        }
+    } else {
+        u32x4 c[DPS];
+        auto fetch = [&](int i) __attribute__((always_inline)) {
+            const long at = (long)(wave + i * NW) * 128;
 #pragma unroll
-            for (int i = 0; i < R; ++i)
-                if (i < mine) stage(i, i);
-            int slot = 0;
-            for (int i = 0; i < mine; ++i) {
-                if (i + R <= mine) wait_counts<(R - 1) * DPS, 15>();
-                else wait_counts<0, 15>();
-                multiply(ring + slot * SLOT);
-                wait_counts<63, 0>();
-                if (i + R < mine) stage(i + R, slot);
-                slot = slot + 1 == R ? 0 : slot + 1;
-            }
-        } else {
-            u32x4 c[DPS];
-            auto fetch = [&](int i) __attribute__((always_inline)) {
-                const long at = (long)(wave + i * NW) * 128;
+            for (int d = 0; d < DPS; ++d) c[d] = chunk_at(src[d], at, rowb - kx[d & 1]);
+        };
+        if (mine > 0) fetch(0);
+        for (int i = 0; i < mine; ++i) {
 #pragma unroll
-                for (int d = 0; d < DPS; ++d) c[d] = chunk_at(src[d], at, rowb - kx[d & 1]);
-            };
-            if (mine > 0) fetch(0);
-            for (int i = 0; i < mine; ++i) {
-#pragma unroll
-                for (int d = 0; d < DPS; ++d) *reinterpret_cast<u32x4*>(ring + d * 1024 + lane * 16) = c[d];
-                if (i + 1 < mine) fetch(i + 1);
-                wave_lds_fence();
-                multiply(ring);
-                wave_lds_fence();
-            }
+            for (int d = 0; d < DPS; ++d) *reinterpret_cast<u32x4*>(ring + d * 1024 + lane * 16) = c[d];
+            if (i + 1 < mine) fetch(i + 1);
+            wave_lds_fence();
+            multiply(ring);
+            wave_lds_fence();
         }
     }
     __syncthreads();
@@ -550,12 +546,9 @@ __global__ __launch_bounds__(64 * NW) void gemm_rows_kernel(GemmArgs a) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) { v.v[e] += lo[e]; v.v[4 + e] += hi[e]; }
     }
-    const long p = r0 + 16 * j + i;
-    if (p >= r1) return;
-    const long row = out_row(a, p);
+    const long row = r0 + 16 * j + i;
     const int n = n0 + half * 8;
-    if (row < 0 || n >= a.N) return;
-    finish8(a, row, n, columns(a, n, min(8, a.N - n), nbase, none), v, none);
+    if (row < r1 && n < a.N) finish8(a, row, n, columns(a, n, min(8, a.N - n), 0, false), v, false);
 }
 
 // Any shape, any alignment: 64 x 64 outputs a block, 4 waves of 32 x 32, slices of 128 bytes of K through registers into
@@ -664,7 +657,7 @@ double slice_cost(const GemmArgs& a) {
 
 template <typename T, int MT, int NW, int R>
 int launch_rows(GemmArgs a, bool whole, hipStream_t st) {
-    const long mt = a.order ? a.M / (16 * MT) + std::min<long>(a.M, a.E + 1) : (a.M + 16 * MT - 1) / (16 * MT);
+    const long mt = (a.M + 16 * MT - 1) / (16 * MT);
     a.n_tiles = (a.N + 15) / 16;
     if (mt * a.n_tiles >= (1l << 32) / (64 * NW)) FR_FAIL(FR_ERR_UNSUPPORTED, "adapter product: more output tiles than a launch takes");
     const int lds = NW * R * (16 + 16 * MT) * 128;

@@ -279,6 +279,8 @@ def _linear_shape(op, x, weight, residual):
     xs, ws = x.shape, weight.shape
     if len(xs) < 1 or len(ws) != 2 or xs[-1] != ws[1] or ws[1] < 1 or ws[0] < 1:
         _fail(op, f"expected x [..., K] and weight [N, K]: got {tuple(xs)} and {tuple(ws)}")
+    if max(ws) >= 1 << 31:
+        _fail(op, f"N and K have to fit 31 bits: got {tuple(ws)}")
     shape = xs[:-1] + ws[:1]
     if residual is not None and residual.shape != shape:
         _fail(op, f"residual is {tuple(shape)}: got {tuple(residual.shape)}")
@@ -332,8 +334,12 @@ def _block_norm_shape(op, x, slot_weights):
     least = 1 if slot_weights is None else 2
     if x.dim() < least or x.shape[-1] < 1:
         _fail(op, f"expected x [..., d], or [..., slots, d] with slot_weights: got {tuple(x.shape)}")
+    if x.shape[-1] > 16384:
+        _fail(op, f"d is at most 16384: got {x.shape[-1]}")
     if slot_weights is None:
         return x.shape
+    if x.shape[-2] >= 1 << 31:
+        _fail(op, "slots have to fit 31 bits")
     if slot_weights.shape != x.shape[:-1] or slot_weights.dtype != torch.float32 or x.shape[-2] < 1:
         _fail(op, f"slot_weights is float32 {tuple(x.shape[:-1])}: got {slot_weights.dtype} {tuple(slot_weights.shape)}")
     return x.shape[:-2] + x.shape[-1:]
@@ -402,8 +408,10 @@ def _route_shape(op, logits, k):
     if logits.dim() != 2 or logits.shape[1] < 1:
         _fail(op, f"expected logits [T, E]: got {tuple(logits.shape)}")
     T, E = logits.shape
-    if not 1 <= k <= E:
-        _fail(op, f"1 <= k <= {E} experts: got {k}")
+    if E > 512:
+        _fail(op, f"at most 512 experts: got {E}")
+    if not 1 <= k <= min(E, 16):
+        _fail(op, f"1 <= k <= 16 of {E} experts: got {k}")
     return T, E
 
 
@@ -418,6 +426,8 @@ def _route(logits, k, score, bias, groups, top_groups, renormalise, scale):
     op = "route"
     dev = _check_tensors(op, logits, bias)
     T, E = _route_shape(op, logits, k)
+    if not 1 <= groups <= 64 or not 1 <= top_groups <= groups:
+        _fail(op, f"1 <= top_groups <= groups <= 64: got {top_groups} of {groups}")
     kind = _type(op, "logits", logits.dtype)
     score = _name(op, _SCORES, score, "score")
     bias = _vector(op, "bias", bias, E, (torch.float32,))
@@ -437,8 +447,10 @@ def _expert_shape(op, x, weight, order, offsets, k, rows, out):
         _fail(op, f"rows is 'tokens' or 'sorted', out 'sorted' or 'slots': got {rows!r}, {out!r}")
     if order.dtype != torch.int32 or offsets.dtype != torch.int32 or order.dim() != 1 or offsets.shape != (weight.shape[0] + 1,):
         _fail(op, f"expected int32 order [T*k] and offsets [{weight.shape[0] + 1}] as route returns them")
-    if k < 1 or order.shape[0] % k:
-        _fail(op, f"{order.shape[0]} slots are no multiple of k = {k}")
+    if k < 1 or order.shape[0] % k or order.shape[0] >= 1 << 31:
+        _fail(op, f"{order.shape[0]} slots are no multiple of k = {k} below 2^31")
+    if max(weight.shape) >= 1 << 31:
+        _fail(op, f"E, N and K have to fit 31 bits: got {tuple(weight.shape)}")
     T = order.shape[0] // k
     if x.shape[0] != (T if rows == "tokens" else T * k):
         _fail(op, f"rows={rows!r} takes {T if rows == 'tokens' else T * k} rows of x: got {x.shape[0]}")

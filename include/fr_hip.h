@@ -244,7 +244,8 @@ int fr_linear(const void* x, int64_t ldx, const void* w, const void* bias, const
  * weight / bias / next_weight / next_bias: fp32 [d] or NULL (= 1 / 0).  gate of gate_type or NULL, element (t, c) at
  * gate[t * gate_ldt + c * gate_ldc] (strides 0 = broadcast; gate_ldc 0 or 1); g by gate_act (FR_GATE_*).  residual [T][d] of
  * res_type (row stride d) or NULL.  out [T][d] of out_type or NULL (not wanted); next_out [T][d] of next_type, or NULL
- * with FR_NORM_NONE as next_norm.  d <= 16384.  out and next_out may not overlap each other; residual may be `out`. */
+ * with FR_NORM_NONE as next_norm.  d <= 16384.  out and next_out may not overlap each other; residual may be `out`.
+ * Squares are summed in fp32: the norms are those of rows whose elements lie between about 1e-19 and 1e18 in magnitude. */
 typedef enum fr_norm { FR_NORM_NONE = 0, FR_NORM_RMS = 1, FR_NORM_LAYER = 2, FR_NORM_L2 = 3 } fr_norm;
 typedef enum fr_gate_act { FR_GATE_NONE = 0, FR_GATE_SIGMOID = 1, FR_GATE_TANH = 2 } fr_gate_act;
 int fr_block_norm(const void* x, int x_type, int slots, const float* slot_weights, int64_t T, int d,

@@ -82,6 +82,7 @@ LINEAR = dict(bias=None, slope=None, residual=None, act="none", out_dtype=None)
     (dict(weight=torch.zeros(0, 8)), "weight"), (dict(x=torch.zeros(2, 0), weight=torch.zeros(4, 0)), "weight"),
     (dict(x=torch.zeros(2, 8, requires_grad=True)), "inference only"), (dict(bias=torch.zeros(4, requires_grad=True)), "inference only"),
     (dict(weight=torch.zeros(4, 8, device="meta")), "all tensors on"),
+    (dict(x=torch.zeros(1, 1).expand(1, (1 << 32) + 8), weight=torch.zeros(1, 1).expand(4, (1 << 32) + 8)), "31 bits"),
 ])
 def test_linear_refuses(change, words):
     with pytest.raises(RuntimeError, match=words):
@@ -99,6 +100,7 @@ NORM = dict(residual=None, slot_weights=None, norm="rms", weight=None, bias=None
     (dict(residual=torch.zeros(3, 8)), "residual"), (dict(gate=torch.zeros(2)), "gate"), (dict(gate=torch.zeros(8), gate_act="relu"), "gate_act"),
     (dict(gate=torch.zeros(8, dtype=torch.int64)), "gate"), (dict(slot_weights=torch.zeros(3)), "slot_weights"),
     (dict(slot_weights=torch.zeros(2).half()), "slot_weights"), (dict(x=torch.zeros(2, 8, requires_grad=True)), "inference only"),
+    (dict(x=torch.zeros(1, 16385)), "16384"), (dict(x=torch.zeros(1, dtype=torch.float32).expand((1 << 32) + 8)), "16384"),
     (dict(x=torch.zeros(2, 8, dtype=torch.float64)), "float32, bfloat16"), (dict(next_dtype=torch.int32, next_norm="l2"), "next_dtype"),
 ])
 def test_block_norm_refuses(change, words):
@@ -110,6 +112,7 @@ ROUTE = dict(k=2, score="softmax", bias=None, groups=1, top_groups=1, renormalis
 
 
 @pytest.mark.parametrize("change, words", [
+    (dict(groups=0), "groups"), (dict(groups=(1 << 32) + 1), "groups"), (dict(groups=2, top_groups=3), "groups"), (dict(groups=4, top_groups=0), "groups"),
     (dict(logits=torch.zeros(8)), "expected logits"), (dict(logits=torch.zeros(2, 0)), "expected logits"), (dict(k=0), "experts"), (dict(k=9), "experts"),
     (dict(score="relu"), "score"), (dict(bias=torch.zeros(7)), "bias"), (dict(bias=torch.zeros(8).half()), "bias"),
     (dict(logits=torch.zeros(2, 8, dtype=torch.int32)), "logits"), (dict(logits=torch.zeros(2, 600)), "512"),
@@ -875,6 +878,26 @@ def test_streams_and_graphs():
             a(xs[0])
             torch.cuda.synchronize()
             assert torch.equal(out, eager), (turn, j)
+
+
+@pytest.mark.gpu
+def test_dispatched_ops_answer_as_the_functions_do():
+    """torch.ops.fr_hip goes through the dispatcher, the functions of adapter straight to the implementation."""
+    g = gen(50)
+    x, w, b = randn(g, 20, 64), randn(g, 48, 64), randn(g, 48)
+    o = torch.ops.fr_hip
+    assert torch.equal(o.linear(x, w, b, None, None, "gelu", torch.bfloat16), adapter.linear(x, w, b, act="gelu", out_dtype=torch.bfloat16))
+    out, nxt = o.block_norm(x, None, None, "rms", None, None, 1e-6, None, "none", 1.0, "l2", None, None, 1e-6, None, torch.bfloat16)
+    want = adapter.block_norm(x, next_norm="l2", next_dtype=torch.bfloat16)
+    assert torch.equal(out, want[0]) and torch.equal(nxt, want[1])
+    out, nxt = o.block_norm(x, None, None, "rms", None, None, 1e-6, None, "none", 1.0, "none", None, None, 1e-6, None, None)
+    assert torch.equal(out, adapter.block_norm(x)) and nxt.numel() == 0
+    got = o.route(x, 3, "softmax", None, 4, 2, True, 1.0)
+    r = adapter.route(x, 3, groups=4, top_groups=2)
+    assert all(torch.equal(a, c) for a, c in zip(got, r))
+    we = randn(g, 64, 16, 64)
+    assert torch.equal(o.expert_linear(x, we, r.order, r.offsets, 3, None, "none", None, "tokens", "slots", None),
+                       adapter.expert_linear(x, we, r, out="slots"))
 
 
 @pytest.mark.gpu
