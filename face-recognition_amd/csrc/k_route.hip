@@ -35,11 +35,29 @@ FR_DEV unsigned row_fold(unsigned v, F f) {
     return v;
 }
 template <int LPR> FR_DEV unsigned row_maxu(unsigned v) { return row_fold<LPR>(v, [](unsigned x, unsigned y) { return max(x, y); }); }
+template <int LPR> FR_DEV unsigned row_addu(unsigned v) { return row_fold<LPR>(v, [](unsigned x, unsigned y) { return x + y; }); }
 template <int LPR> FR_DEV float row_max(float v) {
     return __uint_as_float(row_fold<LPR>(__float_as_uint(v), [](unsigned x, unsigned y) { return __float_as_uint(fmaxf(__uint_as_float(x), __uint_as_float(y))); }));
 }
 template <int LPR> FR_DEV float row_sum(float v) {
     return __uint_as_float(row_fold<LPR>(__float_as_uint(v), [](unsigned x, unsigned y) { return __float_as_uint(__uint_as_float(x) + __uint_as_float(y)); }));
+}
+
+// N unsigned numbers in descending order (Batcher's odd-even merge sort: 63 exchanges for 16, 19 for 8).
+template <int N>
+FR_DEV void sort_down(unsigned (&v)[N]) {
+#pragma unroll
+    for (int p = 1; p < N; p *= 2)
+#pragma unroll
+        for (int k = p; k >= 1; k /= 2)
+#pragma unroll
+            for (int j = k % p; j <= N - 1 - k; j += 2 * k)
+#pragma unroll
+                for (int i = 0; i < k; ++i)
+                    if (i + j + k < N && (i + j) / (p * 2) == (i + j + k) / (p * 2)) {
+                        const unsigned hi = max(v[i + j], v[i + j + k]), lo = min(v[i + j], v[i + j + k]);
+                        v[i + j] = hi; v[i + j + k] = lo;
+                    }
 }
 
 // The weight of a chosen expert with logit l, `top` the greatest chosen logit, m and z the row's greatest and its sum of
@@ -238,8 +256,9 @@ FR_DEV void first_places(const RouteArgs& a, int* next, bool write, F n, G more)
     wave_lds_fence();
 }
 
-// A row takes LPR lanes, a lane up to V experts of one group, in index order over the lanes.  The k best come from k maxima
-// over the row of keys that are unique in their lane: f32 in unsigned order, the low NB bits replaced by an index (greater for lower
+// A row takes LPR > k lanes, a lane up to V experts of one group, in index order over the lanes.  A lane sorts its keys, and
+// the k best (and one more, for the doubt) are maxima over the row of the lanes' heads.  Keys are unique in their lane: f32
+// in unsigned order, the low NB bits replaced by an index (greater for lower
 // ones).  Unscored rows (no bias, one group) order by the logits themselves and put the expert's number there: unique in
 // the row, ties need no care, and with 16-bit logits nothing is lost.  Scored rows put the place in the lane there, 4 bits.
 // A row is done again by the whole wave in doubles where f32 cannot vouch for the choice: where two neighbours in the order
@@ -259,7 +278,10 @@ __global__ __launch_bounds__(64 * RT_WAVES, 4) void route_choose_kernel(RouteArg
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, rl = lane % LPR, base = lane - rl;
     for (int e = threadIdx.x; e <= a.E; e += blockDim.x) count[e] = 0;
     if constexpr (SCORED)                                    // in LDS: registers are what limits the waves a SIMD holds
-        for (int e = threadIdx.x; e < RT_EMAX + V; e += blockDim.x) bias[e] = a.bias && e < a.E ? a.bias[e] : 0.f;
+        for (int e = threadIdx.x; e < RT_EMAX + V; e += blockDim.x) {
+            const float b = a.bias && e < a.E ? a.bias[e] : 0.f;
+            bias[e] = b > -INFINITY ? b : -INFINITY;         // NaN masks too; added to a score, -inf masks it
+        }
     __syncthreads();
     static_assert(!SCORED || V <= 1 << NB, "a lane's keys are unique");
     const bool need_z = SCORED || !a.renormalise;
@@ -305,14 +327,14 @@ __global__ __launch_bounds__(64 * RT_WAVES, 4) void route_choose_kernel(RouteArg
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 const float s = a.score == FR_SCORE_SOFTMAX ? f[v] * rz : __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-l[v] * L2E));
-                const float b = bias[min(e0, RT_EMAX) + v];
-                f[v] = l[v] > -INFINITY && b > -INFINITY ? s + b : -INFINITY;
+                f[v] = l[v] > -INFINITY ? s + bias[min(e0, RT_EMAX) + v] : -INFINITY;
             }
         } else {
 #pragma unroll
             for (int v = 0; v < V; ++v) f[v] = l[v] + 0.f;   // -0 is 0
         }
-        bool doubt = false, kept = true;
+        bool doubt = false;
+        unsigned kept = ~0u;                                 // all bits or none
         if (SCORED && a.groups > 1) {
             float b1 = -INFINITY, b2 = -INFINITY;
 #pragma unroll
@@ -333,51 +355,51 @@ __global__ __launch_bounds__(64 * RT_WAVES, 4) void route_choose_kernel(RouteArg
                 const float v = __shfl(sum, base + o * LG, 64);
                 if (v > sum || (v == sum && o < g)) ++rank;
             }
-            kept = g < a.groups && rank < a.top_groups;
+            const bool keep = g < a.groups && rank < a.top_groups;
+            kept = keep ? ~0u : 0u;
             if (a.top_groups < a.groups) {                   // sums of two: twice the error
-                const float least = -row_max<LPR>(kept ? -sum : -INFINITY), most = row_max<LPR>(!kept && g < a.groups ? sum : -INFINITY);
-                doubt = !(least - most > 2.f * slack * fmaxf(1.f, fabsf(least)));
+                const float least = -row_max<LPR>(keep ? -sum : -INFINITY), most = row_max<LPR>(!keep && g < a.groups ? sum : -INFINITY);
+                // a row without any eligible expert needs no second look
+                doubt = !(least - most > 2.f * slack * fmaxf(1.f, fabsf(least))) && row_max<LPR>(b1) > -INFINITY;
             }
         }
-        unsigned key[V];                                     // 0: not to be chosen
+        unsigned key[V];                                     // up to that of -inf: not to be chosen
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             unsigned u = __float_as_uint(f[v]);
             u ^= (unsigned)((int)u >> 31) | 0x80000000u;
-            key[v] = kept && f[v] > -INFINITY ? (u & ~MASK) | (MASK - (unsigned)(SCORED ? v : e0 + v)) : 0u;
+            key[v] = ((u & ~MASK) | (MASK - (unsigned)(SCORED ? v : e0 + v))) & kept;
         }
-        if (SCORED && a.groups > 1) {                        // a row without any eligible expert needs no second look
-            unsigned live = 0;
-#pragma unroll
-            for (int v = 0; v < V; ++v) live |= f[v] > -INFINITY ? 1u : 0u;
-            doubt = doubt && row_maxu<LPR>(live);
-        }
-        unsigned mine = 0, last = 0;
+        constexpr unsigned LEAST = 0x007FFFFFu | MASK;
+        sort_down<V>(key);
+        unsigned mine = 0, wins = 0;                         // lane j <= k of the row: its j-th key
         if (SCORED && rl < a.k) chosen[r * a.k + rl] = -1;
         wave_lds_fence();
         for (int j = 0; j <= a.k; ++j) {
-            unsigned own = key[0];
-#pragma unroll
-            for (int v = 1; v < V; ++v) own = max(own, key[v]);
-            const unsigned top = row_maxu<LPR>(own);
-            if (j > 0 && top) {
-                const unsigned x = last & ~MASK, y = top & ~MASK;
-                if constexpr (!SCORED) doubt |= a.type == FR_TYPE_F32 && x == y;
-                else {
-                    const float fx = __uint_as_float(x & 0x80000000u ? x ^ 0x80000000u : ~x), fy = __uint_as_float(y & 0x80000000u ? y ^ 0x80000000u : ~y);
-                    doubt |= !(fx - fy > slack * fmaxf(1.f, fabsf(fx)) + 2.f * DROP * fmaxf(fabsf(fx), fabsf(fy)));
-                }
-            }
-            if (j == a.k) break;
-            last = top;
+            const unsigned max0 = row_maxu<LPR>(key[0]), top = max0 > LEAST ? max0 : 0u;
+            if (rl == j) mine = top;
+            const bool here = key[0] == top && top;
             if constexpr (SCORED) {
-                const bool here = own == top && top;
-                if (here) chosen[r * a.k + j] = e0 + (int)(MASK - (top & MASK));
-                const unsigned long long who = (__ballot(here) >> base) & (LPR == 64 ? ~0ull : (1ull << (LPR & 63)) - 1);
-                doubt |= __popcll(who) > 1;                  // equal keys of two lanes
-            } else if (rl == j) mine = top;
+                if (here && j < a.k) chosen[r * a.k + j] = e0 + (int)(MASK - (top & MASK));
+                wins += here;
+            }
+            const unsigned pop = here ? ~0u : 0u;            // the winner's next key moves up: one bit select a key
 #pragma unroll
-            for (int v = 0; v < V; ++v) key[v] = key[v] == top ? 0u : key[v];
+            for (int v = 0; v + 1 < V; ++v) key[v] = (key[v + 1] & pop) | (key[v] & ~pop);
+            key[V - 1] &= ~pop;
+        }
+        {
+            const unsigned x = (unsigned)__shfl((int)mine, max(lane - 1, base), 64) & ~MASK, y = mine & ~MASK;
+            bool close = false;                              // this lane's key to the one before
+            if constexpr (!SCORED) close = a.type == FR_TYPE_F32 && x == y;
+            else {
+                const float fx = __uint_as_float(x & 0x80000000u ? x ^ 0x80000000u : ~x), fy = __uint_as_float(y & 0x80000000u ? y ^ 0x80000000u : ~y);
+                close = !(fx - fy > slack * fmaxf(1.f, fabsf(fx)) + 2.f * DROP * fmaxf(fabsf(fx), fabsf(fy)));
+            }
+            unsigned flag = close && mine && rl > 0 && rl <= a.k;
+            // equal keys of two lanes win the same round: more wins than keys
+            if constexpr (SCORED) flag |= row_addu<LPR>(wins) != row_addu<LPR>(mine && rl <= a.k ? 1u : 0u);
+            doubt |= row_maxu<LPR>(flag) != 0;
         }
         // lane j < k of the row: its j-th choice
         if (!SCORED && rl < a.k) chosen[r * a.k + rl] = mine ? (int)(MASK - (mine & MASK)) : -1;
@@ -482,8 +504,8 @@ extern "C" int fr_route(const void* logits, int logits_type, int64_t T, int E, i
                 logits_type, E, k, score, groups, top_groups, renormalise, (int)((T + RT_ROWS - 1) / RT_ROWS), scale};
     hipStream_t st = (hipStream_t)stream;
     if (a.chunks == 0) a.chunks = 1;                          // no rows: the offsets are written all the same
-    // lanes a row takes: every group a whole number of them, and one for each of the k choices
-    const int V = E <= 64 && groups == 1 ? 8 : 16, per = E / groups, lanes = std::max(groups * ((per + V - 1) / V), k);
+    // lanes a row takes: every group a whole number of them, and one for each of the k choices and the one behind them
+    const int V = E <= 64 && groups == 1 ? 8 : 16, per = E / groups, lanes = std::max(groups * ((per + V - 1) / V), k + 1);
     if (V == 8 && lanes <= 8) launch_choose<8, 8, 1, 6>(a, st);
     else if (lanes <= 8 && E <= 128) launch_choose<16, 8, 2, 8>(a, st);
     else if (lanes <= 16 && E <= 256) launch_choose<16, 16, 4, 8>(a, st);
