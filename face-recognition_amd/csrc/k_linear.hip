@@ -275,7 +275,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_tile_kernel(GemmArgs a) 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int li = lane & 15, lg = lane >> 4, wm = wave / WN, wn = wave % WN;
     int mtiles = (int)((a.M + BM - 1) / BM), mt, nt, expert = 0;
-    if (a.order) mtiles = expert_tiles(a, BM);
+    if (a.order) mtiles = min(expert_tiles(a, BM), (int)(gridDim.x / a.n_tiles));     // the second: tables that lie
     const int tiles = mtiles * a.n_tiles, split = a.splits > 1 ? blockIdx.x / tiles : 0;
     if ((int)blockIdx.x - split * tiles >= tiles || split >= a.splits) return;     // experts: the grid is an upper bound
     tile_of_block(blockIdx.x - split * tiles, mtiles, a.n_tiles, mt, nt);
@@ -642,17 +642,19 @@ int launch_tile(GemmArgs a, hipStream_t st) {
     return FR_OK;
 }
 
-// Time of a slice of 128 bytes of K with as many tiles on the fullest CU as this shape gives it, in us, measured on one
-// card: 256-tiles one after the other, 128-tiles two, 64-tiles three at a time; a tile alone on its CU waits for memory.
-// fp32 is bound by its matrix instructions whatever the tile: there only the rounding to whole tiles differs.
-template <typename T, int B>
-double slice_cost(const GemmArgs& a) {
-    const double rows = a.order ? (double)a.M / B + 0.5 * std::min<long>(a.M, a.E) : (double)((a.M + B - 1) / B);
-    const double on_cu = ceil(rows * ((a.N + B - 1) / B) / 256.0);
+// Output tiles of bm x bn; of the experts' products an estimate (the counts are on the device): half a tile more for each.
+double tile_count(const GemmArgs& a, int bm, int bn) {
+    const double some = a.order ? (double)std::min<long>(a.M, a.E) : 0;
+    const double rows = a.order ? std::max((double)a.M / bm + 0.5 * some, some) : (double)((a.M + bm - 1) / bm);
+    return rows * ((a.N + bn - 1) / bn);
+}
+// Estimated time in us with tiles of bm x bn: `each` for a slice of 128 bytes of K and `fixed` for the rest of a tile, for every
+// tile of the fullest CU.  The constants are least squares over 90 shapes of 64 to 18 000 rows on one card (rms 3 % in fp32,
+// 10 to 15 % in 16 bits); what the rule picks took 1.4 % more than the best of all tiles there (fp32: 1.8 %).
+template <typename T>
+double tile_cost(const GemmArgs& a, int bm, int bn, double each16, double fixed16, double each32, double fixed32) {
     constexpr bool f32 = std::is_same<T, float>::value;
-    const double alone = B == 256 ? (f32 ? 6.8 : 1.33) : B == 128 ? (f32 ? 1.9 : 0.75) : (f32 ? 0.6 : 0.32);
-    const double each = B == 256 ? (f32 ? 6.8 : 1.55) : B == 128 ? (f32 ? 1.72 : 0.475) : (f32 ? 0.44 : 0.19);
-    return on_cu <= 1 ? alone : std::max(alone, on_cu * each);
+    return ceil(tile_count(a, bm, bn) / 256) * (((long)a.K * Elem<T>::BYTES + 127) / 128 * (f32 ? each32 : each16) + (f32 ? fixed32 : fixed16));
 }
 
 template <typename T, int MT, int NW, int R>
@@ -696,10 +698,11 @@ int launch_gemm(GemmArgs a, hipStream_t st) {
     }
     // rows of any alignment, us against gemm_any_kernel: 16384 x 2048 x 4097 bf16 455 and 723, 3001 x 2047 x 2049 68 and 90;
     // a 64-tile alone on its CU has its chunks sooner there (300 x 1001 x 1001: 18 and 15)
-    const double tiles64 = (a.order ? (double)a.M / 64 + 0.5 * std::min<long>(a.M, a.E) : (double)((a.M + 63) / 64)) * ((a.N + 63) / 64);
+    const double tiles64 = tile_count(a, 64, 64);
     if (near && (whole || tiles64 > 256)) {
-        const double c256 = slice_cost<T, 256>(a), c128 = slice_cost<T, 128>(a), c64 = slice_cost<T, 64>(a);
-        if (!whole) return c128 <= c64 ? launch_tile<T, 128, 128, 2, 2, 2, false>(a, st) : launch_tile<T, 64, 64, 2, 2, 2, false>(a, st);
+        const double c256 = tile_cost<T>(a, 256, 256, 1.10, 9.7, 7.28, 8.7), c64 = tile_cost<T>(a, 64, 64, 0.19, 0.4, 0.53, 0.3);
+        const double c128 = tile_cost<T>(a, 128, 128, 0.476, 1.4, 1.95, 1.6), c12864 = tile_cost<T>(a, 128, 64, 0.298, 1.0, 0.956, 1.2);
+        if (!whole) return c128 <= c64 ? launch_tile<T, 128, 128, 2, 4, 2, false>(a, st) : launch_tile<T, 64, 64, 2, 2, 2, false>(a, st);
         const int splits = a.partial ? split_count(a.M, a.N, a.K, Elem<T>::BYTES == 4 ? FR_TYPE_F32 : FR_TYPE_BF16) : 1;
         if (splits > 1) {
             const long slices = (rowb + 127) / 128;
@@ -711,9 +714,12 @@ int launch_gemm(GemmArgs a, hipStream_t st) {
             FR_LAUNCH_CHECK("gemm_join_kernel");
             return FR_OK;
         }
-        if (c256 <= c128 && c256 <= c64) return launch_tile<T, 256, 256, 2, 4, 2>(a, st);
-        if (c128 <= c64) return launch_tile<T, 128, 128, 2, 2, 2>(a, st);
-        return launch_tile<T, 64, 64, 2, 2, 3>(a, st);
+        if (c256 <= std::min(c128, std::min(c12864, c64))) return launch_tile<T, 256, 256, 2, 4, 2>(a, st);
+        if (c12864 <= std::min(c128, c64)) return launch_tile<T, 128, 64, 4, 2, 3>(a, st);
+        // a deeper ring for a tile alone on its CU, more tiles at a time for others: 2048 cubed bf16 (128-tiles) 20 us, 26 with
+        // the ring of 2; 200 x 4096 x 4096 (64-tiles) 16 us, 19 with the ring of 3; 32 experts' 64 rows, 4 tiles a CU, 20 and 16
+        if (c64 <= c128) return tiles64 <= 256 ? launch_tile<T, 64, 64, 2, 2, 5>(a, st) : launch_tile<T, 64, 64, 2, 2, 3>(a, st);
+        return tile_count(a, 128, 128) <= 256 ? launch_tile<T, 128, 128, 2, 4, 3>(a, st) : launch_tile<T, 128, 128, 2, 4, 2>(a, st);
     }
     const long mt = a.order ? a.M / 64 + std::min<long>(a.M, a.E + 1) : (a.M + 63) / 64;
     a.n_tiles = (a.N + 63) / 64;

@@ -757,6 +757,29 @@ def test_linear_large_rows_of_any_alignment(kind, m, k, n):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("m, k, n", [(2000, 1032, 1999), (1900, 520, 1700), (2047, 2056, 1030), (4622, 328, 2599), (5865, 136, 2633), (5014, 72, 1409),
+                                     (5821, 168, 131), (300, 648, 1500), (5726, 8, 140), (2048, 1024, 2048)])
+def test_linear_every_tile(kind, m, k, n):
+    """Sizes at which each of the tiles is the estimated best, in one type or the other."""
+    g, dt = gen(m + k), TYPES[kind]
+    x, w, b, res = randn(g, m, k, dtype=dt), randn(g, n, k, dtype=dt, scale=k ** -0.5), randn(g, n), randn(g, m, n, dtype=dt)
+    want = oa.linear(x, w, b, residual=res, name="relu")
+    close(adapter.linear(x, w, b, residual=res, act="relu"), want, linear_tol(x, w, b, res, want, dt), (kind, m, k, n))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("t, e, k, d, n", [(4448, 12, 1, 328, 2406), (2273, 3, 3, 136, 2273), (2311, 12, 2, 72, 1436), (1228, 12, 1, 72, 1977),
+                                           (501, 12, 1, 176, 1159), (900, 70, 2, 1032, 990)])
+def test_expert_linear_every_tile(kind, t, e, k, d, n):
+    g, dt = gen(t + e + d), TYPES[kind]
+    r = choose(g, t, e, k, 0.1)
+    x, w, b = randn(g, t, d, dtype=dt), randn(g, e, n, d, dtype=dt, scale=d ** -0.5), randn(g, e, n, dtype=dt)
+    check_expert(x, w, r, b, rows="tokens", out="slots", what=(kind, t, e, k, d, n))
+
+
+@pytest.mark.gpu
 def test_expert_linear_nothing():
     r = choose(gen(1), 0, 4, 2)
     assert adapter.expert_linear(torch.zeros(0, 8, device="cuda"), torch.zeros(4, 6, 8, device="cuda"), r, out="slots").shape == (0, 2, 6)
