@@ -19,6 +19,7 @@ struct GemmArgs {
     // experts: order == NULL for the plain product
     const int* order; const int* offsets;
     int E, k, rows_sorted, out_slots;
+    unsigned k_mul; int k_shift;         // s / k = (s k_mul) >> (31 + k_shift) for 0 <= s < 2^31
     int n_tiles;
     int splits, split_slices;            // K in `splits` parts of split_slices slices each, their sums in `partial` [splits][M][N]
     float* partial;
@@ -46,37 +47,56 @@ template <> struct Elem<float> {
     }
 };
 
-// The rows [r0, r1) of the order that row tile `tile` covers, and their expert (E: the slots without one).  False: no such
-// tile.  Every wave of a block computes it.  Bounds are clamped to [0, M), so a bad table reads and writes nothing outside.
-FR_DEV bool expert_tile(const GemmArgs& a, int tile, int bm, int& expert, long& r0, long& r1) {
-    const int lane = threadIdx.x & 63, P = (int)a.M;
+// Sums over the lanes up to each lane.
+FR_DEV int scan_add(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);          // 1, 2, 4 and 8 lanes back in a row of 16
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);          // the row before; the two rows before
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+    return v;
+}
+// Expert e0 + lane (E: the slots without one): its rows [lo, hi) of the order and the row tiles from expert e0 to its end.
+// Bounds are clamped to [0, M), so a bad table reads and writes nothing outside.
+struct ExpertScan { int lo, hi, tiles, upto; };
+FR_DEV ExpertScan scan_experts(const GemmArgs& a, int e0, int bm) {
+    const int e = e0 + (threadIdx.x & 63), P = (int)a.M;
+    ExpertScan x{};
+    if (e <= a.E) {
+        x.lo = min(max(a.offsets[e], 0), P);
+        x.hi = e < a.E ? min(max(a.offsets[e + 1], x.lo), P) : P;
+    }
+    x.tiles = (x.hi - x.lo + bm - 1) / bm;
+    x.upto = scan_add(x.tiles);
+    return x;
+}
+// Number of row tiles; `x`: the scan of the first 64.
+FR_DEV int expert_tiles(const GemmArgs& a, int bm, const ExpertScan& x) {
+    int n = __builtin_amdgcn_readlane(x.upto, 63);
+    for (int e0 = 64; e0 <= a.E; e0 += 64) n += __builtin_amdgcn_readlane(scan_experts(a, e0, bm).upto, 63);
+    return n;
+}
+// The rows [r0, r1) of the order that row tile `tile` covers, and their expert.  False: no such tile.  Every wave of a block
+// computes it, from the scan of the first 64 on.
+FR_DEV bool expert_tile(const GemmArgs& a, int tile, int bm, ExpertScan x, int& expert, long& r0, long& r1) {
     int before = 0;
-    for (int e0 = 0; e0 <= a.E; e0 += 64) {
-        const int e = e0 + lane;
-        int lo = 0, hi = 0;
-        if (e <= a.E) {
-            lo = min(max(a.offsets[e], 0), P);
-            hi = e < a.E ? min(max(a.offsets[e + 1], lo), P) : P;
-        }
-        const int nt = (hi - lo + bm - 1) / bm;
-        int s = nt;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) { const int t = __shfl_up(s, o, 64); if (lane >= o) s += t; }
-        const unsigned long long past = __ballot(before + s > tile);
+    for (int e0 = 0;;) {
+        const unsigned long long past = __ballot(before + x.upto > tile);
         if (past) {
             const int f = __ffsll(past) - 1;
-            const int first = before + __shfl(s - nt, f, 64);
-            lo = __shfl(lo, f, 64); hi = __shfl(hi, f, 64);
-            expert = __builtin_amdgcn_readfirstlane(e0 + f);
-            const long begin = __builtin_amdgcn_readfirstlane(lo), end = __builtin_amdgcn_readfirstlane(hi);
-            r0 = begin + (long)__builtin_amdgcn_readfirstlane(tile - first) * bm;
+            const int first = before + __builtin_amdgcn_readlane(x.upto - x.tiles, f);
+            const long begin = __builtin_amdgcn_readlane(x.lo, f), end = __builtin_amdgcn_readlane(x.hi, f);
+            expert = e0 + f;
+            r0 = begin + (long)(tile - first) * bm;
             r1 = min(r0 + bm, end);
-            if (r0 < begin || r0 >= end) return false;       // only where the counts of a table that lies have overflowed
-            return true;
+            return r0 >= begin && r0 < end;                  // false only where the counts of a table that lies have overflowed
         }
-        before += __shfl(s, 63, 64);
+        before += __builtin_amdgcn_readlane(x.upto, 63);
+        e0 += 64;
+        if (e0 > a.E) return false;
+        x = scan_experts(a, e0, bm);
     }
-    return false;
 }
 
 // Slot of position p of the order, -1 if the table names none.
@@ -88,7 +108,7 @@ FR_DEV int slot_at(const GemmArgs& a, long p) {
 FR_DEV long x_row(const GemmArgs& a, long p) {
     if (!a.order || a.rows_sorted) return p;
     const int s = slot_at(a, p);
-    return s < 0 ? 0 : s / a.k;
+    return s < 0 ? 0 : __umulhi(2u * s, a.k_mul) >> a.k_shift;     // s / k
 }
 // Row of the output for position p of the order; -1: none.
 FR_DEV long out_row(const GemmArgs& a, long p) {
@@ -103,10 +123,14 @@ FR_DEV Vec8f get8n(const void* base, long i, int n, int type) {
     for (int j = 0; j < 8; ++j) o.v[j] = j < n ? load1(base, i + j, type) : 0.f;
     return o;
 }
-template <int ACT>
-FR_DEV void act8c(Vec8f& v, const Vec8f& slope) {
+template <int ACT, int Q>
+FR_DEV void act_rows(Vec8f (&v)[Q], const Vec8f& slope) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v.v[j] = adapter_act(v.v[j], ACT, slope.v[j]);
+    for (int e = 0; e < Q; ++e) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[e].v[j] = adapter_act(v[e].v[j], ACT, slope.v[j]);
+        __builtin_amdgcn_sched_barrier(0);                   // rows mixed with each other take registers that there are not
+    }
 }
 FR_DEV void put8n(void* base, long i, int n, int type, const Vec8f& v) {
     if (n == 8) { store8t<false>(base, i, type, v); return; }
@@ -122,16 +146,19 @@ FR_DEV Columns columns(const GemmArgs& a, int n, int have, long nbase, bool none
     if (a.act == FR_ACT_PRELU) c.slope = get8n(a.slope, nbase + n, have, FR_TYPE_F32);
     return c;
 }
-FR_DEV void activate(const GemmArgs& a, Vec8f& v, const Columns& c) {
+template <int Q>
+FR_DEV void activate(const GemmArgs& a, Vec8f (&v)[Q], const Columns& c) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v.v[j] += c.bias.v[j];
+    for (int e = 0; e < Q; ++e)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[e].v[j] += c.bias.v[j];
     switch (a.act) {
-        case FR_ACT_PRELU: act8c<FR_ACT_PRELU>(v, c.slope); break;
-        case FR_ACT_HSWISH: act8c<FR_ACT_HSWISH>(v, c.slope); break;
-        case FR_ACT_RELU: act8c<FR_ACT_RELU>(v, c.slope); break;
-        case FR_ACT_HSIGMOID: act8c<FR_ACT_HSIGMOID>(v, c.slope); break;
-        case FR_ACT_GELU: act8c<FR_ACT_GELU>(v, c.slope); break;
-        case FR_ACT_SILU: act8c<FR_ACT_SILU>(v, c.slope); break;
+        case FR_ACT_PRELU: act_rows<FR_ACT_PRELU>(v, c.slope); break;
+        case FR_ACT_HSWISH: act_rows<FR_ACT_HSWISH>(v, c.slope); break;
+        case FR_ACT_RELU: act_rows<FR_ACT_RELU>(v, c.slope); break;
+        case FR_ACT_HSIGMOID: act_rows<FR_ACT_HSIGMOID>(v, c.slope); break;
+        case FR_ACT_GELU: act_rows<FR_ACT_GELU>(v, c.slope); break;
+        case FR_ACT_SILU: act_rows<FR_ACT_SILU>(v, c.slope); break;
         default: break;
     }
 }
@@ -139,49 +166,32 @@ FR_DEV void activate(const GemmArgs& a, Vec8f& v, const Columns& c) {
 FR_DEV void finish8(const GemmArgs& a, long row, int n, const Columns& c, Vec8f v, bool none) {
     const int have = min(8, a.N - n);
     if (have <= 0) return;
+    Vec8f one[1] = {v};
     if (!none) {
-        activate(a, v, c);
+        activate(a, one, c);
         if (a.res) {
             const Vec8f r = get8n(a.res, row * a.ldr + n, have, a.res_type);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v.v[j] += r.v[j];
+            for (int j = 0; j < 8; ++j) one[0].v[j] += r.v[j];
         }
     }
-    put8n(a.out, row * a.N + n, have, a.out_type, v);
+    put8n(a.out, row * a.N + n, have, a.out_type, one[0]);
 }
-// The same for IT rows RPI apart, from position p0, their sums in LDS `PITCH` bytes a row apart; four rows at a time.
-template <int RPI, int IT, int PITCH>
-FR_DEV void finish_rows(const GemmArgs& a, long p0, long r1, int n, int have, const Columns& c, const unsigned char* at, bool none) {
-    constexpr int Q = IT < 4 ? IT : 4;
-#pragma unroll 1
-    for (int k = 0; k < IT; k += Q) {
-        if (p0 + k * RPI >= r1) break;
-        long row[Q];
-        Raw8 res[Q];
+// Q rows' residuals added, and their eight outputs from column n stored (rows < 0: none).
+template <int TYPE, int Q>
+FR_DEV void add_rows(Vec8f (&v)[Q], const Raw8 (&res)[Q]) {
 #pragma unroll
-        for (int e = 0; e < Q; ++e) {
-            const long p = p0 + (k + e) * RPI;
-            row[e] = p < r1 ? out_row(a, p) : -1;
-            if (a.res && have == 8) res[e] = raw_load8<false>(a.res, max(row[e], 0l) * a.ldr + n, a.res_type);
-        }
+    for (int e = 0; e < Q; ++e) {
+        const Vec8f r = raw_to_f(res[e], TYPE);
 #pragma unroll
-        for (int e = 0; e < Q; ++e) {
-            Vec8f v;
-            const f32x4 lo = *reinterpret_cast<const f32x4*>(at + (k + e) * RPI * PITCH), hi = *reinterpret_cast<const f32x4*>(at + (k + e) * RPI * PITCH + 16);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) { v.v[j] = lo[j]; v.v[4 + j] = hi[j]; }
-            if (row[e] < 0) continue;
-            if (!none) {
-                activate(a, v, c);
-                if (a.res) {
-                    const Vec8f r = have == 8 ? raw_to_f(res[e], a.res_type) : get8n(a.res, row[e] * a.ldr + n, have, a.res_type);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) v.v[j] += r.v[j];
-                }
-            }
-            put8n(a.out, row[e] * a.N + n, have, a.out_type, v);
-        }
+        for (int j = 0; j < 8; ++j) v[e].v[j] += r.v[j];
     }
+}
+template <int TYPE, int Q>
+FR_DEV void put_rows(const GemmArgs& a, const long (&row)[Q], int n, const Vec8f (&v)[Q]) {
+#pragma unroll
+    for (int e = 0; e < Q; ++e)
+        if (row[e] >= 0) store8t<false>(a.out, row[e] * a.N + n, TYPE, v[e]);
 }
 
 // 16 bytes of a row from byte `at` of its `len`, zeros behind its end; any alignment.
@@ -231,20 +241,6 @@ FR_DEV void block_barrier() {                              // without the waits 
 // LDS written by other lanes of this wave is read behind it (a wave's LDS accesses are carried out in order).
 FR_DEV void wave_lds_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); __builtin_amdgcn_wave_barrier(); }
 
-// Number of row tiles of all experts and of the slots without one.
-FR_DEV int expert_tiles(const GemmArgs& a, int bm) {
-    const int lane = threadIdx.x & 63, P = (int)a.M;
-    int n = 0;
-    for (int e = lane; e <= a.E; e += 64) {
-        const int lo = min(max(a.offsets[e], 0), P);
-        const int hi = e < a.E ? min(max(a.offsets[e + 1], lo), P) : P;
-        n += (hi - lo + bm - 1) / bm;
-    }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
-    return __builtin_amdgcn_readfirstlane(n);
-}
-
 // Block -> output tile.  Blocks go to the 8 XCDs in turn and each XCD has its own L2: a contiguous run of tiles for each,
 // walked in groups of 4 row tiles by every n tile, so that the blocks of an XCD that run at the same time share their operands
 // (groups of 8: 4 % slower at 16384 x 2048 x 8192, equal at 8192 cubed; of 16: 15 % slower there).
@@ -270,17 +266,21 @@ template <typename T, int BM, int BN, int WM, int WN, int ST, bool WHOLE>
 __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_tile_kernel(GemmArgs a) {
     constexpr int NW = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16, XB = BM * 128, BUF = (BM + BN) * 128;
     constexpr int XI = BM / 8 / NW, WI = BN / 8 / NW, DMA = XI + WI, DPG = (DMA + TM - 1) / TM;     // DMA instructions a wave and slice, and a group of products
-    static_assert(TN <= TM && NW % 2 == 0 && (WHOLE || ST == 2), "the interleaving below");
+    static_assert(TN <= TM && TN <= 4 && NW % 2 == 0 && (WHOLE || ST == 2), "the interleaving below");
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int li = lane & 15, lg = lane >> 4, wm = wave / WN, wn = wave % WN;
     int mtiles = (int)((a.M + BM - 1) / BM), mt, nt, expert = 0;
-    if (a.order) mtiles = min(expert_tiles(a, BM), (int)(gridDim.x / a.n_tiles));     // the second: tables that lie
+    ExpertScan scan{};
+    if (a.order) {
+        scan = scan_experts(a, 0, BM);
+        mtiles = min(expert_tiles(a, BM, scan), (int)(gridDim.x / a.n_tiles));     // the second: tables that lie
+    }
     const int tiles = mtiles * a.n_tiles, split = a.splits > 1 ? blockIdx.x / tiles : 0;
     if ((int)blockIdx.x - split * tiles >= tiles || split >= a.splits) return;     // experts: the grid is an upper bound
     tile_of_block(blockIdx.x - split * tiles, mtiles, a.n_tiles, mt, nt);
     long r0 = (long)mt * BM, r1 = min(r0 + BM, a.M);
-    if (a.order && !expert_tile(a, mt, BM, expert, r0, r1)) return;
+    if (a.order && !expert_tile(a, mt, BM, scan, expert, r0, r1)) return;
     const bool none = a.order && expert == a.E;
     const int n0 = nt * BN;
     const long nbase = (long)expert * a.N, pitch = (long)a.K * Elem<T>::BYTES, k0 = (long)split * a.split_slices * 128;
@@ -295,12 +295,12 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_tile_kernel(GemmArgs a) 
     const unsigned char* wbase = reinterpret_cast<const unsigned char*>(a.w) + (none ? 0 : (nbase + n0) * pitch) + k0;
     unsigned off[DMA];                                       // x rows, then weight rows
 #pragma unroll
+    for (int j = 0; j < WI; ++j) off[XI + j] = (unsigned)(min(8 * (wave + NW * j) + (lane >> 3), a.N - 1 - n0) * pitch) + kx;
+#pragma unroll
     for (int j = 0; j < XI; ++j) {
         const long p = min(r0 + 8 * (wave + NW * j) + (lane >> 3), r1 - 1);
         off[j] = (unsigned)((gather ? x_row(a, p) : p - r0) * a.ldx * Elem<T>::BYTES) + kx;
     }
-#pragma unroll
-    for (int j = 0; j < WI; ++j) off[XI + j] = (unsigned)(min(8 * (wave + NW * j) + (lane >> 3), a.N - 1 - n0) * pitch) + kx;
     auto place = [&](int into, int d) __attribute__((always_inline)) {          // of instruction d in LDS
         return smem + into + (d < XI ? wave + NW * d : BM / 8 + wave + NW * (d - XI)) * 1024;
     };
@@ -311,19 +311,20 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_tile_kernel(GemmArgs a) 
         if constexpr (WHOLE) __builtin_amdgcn_global_load_lds((glb_ptr_t)src, (lds_ptr_t)place(into, d), 16, 0, 0);
         else held[d] = *reinterpret_cast<const u32x4_any*>(src);
     };
-    auto stage = [&](int s, int into) {                      // a whole slice; K may end inside it: zeros behind its end
+    // instructions [d0, d1) of a slice in which K may end: zeros behind its end
+    auto stage = [&](int s, int into, int d0, int d1) __attribute__((always_inline)) {
         const long at = (long)s * 128;
         if constexpr (WHOLE) {
             const unsigned lo = at + kx >= rowb ? 0u : ~0u;
             const unsigned long long m = ((unsigned long long)lo << 32) | lo, zero = (unsigned long long)&g_zero16 & ~m;
 #pragma unroll
-            for (int d = 0; d < DMA; ++d) {
+            for (int d = d0; d < d1; ++d) {
                 const unsigned long long u = (unsigned long long)((d < XI ? xbase : wbase) + at + off[d]);
                 __builtin_amdgcn_global_load_lds((glb_ptr_t)((u & m) | zero), (lds_ptr_t)place(into, d), 16, 0, 0);
             }
         } else {
 #pragma unroll
-            for (int d = 0; d < DMA; ++d)
+            for (int d = d0; d < d1; ++d)
                 *reinterpret_cast<u32x4*>(place(into, d) + lane * 16) = chunk_at((d < XI ? xbase : wbase) + off[d], at, rowb - kx);
         }
     };
@@ -365,7 +366,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_tile_kernel(GemmArgs a) 
         if (fast || s + ST - 1 < slices) wait_counts<DMA * (ST - 2), 0>();
         else wait_counts<0, 0>();
         block_barrier();
-        if (!fast && s + ST < slices) stage(s + ST, cur);
+        if (!fast && s + ST < slices) stage(s + ST, cur, 0, DMA);
         holds = fast;
         const unsigned char *xs = xbase + (long)(s + ST) * 128, *ws = wbase + (long)(s + ST) * 128;
         asm("" : "+s"(xs), "+s"(ws));                        // scalar bases: the lanes add their 32-bit offsets
@@ -385,9 +386,15 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_tile_kernel(GemmArgs a) 
         }
     };
     if (slices) {
-        for (int s = 0; s < ST && s < slices; ++s) stage(s, s * BUF);
+        // the weights first: the rows of x may still be looked up (rings of 2, whose next wait is for everything; the deeper
+        // ones' waits count in the order of the slices)
+        if constexpr (ST == 2) {
+            for (int s = 0; s < ST && s < slices; ++s) stage(s, s * BUF, XI, DMA);
+            for (int s = 0; s < ST && s < slices; ++s) stage(s, s * BUF, 0, XI);
+        } else
+            for (int s = 0; s < ST && s < slices; ++s) stage(s, s * BUF, 0, DMA);
         if constexpr (!WHOLE) wait_counts<0, 0>();
-        if (slices >= ST) wait_counts<DMA * (ST - 1), 15>();
+        if (slices >= ST) wait_counts<(ST == 2 ? XI : DMA) * (ST - 1), 15>();
         else wait_counts<0, 15>();
         block_barrier();
 #pragma unroll
@@ -397,32 +404,86 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_tile_kernel(GemmArgs a) 
         for (; s < slices; ++s) slice(s, false);
     }
 
-    // epilogue: up to 64 x 64 of the wave's outputs at a time through its part of LDS (rows 16 bytes more than a multiple of
-    // 128: writes of 16 rows fall on different banks), then 8 outputs a lane, whole lines.  A lane keeps its columns, so bias
-    // and slopes are loaded once; residuals of four rows are asked for together.
-    constexpr int EM = TM < 4 ? TM : 4, EN = TN < 4 ? TN : 4, PITCH = EN * 64 + 16, LPR = EN * 2, RPI = 64 / LPR, IT = EM * 16 / RPI;
+    // epilogue: up to 64 rows of the wave's outputs at a time through its part of LDS (rows 16 bytes more than a multiple of 128:
+    // writes of 16 rows fall on different banks), then 8 outputs a lane, whole lines.  A lane keeps its columns, so bias and
+    // slopes are loaded once.  Groups of Q rows in one rolled loop: each choice (type, activation) is made once a group, and a
+    // group's residuals are asked for before the group before it is stored, so that the wait for them is not one for the stores.
+    // Unrolled rows with the choices inside were 100 KB of instructions, 9 us a 256-tile and 21 with residuals.
+    constexpr int EM = TM < 4 ? TM : 4, PITCH = TN * 64 + 16, LPR = TN * 2, RPI = 64 / LPR, IT = EM * 16 / RPI, Q = IT < 2 ? IT : 2;
+    constexpr int PER = IT / Q, GROUPS = TM / EM * PER;
     unsigned char* part = smem + wave * EM * 16 * PITCH;
     GemmArgs o = a;
     if (a.splits > 1) {                                      // a part's plain sums; gemm_join_kernel does the rest
         o.bias = o.res = nullptr; o.act = FR_ACT_NONE; o.out_type = FR_TYPE_F32;
         o.out = a.partial + (long)split * a.M * a.N;
     }
+    const int n = n0 + wn * TN * 16 + (lane % LPR) * 8, have = min(8, a.N - n);
+    const long p0 = r0 + wm * TM * 16 + lane / LPR;
+    const unsigned char* at = part + (lane / LPR) * PITCH + (lane % LPR) * 32;
+    const bool add = o.res && have == 8;
+    Raw8 ahead[Q];
+    long row[Q];
+    auto rows_of = [&](int g) __attribute__((always_inline)) {
+#pragma unroll
+        for (int e = 0; e < Q; ++e) {
+            const long p = p0 + (g * Q + e) * RPI;
+            row[e] = p < r1 ? out_row(o, p) : -1;
+        }
+        if (!add) return;
+        if (o.res_type == FR_TYPE_F32) {
+#pragma unroll
+            for (int e = 0; e < Q; ++e) ahead[e] = raw_load8<false>(o.res, max(row[e], 0l) * o.ldr + n, FR_TYPE_F32);
+        } else {
+#pragma unroll
+            for (int e = 0; e < Q; ++e) ahead[e] = raw_load8<false>(o.res, max(row[e], 0l) * o.ldr + n, FR_TYPE_BF16);
+        }
+    };
+    const Columns col = columns(o, n, have, nbase, none);
+    rows_of(0);
     __syncthreads();                                         // the ring is read
 #pragma unroll
-    for (int q = 0; q < TN / EN; ++q) {
-        const int n = n0 + (wn * TN + EN * q) * 16 + (lane % LPR) * 8, have = min(8, a.N - n);
-        const Columns col = columns(o, n, have, nbase, none);
+    for (int u = 0; u < TM / EM; ++u) {
+        wave_lds_fence();                                    // the rows before have been read
 #pragma unroll
-        for (int u = 0; u < TM / EM; ++u) {
+        for (int j = 0; j < EM; ++j)
 #pragma unroll
-            for (int j = 0; j < EM; ++j)
+            for (int i = 0; i < TN; ++i) *reinterpret_cast<f32x4*>(part + (16 * j + li) * PITCH + i * 64 + lg * 16) = acc[i][EM * u + j];
+        wave_lds_fence();
+#pragma unroll 1
+        for (int g = u * PER; g < (u + 1) * PER; ++g) {
+            const unsigned char* from = at + (g - u * PER) * Q * RPI * PITCH;
+            long to[Q];
+            if (have == 8) {
+                Vec8f v[Q];
 #pragma unroll
-                for (int i = 0; i < EN; ++i) *reinterpret_cast<f32x4*>(part + (16 * j + li) * PITCH + i * 64 + lg * 16) = acc[EN * q + i][EM * u + j];
-            wave_lds_fence();
-            const long p0 = r0 + (wm * TM + EM * u) * 16 + lane / LPR;
-            const unsigned char* at = part + (lane / LPR) * PITCH + (lane % LPR) * 32;
-            if (have > 0) finish_rows<RPI, IT, PITCH>(o, p0, r1, n, have, col, at, none);
-            wave_lds_fence();
+                for (int e = 0; e < Q; ++e) {
+                    const f32x4 lo = *reinterpret_cast<const f32x4*>(from + e * RPI * PITCH), hi = *reinterpret_cast<const f32x4*>(from + e * RPI * PITCH + 16);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) { v[e].v[j] = lo[j]; v[e].v[4 + j] = hi[j]; }
+                }
+                if (!none) activate(o, v, col);
+                if (add) {
+                    if (o.res_type == FR_TYPE_F32) add_rows<FR_TYPE_F32>(v, ahead);
+                    else if (o.res_type == FR_TYPE_BF16) add_rows<FR_TYPE_BF16>(v, ahead);
+                    else add_rows<FR_TYPE_F16>(v, ahead);
+                }
+#pragma unroll
+                for (int e = 0; e < Q; ++e) to[e] = row[e];
+                if (g + 1 < GROUPS) rows_of(g + 1);
+                if (o.out_type == FR_TYPE_F32) put_rows<FR_TYPE_F32>(o, to, n, v);
+                else if (o.out_type == FR_TYPE_BF16) put_rows<FR_TYPE_BF16>(o, to, n, v);
+                else put_rows<FR_TYPE_F16>(o, to, n, v);
+            } else if (have > 0) {                               // the last columns, where N ends inside the lane's eight
+#pragma unroll 1
+                for (int e = 0; e < Q; ++e) {
+                    const long p = p0 + (g * Q + e) * RPI, r = p < r1 ? out_row(o, p) : -1;
+                    const f32x4 lo = *reinterpret_cast<const f32x4*>(from + e * RPI * PITCH), hi = *reinterpret_cast<const f32x4*>(from + e * RPI * PITCH + 16);
+                    Vec8f v;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) { v.v[j] = lo[j]; v.v[4 + j] = hi[j]; }
+                    if (r >= 0) finish8(o, r, n, col, v, none);
+                }
+            }
         }
     }
 }
@@ -561,7 +622,7 @@ __global__ __launch_bounds__(256) void gemm_any_kernel(GemmArgs a) {
     if (!a.order && (long)mt * 64 >= a.M) return;
     long r0 = (long)mt * 64, r1 = min(r0 + 64, a.M);
     int expert = 0;
-    if (a.order && !expert_tile(a, mt, 64, expert, r0, r1)) return;
+    if (a.order && !expert_tile(a, mt, 64, scan_experts(a, 0, 64), expert, r0, r1)) return;
     const bool none = a.order && expert == a.E;
     const long nbase = (long)expert * a.N;
     const long rowb = (long)a.K * Elem<T>::BYTES;
@@ -780,5 +841,8 @@ extern "C" int fr_expert_linear(const void* x, int rows_sorted, const void* w, c
     a.M = T * k; a.ldx = K; a.N = N; a.K = K;
     a.bias_type = bias_type; a.out_type = out_type; a.act = act;
     a.order = order; a.offsets = offsets; a.E = E; a.k = k; a.rows_sorted = rows_sorted; a.out_slots = out_slots;
+    // k_mul = (2^(31 + k_shift) + e) / k with e < k <= 2^k_shift: s e / (k 2^(31 + k_shift)) < 1 / k takes no quotient to the next
+    while ((1l << a.k_shift) < k) ++a.k_shift;
+    a.k_mul = (unsigned)(((1ull << (31 + a.k_shift)) + k - 1) / k);
     return launch_type(type, a, (hipStream_t)stream);
 }

@@ -780,6 +780,16 @@ def test_expert_linear_every_tile(kind, t, e, k, d, n):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("e", [62, 63, 64, 65, 127, 128, 200])
+@pytest.mark.parametrize("t, k", [(2, 1), (90, 7), (1500, 3)])
+def test_expert_linear_many_experts(e, t, k):
+    g = gen(t + e)
+    r = choose(g, t, e, k, 0.2)
+    x, w, b = randn(g, t, 64, dtype=torch.bfloat16), randn(g, e, 40, 64, dtype=torch.bfloat16, scale=0.125), randn(g, e, 40)
+    check_expert(x, w, r, b, act="silu", rows="tokens", out="slots", what=(e, t, k))
+
+
+@pytest.mark.gpu
 def test_expert_linear_nothing():
     r = choose(gen(1), 0, 4, 2)
     assert adapter.expert_linear(torch.zeros(0, 8, device="cuda"), torch.zeros(4, 6, 8, device="cuda"), r, out="slots").shape == (0, 2, 6)
