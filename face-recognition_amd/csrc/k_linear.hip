@@ -123,14 +123,10 @@ FR_DEV Vec8f get8n(const void* base, long i, int n, int type) {
     for (int j = 0; j < 8; ++j) o.v[j] = j < n ? load1(base, i + j, type) : 0.f;
     return o;
 }
-template <int ACT, int Q>
-FR_DEV void act_rows(Vec8f (&v)[Q], const Vec8f& slope) {
+template <int ACT>
+FR_DEV void act8(Vec8f& v, const Vec8f& slope) {
 #pragma unroll
-    for (int e = 0; e < Q; ++e) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[e].v[j] = adapter_act(v[e].v[j], ACT, slope.v[j]);
-        __builtin_amdgcn_sched_barrier(0);                   // rows mixed with each other take registers that there are not
-    }
+    for (int j = 0; j < 8; ++j) v.v[j] = adapter_act(v.v[j], ACT, slope.v[j]);
 }
 FR_DEV void put8n(void* base, long i, int n, int type, const Vec8f& v) {
     if (n == 8) { store8t<false>(base, i, type, v); return; }
@@ -146,52 +142,33 @@ FR_DEV Columns columns(const GemmArgs& a, int n, int have, long nbase, bool none
     if (a.act == FR_ACT_PRELU) c.slope = get8n(a.slope, nbase + n, have, FR_TYPE_F32);
     return c;
 }
-template <int Q>
-FR_DEV void activate(const GemmArgs& a, Vec8f (&v)[Q], const Columns& c) {
+FR_DEV void activate(const GemmArgs& a, Vec8f& v, const Columns& c) {
 #pragma unroll
-    for (int e = 0; e < Q; ++e)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[e].v[j] += c.bias.v[j];
+    for (int j = 0; j < 8; ++j) v.v[j] += c.bias.v[j];
     switch (a.act) {
-        case FR_ACT_PRELU: act_rows<FR_ACT_PRELU>(v, c.slope); break;
-        case FR_ACT_HSWISH: act_rows<FR_ACT_HSWISH>(v, c.slope); break;
-        case FR_ACT_RELU: act_rows<FR_ACT_RELU>(v, c.slope); break;
-        case FR_ACT_HSIGMOID: act_rows<FR_ACT_HSIGMOID>(v, c.slope); break;
-        case FR_ACT_GELU: act_rows<FR_ACT_GELU>(v, c.slope); break;
-        case FR_ACT_SILU: act_rows<FR_ACT_SILU>(v, c.slope); break;
+        case FR_ACT_PRELU: act8<FR_ACT_PRELU>(v, c.slope); break;
+        case FR_ACT_HSWISH: act8<FR_ACT_HSWISH>(v, c.slope); break;
+        case FR_ACT_RELU: act8<FR_ACT_RELU>(v, c.slope); break;
+        case FR_ACT_HSIGMOID: act8<FR_ACT_HSIGMOID>(v, c.slope); break;
+        case FR_ACT_GELU: act8<FR_ACT_GELU>(v, c.slope); break;
+        case FR_ACT_SILU: act8<FR_ACT_SILU>(v, c.slope); break;
         default: break;
     }
+}
+FR_DEV void add8n(const GemmArgs& a, Vec8f& v, long row, int n, int have) {       // the residual
+    const Vec8f r = get8n(a.res, row * a.ldr + n, have, a.res_type);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v.v[j] += r.v[j];
 }
 // Eight outputs n .. n+7 (as many as N has) of row `row`; `none`: of a slot without an expert, zeros.
 FR_DEV void finish8(const GemmArgs& a, long row, int n, const Columns& c, Vec8f v, bool none) {
     const int have = min(8, a.N - n);
     if (have <= 0) return;
-    Vec8f one[1] = {v};
     if (!none) {
-        activate(a, one, c);
-        if (a.res) {
-            const Vec8f r = get8n(a.res, row * a.ldr + n, have, a.res_type);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) one[0].v[j] += r.v[j];
-        }
+        activate(a, v, c);
+        if (a.res) add8n(a, v, row, n, have);
     }
-    put8n(a.out, row * a.N + n, have, a.out_type, one[0]);
-}
-// Q rows' residuals added, and their eight outputs from column n stored (rows < 0: none).
-template <int TYPE, int Q>
-FR_DEV void add_rows(Vec8f (&v)[Q], const Raw8 (&res)[Q]) {
-#pragma unroll
-    for (int e = 0; e < Q; ++e) {
-        const Vec8f r = raw_to_f(res[e], TYPE);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[e].v[j] += r.v[j];
-    }
-}
-template <int TYPE, int Q>
-FR_DEV void put_rows(const GemmArgs& a, const long (&row)[Q], int n, const Vec8f (&v)[Q]) {
-#pragma unroll
-    for (int e = 0; e < Q; ++e)
-        if (row[e] >= 0) store8t<false>(a.out, row[e] * a.N + n, TYPE, v[e]);
+    put8n(a.out, row * a.N + n, have, a.out_type, v);
 }
 
 // 16 bytes of a row from byte `at` of its `len`, zeros behind its end; any alignment.
@@ -220,6 +197,8 @@ FR_DEV void column(f32x4 (&acc)[TN][TM], int j, const u32x4 (&w)[TN], const u32x
         for (int i = 0; i < TN; ++i) Elem<T>::mma(acc[i][j], w[i], x);
     }
 }
+
+template <int VALUE> using Is = std::integral_constant<int, VALUE>;
 
 // ---- the staged kernel --------------------------------------------------------------------------------------------------
 typedef __attribute__((address_space(3))) void* lds_ptr_t;
@@ -254,8 +233,9 @@ FR_DEV void tile_of_block(int block, int mtiles, int ntiles, int& mt, int& nt) {
 
 // BM x BN outputs a block of WM x WN waves; slices of 128 bytes of K through a ring of ST buffers in LDS, brought by LDS-DMA
 // (16 bytes a lane, 8 rows an instruction: whole lines of 128 bytes; with rows of 64 bytes the DMA alone was slower, 24
-// against 43 bytes a clock and CU).  Rows are 16-byte aligned whole chunks.  LDS row r keeps its piece p at
-// p ^ ((r >> 1) & 7), so that the 16 rows of a fragment read fall on 16 different bank groups.
+// against 43 bytes a clock and CU).  Rows are 16-byte aligned whole chunks.  A row in LDS keeps its piece p
+// at p ^ key, x row r with the key (r >> 1) & 7, weight row r with that of its bits 1, 3 and 4, so that the 16 rows of a
+// fragment read fall on 16 different bank groups.
 // A slice is two halves of 64 bytes, their fragments in two register sets: while one set is multiplied the other is read.
 // The one barrier of a slice stands between its halves: there its last fragments have been read and the next slice has
 // landed, and behind it the DMA of slice s + ST goes into its buffer, spread over the second half's products (in one
@@ -263,10 +243,10 @@ FR_DEV void tile_of_block(int block, int mtiles, int ntiles, int& mt, int& nt) {
 // WHOLE false: rows of any alignment.  The chunks of slice s + ST go to registers in the second half of slice s and to LDS in
 // the first half of the next, where ST = 2 wants them by its barrier.
 template <typename T, int BM, int BN, int WM, int WN, int ST, bool WHOLE>
-__global__ __launch_bounds__(64 * WM * WN, 2) void gemm_tile_kernel(GemmArgs a) {
+__global__ __launch_bounds__(64 * WM * WN, BM == 128 && BN == 128 && ST == 2 ? 4 : 2) void gemm_tile_kernel(GemmArgs a) {
     constexpr int NW = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16, XB = BM * 128, BUF = (BM + BN) * 128;
     constexpr int XI = BM / 8 / NW, WI = BN / 8 / NW, DMA = XI + WI, DPG = (DMA + TM - 1) / TM;     // DMA instructions a wave and slice, and a group of products
-    static_assert(TN <= TM && TN <= 4 && NW % 2 == 0 && (WHOLE || ST == 2), "the interleaving below");
+    static_assert(TN <= TM && TN % 2 == 0 && NW % 4 == 0 && (WHOLE || ST == 2), "the interleaving below");
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int li = lane & 15, lg = lane >> 4, wm = wave / WN, wn = wave % WN;
@@ -289,13 +269,14 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_tile_kernel(GemmArgs a) 
 
     // this lane's sources: row 8 (wave + NW j) + lane / 8, chunk (lane % 8) ^ key of the slice, as 32-bit offsets from the
     // tile's first row (the matrix's where rows are gathered)
-    const int kx = ((lane & 7) ^ (((8 * wave + (lane >> 3)) >> 1) & 7)) * 16;    // the same for every j: NW is even
+    const int kx = ((lane & 7) ^ (((8 * wave + (lane >> 3)) >> 1) & 7)) * 16;    // the same for every j: NW is a multiple of 4
+    const int kw = ((lane & 7) ^ (((lane >> 4) & 1) | ((wave & 3) << 1))) * 16;
     const bool gather = a.order && !a.rows_sorted;
     const unsigned char* xbase = reinterpret_cast<const unsigned char*>(a.x) + (gather ? 0 : r0 * a.ldx * Elem<T>::BYTES) + k0;
     const unsigned char* wbase = reinterpret_cast<const unsigned char*>(a.w) + (none ? 0 : (nbase + n0) * pitch) + k0;
     unsigned off[DMA];                                       // x rows, then weight rows
 #pragma unroll
-    for (int j = 0; j < WI; ++j) off[XI + j] = (unsigned)(min(8 * (wave + NW * j) + (lane >> 3), a.N - 1 - n0) * pitch) + kx;
+    for (int j = 0; j < WI; ++j) off[XI + j] = (unsigned)(min(8 * (wave + NW * j) + (lane >> 3), a.N - 1 - n0) * pitch) + kw;
 #pragma unroll
     for (int j = 0; j < XI; ++j) {
         const long p = min(r0 + 8 * (wave + NW * j) + (lane >> 3), r1 - 1);
@@ -315,23 +296,24 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_tile_kernel(GemmArgs a) 
     auto stage = [&](int s, int into, int d0, int d1) __attribute__((always_inline)) {
         const long at = (long)s * 128;
         if constexpr (WHOLE) {
-            const unsigned lo = at + kx >= rowb ? 0u : ~0u;
-            const unsigned long long m = ((unsigned long long)lo << 32) | lo, zero = (unsigned long long)&g_zero16 & ~m;
 #pragma unroll
             for (int d = d0; d < d1; ++d) {
+                const unsigned lo = at + (d < XI ? kx : kw) >= rowb ? 0u : ~0u;
+                const unsigned long long m = ((unsigned long long)lo << 32) | lo, zero = (unsigned long long)&g_zero16 & ~m;
                 const unsigned long long u = (unsigned long long)((d < XI ? xbase : wbase) + at + off[d]);
                 __builtin_amdgcn_global_load_lds((glb_ptr_t)((u & m) | zero), (lds_ptr_t)place(into, d), 16, 0, 0);
             }
         } else {
 #pragma unroll
             for (int d = d0; d < d1; ++d)
-                *reinterpret_cast<u32x4*>(place(into, d) + lane * 16) = chunk_at((d < XI ? xbase : wbase) + off[d], at, rowb - kx);
+                *reinterpret_cast<u32x4*>(place(into, d) + lane * 16) = chunk_at((d < XI ? xbase : wbase) + off[d], at, rowb - (d < XI ? kx : kw));
         }
     };
 
-    // fragments: rows 16 t + li of the wave's part, piece (4 h + lg) ^ key; the key is that of li
-    const int fo = ((lg ^ ((li >> 1) & 7)) << 4) + li * 128;
-    const int xo = wm * TM * 2048 + fo, wo = XB + wn * TN * 2048 + fo;
+    // fragments, piece (4 h + lg) ^ key: rows 16 t + li of the wave's part of x; of the weights rows 32 (t / 2) + 8 (li / 4) +
+    // 4 (t % 2) + li % 4, so that a lane's accumulators of two tiles are 8 consecutive outputs
+    const int xo = wm * TM * 2048 + li * 128 + ((lg ^ ((li >> 1) & 7)) << 4);
+    const int wo = XB + wn * TN * 2048 + (8 * (li >> 2) + (li & 3)) * 128 + ((lg ^ (((li >> 1) & 1) | ((li >> 2) << 1))) << 4);
     f32x4 acc[TN][TM];
 #pragma unroll
     for (int i = 0; i < TN; ++i)
@@ -339,7 +321,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_tile_kernel(GemmArgs a) 
         for (int j = 0; j < TM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     u32x4 wf[2][TN], xf[2][TM];
     auto fetch = [&](int from, int h, int q) __attribute__((always_inline)) {    // fragment q of half h: weights, then x
-        if (q < TN) wf[h][q] = *reinterpret_cast<const u32x4*>(smem + from + (wo ^ (h << 6)) + q * 2048);
+        if (q < TN) wf[h][q] = *reinterpret_cast<const u32x4*>(smem + from + (wo ^ (h << 6)) + (q >> 1) * 4096 + (q & 1) * 512);
         else if (q < TN + TM) xf[h][q - TN] = *reinterpret_cast<const u32x4*>(smem + from + (xo ^ (h << 6)) + (q - TN) * 2048);
     };
     constexpr int FPG = TM == 8 ? 2 : TM == 4 ? 3 : 4;       // fragment reads a group of products: done before the last groups
@@ -404,87 +386,114 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_tile_kernel(GemmArgs a) 
         for (; s < slices; ++s) slice(s, false);
     }
 
-    // epilogue: up to 64 rows of the wave's outputs at a time through its part of LDS (rows 16 bytes more than a multiple of 128:
-    // writes of 16 rows fall on different banks), then 8 outputs a lane, whole lines.  A lane keeps its columns, so bias and
-    // slopes are loaded once.  Groups of Q rows in one rolled loop: each choice (type, activation) is made once a group, and a
-    // group's residuals are asked for before the group before it is stored, so that the wait for them is not one for the stores.
-    // Unrolled rows with the choices inside were 100 KB of instructions, 9 us a 256-tile and 21 with residuals.
-    constexpr int EM = TM < 4 ? TM : 4, PITCH = TN * 64 + 16, LPR = TN * 2, RPI = 64 / LPR, IT = EM * 16 / RPI, Q = IT < 2 ? IT : 2;
-    constexpr int PER = IT / Q, GROUPS = TM / EM * PER;
-    unsigned char* part = smem + wave * EM * 16 * PITCH;
+    // epilogue, from the registers: vector q of x row 16 j + li is outputs n + 32 q .. + 7, a store 16 rows of 64 bytes (fp32: two
+    // of 64).  Each choice of type or activation is made once for all vectors it concerns; a part's residuals are asked for
+    // before the part before it is stored, so that the wait for them is not one for the stores.
+    // Through LDS instead, whole lines a store, the epilogue of a 256-tile took 12 400 clocks (without residual or activation).
+    constexpr int V = TN / 2, R = 2;                         // a part: R rows
     GemmArgs o = a;
     if (a.splits > 1) {                                      // a part's plain sums; gemm_join_kernel does the rest
         o.bias = o.res = nullptr; o.act = FR_ACT_NONE; o.out_type = FR_TYPE_F32;
         o.out = a.partial + (long)split * a.M * a.N;
     }
-    const int n = n0 + wn * TN * 16 + (lane % LPR) * 8, have = min(8, a.N - n);
-    const long p0 = r0 + wm * TM * 16 + lane / LPR;
-    const unsigned char* at = part + (lane / LPR) * PITCH + (lane % LPR) * 32;
-    const bool add = o.res && have == 8;
-    Raw8 ahead[Q];
-    long row[Q];
-    auto rows_of = [&](int g) __attribute__((always_inline)) {
+    const int n = n0 + wn * TN * 16 + lg * 8;
+    const long p0 = r0 + wm * TM * 16 + li;
+    long row[R];
+    Raw8 ahead[R][V];
+    auto rows_of = [&](int j0) __attribute__((always_inline)) {
 #pragma unroll
-        for (int e = 0; e < Q; ++e) {
-            const long p = p0 + (g * Q + e) * RPI;
-            row[e] = p < r1 ? out_row(o, p) : -1;
-        }
-        if (!add) return;
-        if (o.res_type == FR_TYPE_F32) {
+        for (int e = 0; e < R; ++e) row[e] = p0 + (j0 + e) * 16 < r1 ? out_row(o, p0 + (j0 + e) * 16) : -1;
+        auto ask = [&](auto type) __attribute__((always_inline)) {
 #pragma unroll
-            for (int e = 0; e < Q; ++e) ahead[e] = raw_load8<false>(o.res, max(row[e], 0l) * o.ldr + n, FR_TYPE_F32);
-        } else {
+            for (int e = 0; e < R; ++e)
 #pragma unroll
-            for (int e = 0; e < Q; ++e) ahead[e] = raw_load8<false>(o.res, max(row[e], 0l) * o.ldr + n, FR_TYPE_BF16);
-        }
+                for (int q = 0; q < V; ++q)
+                    if (row[e] >= 0 && n + 32 * q + 8 <= o.N) ahead[e][q] = raw_load8<false>(o.res, row[e] * o.ldr + n + 32 * q, type());
+        };
+        if (!o.res) return;
+        if (o.res_type == FR_TYPE_F32) ask(Is<FR_TYPE_F32>());
+        else ask(Is<FR_TYPE_BF16>());
     };
-    const Columns col = columns(o, n, have, nbase, none);
+    Columns col[V];
+#pragma unroll
+    for (int q = 0; q < V; ++q) col[q] = columns(o, n + 32 * q, min(8, a.N - n - 32 * q), nbase, none);
     rows_of(0);
-    __syncthreads();                                         // the ring is read
+    const bool ragged = n0 + BN > a.N && a.N % 8;            // some lane's vector has N's end inside
+    if (ragged) __syncthreads();                             // the ring is read
 #pragma unroll
-    for (int u = 0; u < TM / EM; ++u) {
-        wave_lds_fence();                                    // the rows before have been read
+    for (int j0 = 0; j0 < TM; j0 += R) {
+        Vec8f v[R][V];
+        long to[R];
+        auto each = [&](auto f) __attribute__((always_inline)) {
 #pragma unroll
-        for (int j = 0; j < EM; ++j)
+            for (int e = 0; e < R; ++e)
 #pragma unroll
-            for (int i = 0; i < TN; ++i) *reinterpret_cast<f32x4*>(part + (16 * j + li) * PITCH + i * 64 + lg * 16) = acc[i][EM * u + j];
-        wave_lds_fence();
-#pragma unroll 1
-        for (int g = u * PER; g < (u + 1) * PER; ++g) {
-            const unsigned char* from = at + (g - u * PER) * Q * RPI * PITCH;
-            long to[Q];
-            if (have == 8) {
-                Vec8f v[Q];
+                for (int q = 0; q < V; ++q) f(e, q);
+        };
+        each([&](int e, int q) __attribute__((always_inline)) {
 #pragma unroll
-                for (int e = 0; e < Q; ++e) {
-                    const f32x4 lo = *reinterpret_cast<const f32x4*>(from + e * RPI * PITCH), hi = *reinterpret_cast<const f32x4*>(from + e * RPI * PITCH + 16);
+            for (int r = 0; r < 4; ++r) { v[e][q].v[r] = acc[2 * q][j0 + e][r]; v[e][q].v[4 + r] = acc[2 * q + 1][j0 + e][r]; }
+        });
+        if (!none) {
+            each([&](int e, int q) __attribute__((always_inline)) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) { v[e].v[j] = lo[j]; v[e].v[4 + j] = hi[j]; }
-                }
-                if (!none) activate(o, v, col);
-                if (add) {
-                    if (o.res_type == FR_TYPE_F32) add_rows<FR_TYPE_F32>(v, ahead);
-                    else if (o.res_type == FR_TYPE_BF16) add_rows<FR_TYPE_BF16>(v, ahead);
-                    else add_rows<FR_TYPE_F16>(v, ahead);
-                }
-#pragma unroll
-                for (int e = 0; e < Q; ++e) to[e] = row[e];
-                if (g + 1 < GROUPS) rows_of(g + 1);
-                if (o.out_type == FR_TYPE_F32) put_rows<FR_TYPE_F32>(o, to, n, v);
-                else if (o.out_type == FR_TYPE_BF16) put_rows<FR_TYPE_BF16>(o, to, n, v);
-                else put_rows<FR_TYPE_F16>(o, to, n, v);
-            } else if (have > 0) {                               // the last columns, where N ends inside the lane's eight
-#pragma unroll 1
-                for (int e = 0; e < Q; ++e) {
-                    const long p = p0 + (g * Q + e) * RPI, r = p < r1 ? out_row(o, p) : -1;
-                    const f32x4 lo = *reinterpret_cast<const f32x4*>(from + e * RPI * PITCH), hi = *reinterpret_cast<const f32x4*>(from + e * RPI * PITCH + 16);
-                    Vec8f v;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) { v.v[j] = lo[j]; v.v[4 + j] = hi[j]; }
-                    if (r >= 0) finish8(o, r, n, col, v, none);
-                }
+                for (int i = 0; i < 8; ++i) v[e][q].v[i] += col[q].bias.v[i];
+            });
+            auto all = [&](auto act) __attribute__((always_inline)) {
+                each([&](int e, int q) __attribute__((always_inline)) {
+                    act8<act()>(v[e][q], col[q].slope);
+                    __builtin_amdgcn_sched_barrier(0);       // vectors mixed with each other take registers that there are not
+                });
+            };
+            switch (o.act) {
+                case FR_ACT_PRELU: all(Is<FR_ACT_PRELU>()); break;
+                case FR_ACT_HSWISH: all(Is<FR_ACT_HSWISH>()); break;
+                case FR_ACT_RELU: all(Is<FR_ACT_RELU>()); break;
+                case FR_ACT_HSIGMOID: all(Is<FR_ACT_HSIGMOID>()); break;
+                case FR_ACT_GELU: all(Is<FR_ACT_GELU>()); break;
+                case FR_ACT_SILU: all(Is<FR_ACT_SILU>()); break;
+                default: break;
             }
         }
+        if (ragged)
+            each([&](int e, int q) __attribute__((always_inline)) {
+                if (n + 32 * q < a.N && n + 32 * q + 8 > a.N) *reinterpret_cast<Vec8f*>(smem + ((wave * TM + j0 + e) * 64 + lane) * 32) = v[e][q];
+            });
+        auto add = [&](auto type) __attribute__((always_inline)) {
+            each([&](int e, int q) __attribute__((always_inline)) {
+                const Vec8f r = raw_to_f(ahead[e][q], type());
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[e][q].v[i] += r.v[i];
+            });
+        };
+        if (o.res) {
+            if (o.res_type == FR_TYPE_F32) add(Is<FR_TYPE_F32>());
+            else if (o.res_type == FR_TYPE_BF16) add(Is<FR_TYPE_BF16>());
+            else add(Is<FR_TYPE_F16>());
+        }
+#pragma unroll
+        for (int e = 0; e < R; ++e) to[e] = row[e];
+        if (j0 + R < TM) rows_of(j0 + R);
+        auto put = [&](auto type) __attribute__((always_inline)) {
+            each([&](int e, int q) __attribute__((always_inline)) {
+                if (to[e] >= 0 && n + 32 * q + 8 <= o.N) store8t<false>(o.out, to[e] * o.N + n + 32 * q, type(), v[e][q]);
+            });
+        };
+        if (o.out_type == FR_TYPE_F32) put(Is<FR_TYPE_F32>());
+        else if (o.out_type == FR_TYPE_BF16) put(Is<FR_TYPE_BF16>());
+        else put(Is<FR_TYPE_F16>());
+    }
+    if (ragged) {                                            // those vectors, one element at a time
+        const int q = a.N > n ? (a.N - n) / 32 : V, at = n + 32 * q, have = a.N - at;
+        if (q < V && have > 0 && have < 8)
+#pragma unroll 1
+            for (int j = 0; j < TM; ++j) {
+                const long p = p0 + j * 16, r = p < r1 ? out_row(o, p) : -1;
+                Vec8f v = *reinterpret_cast<const Vec8f*>(smem + ((wave * TM + j) * 64 + lane) * 32);
+                if (r < 0) continue;
+                if (o.res) add8n(o, v, r, at, have);
+                put8n(o.out, r * o.N + at, have, o.out_type, v);
+            }
     }
 }
 
@@ -696,7 +705,8 @@ int launch_tile(GemmArgs a, hipStream_t st) {
     const long mt = a.order ? a.M / BM + std::min<long>(a.M, a.E + 1) : (a.M + BM - 1) / BM;
     a.n_tiles = (a.N + BN - 1) / BN;
     if (mt * a.n_tiles * a.splits >= (1l << 32) / (64 * WM * WN)) FR_FAIL(FR_ERR_UNSUPPORTED, "adapter product: more output tiles than a launch takes");
-    const int lds = std::max(ST * (BM + BN) * 128, WM * WN * std::min(64, BM / WM) * (std::min(64, BN / WN) * 4 + 16));    // the ring; the epilogue's rows
+    const int lds = ST * (BM + BN) * 128;
+    static_assert(WN * BM <= ST * (BM + BN), "the ring has room for the vectors that N ends in: 32 bytes a lane and row tile");
     FR_BIG_LDS_ONCE((gemm_tile_kernel<T, BM, BN, WM, WN, ST, WHOLE>), lds);
     hipLaunchKernelGGL((gemm_tile_kernel<T, BM, BN, WM, WN, ST, WHOLE>), dim3((unsigned)(mt * a.n_tiles * a.splits)), dim3(64 * WM * WN), lds, st, a);
     FR_LAUNCH_CHECK("gemm_tile_kernel");
