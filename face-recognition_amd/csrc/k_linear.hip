@@ -721,7 +721,8 @@ double tile_count(const GemmArgs& a, int bm, int bn) {
 }
 // Estimated time in us with tiles of bm x bn: `each` for a slice of 128 bytes of K and `fixed` for the rest of a tile, for every
 // tile of the fullest CU.  The constants are least squares over 90 shapes of 64 to 18 000 rows on one card (rms 3 % in fp32,
-// 10 to 15 % in 16 bits); what the rule picks took 1.4 % more than the best of all tiles there (fp32: 1.8 %).
+// 13 to 15 % in 16 bits); what the rule picks took 1.5 % more than the best of all tiles there (fp32: 1.8 %), and in 16 bits
+// 0.79 of the time of the library's plain product (fp32: 1.03).
 template <typename T>
 double tile_cost(const GemmArgs& a, int bm, int bn, double each16, double fixed16, double each32, double fixed32) {
     constexpr bool f32 = std::is_same<T, float>::value;
@@ -771,8 +772,10 @@ int launch_gemm(GemmArgs a, hipStream_t st) {
     // a 64-tile alone on its CU has its chunks sooner there (300 x 1001 x 1001: 18 and 15)
     const double tiles64 = tile_count(a, 64, 64);
     if (near && (whole || tiles64 > 256)) {
-        const double c256 = tile_cost<T>(a, 256, 256, 1.10, 9.7, 7.28, 8.7), c64 = tile_cost<T>(a, 64, 64, 0.19, 0.4, 0.53, 0.3);
-        const double c128 = tile_cost<T>(a, 128, 128, 0.476, 1.4, 1.95, 1.6), c12864 = tile_cost<T>(a, 128, 64, 0.298, 1.0, 0.956, 1.2);
+        const bool alone = tile_count(a, 128, 128) <= 256;
+        const double c256 = tile_cost<T>(a, 256, 256, 1.10, 5.5, 7.29, 9.0), c64 = tile_cost<T>(a, 64, 64, 0.195, 0.3, 0.535, 0.3);
+        const double c128 = alone ? tile_cost<T>(a, 128, 128, 0.412, 0.0, 1.85, 0.8) : tile_cost<T>(a, 128, 128, 0.474, 0.9, 1.91, 1.8);
+        const double c12864 = tile_cost<T>(a, 128, 64, 0.296, 0.8, 0.99, 1.1);
         if (!whole) return c128 <= c64 ? launch_tile<T, 128, 128, 2, 4, 2, false>(a, st) : launch_tile<T, 64, 64, 2, 2, 2, false>(a, st);
         const int splits = a.partial ? split_count(a.M, a.N, a.K, Elem<T>::BYTES == 4 ? FR_TYPE_F32 : FR_TYPE_BF16) : 1;
         if (splits > 1) {
@@ -790,7 +793,7 @@ int launch_gemm(GemmArgs a, hipStream_t st) {
         // a deeper ring for a tile alone on its CU, more tiles at a time for others: 2048 cubed bf16 (128-tiles) 20 us, 26 with
         // the ring of 2; 200 x 4096 x 4096 (64-tiles) 16 us, 19 with the ring of 3; 32 experts' 64 rows, 4 tiles a CU, 20 and 16
         if (c64 <= c128) return tiles64 <= 256 ? launch_tile<T, 64, 64, 2, 2, 5>(a, st) : launch_tile<T, 64, 64, 2, 2, 3>(a, st);
-        return tile_count(a, 128, 128) <= 256 ? launch_tile<T, 128, 128, 2, 4, 3>(a, st) : launch_tile<T, 128, 128, 2, 4, 2>(a, st);
+        return alone ? launch_tile<T, 128, 128, 2, 4, 3>(a, st) : launch_tile<T, 128, 128, 2, 4, 2>(a, st);
     }
     const long mt = a.order ? a.M / 64 + std::min<long>(a.M, a.E + 1) : (a.M + 63) / 64;
     a.n_tiles = (a.N + 63) / 64;
