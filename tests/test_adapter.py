@@ -759,7 +759,7 @@ def test_linear_large_rows_of_any_alignment(kind, m, k, n):
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("m, k, n", [(2000, 1032, 1999), (1900, 520, 1700), (2047, 2056, 1030), (4622, 328, 2599), (5865, 136, 2633), (5014, 72, 1409),
-                                     (5821, 168, 131), (300, 648, 1500), (5726, 8, 140), (2048, 1024, 2048)])
+                                     (5821, 168, 131), (300, 648, 1500), (5726, 8, 140), (2048, 1024, 2048), (8866, 424, 69), (8831, 168, 1732)])
 def test_linear_every_tile(kind, m, k, n):
     """Sizes at which each of the tiles is the estimated best, in one type or the other."""
     g, dt = gen(m + k), TYPES[kind]
@@ -771,7 +771,7 @@ def test_linear_every_tile(kind, m, k, n):
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("t, e, k, d, n", [(4448, 12, 1, 328, 2406), (2273, 3, 3, 136, 2273), (2311, 12, 2, 72, 1436), (1228, 12, 1, 72, 1977),
-                                           (501, 12, 1, 176, 1159), (900, 70, 2, 1032, 990)])
+                                           (501, 12, 1, 176, 1159), (900, 70, 2, 1032, 990), (89, 8, 3, 400, 2002), (3342, 7, 3, 176, 1519), (376, 11, 1, 216, 1462)])
 def test_expert_linear_every_tile(kind, t, e, k, d, n):
     g, dt = gen(t + e + d), TYPES[kind]
     r = choose(g, t, e, k, 0.1)
