@@ -78,6 +78,17 @@ FR_DEV void store8t(void* base, long i, int type, const Vec8f& x) {
     }
 }
 
+// Sums over the lanes up to each lane.
+FR_DEV int scan_add(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);          // 1, 2, 4 and 8 lanes back in a row of 16
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);          // the row before; the two rows before
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+    return v;
+}
+
 // act(v) of the adapter products.  GELU is the erf form v Phi(v), SiLU v sigmoid(v).
 // exp2 and reciprocal are the hardware's (1 ulp).  Phi(-a) = erfc(a / sqrt 2) / 2 = t P(t) exp(-a^2 / 2) with
 // t = 1 / (1 + 0.3 a / sqrt 2): P is a minimax fit of erfcx(z) / t over t in (0.23, 1], 2.0e-8 relative, so small values of

@@ -47,16 +47,6 @@ template <> struct Elem<float> {
     }
 };
 
-// Sums over the lanes up to each lane.
-FR_DEV int scan_add(int v) {
-    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);          // 1, 2, 4 and 8 lanes back in a row of 16
-    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);          // the row before; the two rows before
-    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
-    return v;
-}
 // Expert e0 + lane (E: the slots without one): its rows [lo, hi) of the order and the row tiles from expert e0 to its end.
 // Bounds are clamped to [0, M), so a bad table reads and writes nothing outside.
 struct ExpertScan { int lo, hi, tiles, upto; };

@@ -6,7 +6,6 @@
 namespace {
 
 constexpr int RT_ROWS = 64;              // rows of a chunk = rows of a block of route_choose_kernel
-constexpr int RT_WAVES = 4;
 constexpr int RT_EMAX = 512, RT_KMAX = 16;
 
 struct RouteArgs {
@@ -201,18 +200,24 @@ FR_DEV void choose_exact(const RouteArgs& a, long row, double* keys, int* chosen
     wave_lds_fence();
 }
 
-// Places of one chunk's slots, by one wave: next[e] is the place of expert e's first slot here (E: none).  Equal experts
-// among 64 slots find each other by the bits of their number.
-FR_DEV void place_slots(const RouteArgs& a, int* next, const int* experts, int n, long slot0) {
+// The experts of a chunk's slots, 64 rows * k: k a lane.
+struct Slots { int ex[RT_KMAX]; };
+FR_DEV Slots load_slots(const int* experts, int n) {
     const int lane = threadIdx.x & 63;
-    int ex[RT_KMAX];                                         // 64 rows * k slots: k a lane, all asked for before the first is used
+    Slots s;
 #pragma unroll
-    for (int j = 0; j < RT_KMAX; ++j) ex[j] = j * 64 + lane < n ? experts[j * 64 + lane] : 0;
+    for (int j = 0; j < RT_KMAX; ++j) s.ex[j] = j * 64 + lane < n ? experts[j * 64 + lane] : 0;
+    return s;
+}
+// Their places, by one wave: next[e] is the place of expert e's first slot here (E: none).  Equal experts among 64 slots find
+// each other by the bits of their number.
+FR_DEV void place_slots(const RouteArgs& a, int* next, const Slots& s, int n, long slot0) {
+    const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int j = 0; j < RT_KMAX; ++j) {
         if (j * 64 >= n) break;
         const bool on = j * 64 + lane < n;
-        const int e = ex[j] < 0 ? a.E : ex[j];
+        const int e = s.ex[j] < 0 ? a.E : s.ex[j];
         unsigned long long same = __ballot(on);              // lanes with this lane's expert
         for (int bit = 0; (1 << bit) <= a.E; ++bit) {
             const bool set = (e >> bit) & 1;
@@ -244,14 +249,12 @@ FR_DEV void first_places(const RouteArgs& a, int* next, bool write, F n, G more)
     for (int q = 0; q <= RT_EMAX / 64; ++q) {
         if (q * 64 > a.E) break;
         const int e = q * 64 + lane;
-        int s = c[q];
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) { const int t = __shfl_up(s, o, 64); if (lane >= o) s += t; }
+        const int s = scan_add(c[q]);
         if (e <= a.E) {
             next[e] = before + s - c[q] + m[q];
             if (write) a.offsets[e] = before + s - c[q];
         }
-        before += __shfl(s, 63, 64);
+        before += __builtin_amdgcn_readlane(s, 63);
     }
     wave_lds_fence();
 }
@@ -267,15 +270,15 @@ FR_DEV void first_places(const RouteArgs& a, int* next, bool write, F n, G more)
 // (the row's sum of up to 512 besides).  At 65536 x 256, biased sigmoids, 8 of 256 in 4 of 8 groups, one row in 500 goes
 // that way; with the expert's number in the scored keys too it was one in 50, which took more time than all the rest.
 template <int V, int LPR, int NE, int NB, bool SCORED>
-__global__ __launch_bounds__(64 * RT_WAVES, 4) void route_choose_kernel(RouteArgs a) {
+__global__ __launch_bounds__(512, 4) void route_choose_kernel(RouteArgs a) {
     __shared__ int count[RT_EMAX + 1];
     __shared__ int chosen[RT_ROWS * RT_KMAX];
     __shared__ float bias[SCORED ? RT_EMAX + V : 1];
-    __shared__ double keys[RT_WAVES][NE * 64];
+    extern __shared__ double keys[];                         // [waves][NE * 64]
     constexpr unsigned MASK = (1u << NB) - 1;
     constexpr int RPW = 64 / LPR;
     constexpr float L2E = 1.4426950408889634f, DROP = 1.f / (float)(1u << (23 - NB));
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, rl = lane % LPR, base = lane - rl;
+    const int wave = threadIdx.x >> 6, waves = blockDim.x >> 6, lane = threadIdx.x & 63, rl = lane % LPR, base = lane - rl;
     for (int e = threadIdx.x; e <= a.E; e += blockDim.x) count[e] = 0;
     if constexpr (SCORED)                                    // in LDS: registers are what limits the waves a SIMD holds
         for (int e = threadIdx.x; e < RT_EMAX + V; e += blockDim.x) {
@@ -289,7 +292,7 @@ __global__ __launch_bounds__(64 * RT_WAVES, 4) void route_choose_kernel(RouteArg
     const float slack = a.score == FR_SCORE_SOFTMAX ? 0x1p-18f : 0x1p-21f;
     const int e0 = g * per + part * V, cnt = g < a.groups ? min(V, per - part * V) : 0;
 #pragma unroll 1
-    for (int it = wave; it * RPW < RT_ROWS; it += RT_WAVES) {
+    for (int it = wave; it * RPW < RT_ROWS && (long)blockIdx.x * RT_ROWS + it * RPW < a.T; it += waves) {
         const int r = it * RPW + lane / LPR;
         const long row = (long)blockIdx.x * RT_ROWS + r;
         const int have = row < a.T ? cnt : 0;
@@ -408,7 +411,7 @@ __global__ __launch_bounds__(64 * RT_WAVES, 4) void route_choose_kernel(RouteArg
         while (again) {
             const int rr = it * RPW + (__ffsll(again) - 1) / LPR;
             again &= again - 1;
-            choose_exact<NE>(a, (long)blockIdx.x * RT_ROWS + rr, keys[wave], chosen + rr * a.k);
+            choose_exact<NE>(a, (long)blockIdx.x * RT_ROWS + rr, keys + wave * NE * 64, chosen + rr * a.k);
         }
         const int pick = rl < a.k && row < a.T ? chosen[r * a.k + rl] : -1;
         const float pl = pick >= 0 ? load1(a.logits, row * a.E + pick, a.type) : -INFINITY;
@@ -429,7 +432,7 @@ __global__ __launch_bounds__(64 * RT_WAVES, 4) void route_choose_kernel(RouteArg
         for (int e = threadIdx.x; e <= a.E; e += blockDim.x) a.counts[(long)e * a.chunks + blockIdx.x] = count[e];
     } else if (wave == 0) {                                  // one chunk is all: order it here, one launch in place of three
         first_places(a, count, true, [&](int e) { return count[e]; }, [](int) { return 0; });
-        place_slots(a, count, chosen, (int)(a.T * a.k), 0);
+        place_slots(a, count, load_slots(chosen, (int)(a.T * a.k)), (int)(a.T * a.k), 0);
     }
 }
 
@@ -444,9 +447,7 @@ __global__ __launch_bounds__(256) void route_scan_kernel(RouteArgs a) {
         int n[4], t = 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) { n[j] = c + j < a.chunks ? row[c + j] : 0; t += n[j]; }
-        int s = t;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) { const int u = __shfl_up(s, o, 64); if (lane >= o) s += u; }
+        const int s = scan_add(t);
         int* p = part[turn & 1];
         if (lane == 63) p[wave] = s;
         __syncthreads();
@@ -465,15 +466,23 @@ __global__ __launch_bounds__(256) void route_scan_kernel(RouteArgs a) {
 // Places of a chunk's slots: first place of the expert + its slots in earlier chunks + earlier in this chunk.
 __global__ __launch_bounds__(64) void route_place_kernel(RouteArgs a) {
     __shared__ int next[RT_EMAX + 1];
-    first_places(a, next, blockIdx.x == 0, [&](int e) { return a.totals[e]; }, [&](int e) { return a.counts[(long)e * a.chunks + blockIdx.x]; });
     const long s0 = (long)blockIdx.x * RT_ROWS * a.k;
-    place_slots(a, next, a.experts + s0, (int)min((long)RT_ROWS * a.k, a.T * a.k - s0), s0);
+    const int n = (int)min((long)RT_ROWS * a.k, a.T * a.k - s0);
+    const Slots slots = load_slots(a.experts + s0, n);       // on their way while the places are found
+    first_places(a, next, blockIdx.x == 0, [&](int e) { return a.totals[e]; }, [&](int e) { return a.counts[(long)e * a.chunks + blockIdx.x]; });
+    place_slots(a, next, slots, n, s0);
 }
 
+// Blocks of 8 waves while 4 would leave places for waves empty (256 CUs hold 1024 blocks of 4): 20000 x 512 62 us, 79 by 4;
+// 65536 x 256, all 1024 blocks at once, 66 us by 4, 69 by 8.
 template <int V, int LPR, int NE, int NB>
 void launch_choose(const RouteArgs& a, hipStream_t st) {
-    if (a.bias || a.groups > 1) hipLaunchKernelGGL((route_choose_kernel<V, LPR, NE, 4, true>), dim3(a.chunks), dim3(64 * RT_WAVES), 0, st, a);
-    else hipLaunchKernelGGL((route_choose_kernel<V, LPR, NE, NB, false>), dim3(a.chunks), dim3(64 * RT_WAVES), 0, st, a);
+    const long needed = (a.T * LPR + 63) / 64;                // of a single chunk
+    const int waves = a.chunks > 512 ? 4 : (int)std::max(1l, std::min(8l, needed));
+    const dim3 grid(a.chunks), block(64 * waves);
+    const size_t lds = (size_t)waves * NE * 64 * sizeof(double);
+    if (a.bias || a.groups > 1) hipLaunchKernelGGL((route_choose_kernel<V, LPR, NE, 4, true>), grid, block, lds, st, a);
+    else hipLaunchKernelGGL((route_choose_kernel<V, LPR, NE, NB, false>), grid, block, lds, st, a);
 }
 
 }  // namespace

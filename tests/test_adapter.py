@@ -619,6 +619,15 @@ def test_route_many_rows():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("e, k", [(8, 2), (64, 4), (100, 3), (256, 8), (500, 10)])
+@pytest.mark.parametrize("t", [2, 4, 5, 9, 31, 32, 33, 63, 64, 65, 129])
+def test_route_few_rows(e, k, t):
+    g = gen(t + e)
+    check_route(randn(g, t, e), k, (t, e, k))
+    check_route(randn(g, t, e, dtype=torch.bfloat16), k, (t, e, k), score="sigmoid", bias=randn(g, e, scale=0.1))
+
+
+@pytest.mark.gpu
 def test_route_nothing():
     got = adapter.route(torch.zeros(0, 12, device="cuda"), 3)
     assert got.weights.shape == got.experts.shape == (0, 3) and got.order.shape == (0,) and got.offsets.tolist() == [0] * 13
