@@ -3,10 +3,14 @@ library is missing or a call fails, a RuntimeError is raised."""
 from __future__ import annotations
 
 import ctypes as C
+import functools
+import importlib.machinery
+import importlib.util
 import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libfr_hip.so")
+CALLS_PATH = os.path.join(_HERE, "_fr_calls.so")
 
 FR_PREC_BF16, FR_PREC_F32, FR_PREC_F24 = 0, 1, 2
 FR_PLAN_NO_FUSE = 0x100
@@ -105,6 +109,19 @@ def lib() -> C.CDLL:
             fn.restype, fn.argtypes = res, args
         _lib = l
     return _lib
+
+
+@functools.lru_cache(maxsize=None)
+def calls():
+    """The module of csrc/calls.cpp (built with the library), its entries bound to ``lib()``."""
+    if not os.path.exists(CALLS_PATH):
+        raise RuntimeError(f"{CALLS_PATH} is missing: it must be built (python -c 'import __graft_entry__ as g; g.build()')")
+    loader = importlib.machinery.ExtensionFileLoader("_fr_calls", CALLS_PATH)
+    module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_fr_calls", loader))
+    loader.exec_module(module)
+    names = ("fr_linear", "fr_linear_workspace_bytes", "fr_block_norm", "fr_route", "fr_route_workspace_bytes", "fr_expert_linear", "fr_last_error")
+    module.bind(*(C.cast(getattr(lib(), name), C.c_void_p).value for name in names))
+    return module
 
 
 def check(rc: int, what: str) -> None:

@@ -192,6 +192,8 @@ _ACTS = {"none": _lib.FR_ACT_NONE, "prelu": _lib.FR_ACT_PRELU, "hswish": _lib.FR
 _NORMS = {"none": _lib.FR_NORM_NONE, "rms": _lib.FR_NORM_RMS, "layer": _lib.FR_NORM_LAYER, "l2": _lib.FR_NORM_L2}
 _GATE_ACTS = {"none": _lib.FR_GATE_NONE, "sigmoid": _lib.FR_GATE_SIGMOID, "tanh": _lib.FR_GATE_TANH}
 _SCORES = {"softmax": _lib.FR_SCORE_SOFTMAX, "sigmoid": _lib.FR_SCORE_SIGMOID}
+_ROWS = {"tokens": 0, "sorted": 1}
+_OUTS = {"sorted": 0, "slots": 1}
 
 
 def _fail(op, what):
@@ -231,16 +233,24 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+def _current_device():
+    return torch._C._cuda_getDevice()
+
+
+def _current_stream(index):
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 def _call(name, dev, *args):
     """One C-ABI call on the device's current stream.  A call on one row takes a few microseconds on the GPU, so the host's
     share counts: no Stream object, no device switch where none is needed."""
     index = dev.index
     fn = _entry(name)
-    if torch._C._cuda_getDevice() == index:
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if _current_device() == index:
+        rc = fn(*args, _current_stream(index))
     else:
         with torch.cuda.device(dev):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+            rc = fn(*args, _current_stream(index))
     if rc:
         _lib.check(rc, name)
 
@@ -287,8 +297,15 @@ def _linear_shape(op, x, weight, residual):
     return shape
 
 
+# Each of the four first offers its call to csrc/calls.cpp, which takes the usual ones (plain contiguous tensors on the current
+# device) with a third of the host's time; the rest, and every wrong one, is dealt with here.
 def _linear(x, weight, bias, slope, residual, act, out_dtype):
     op = "linear"
+    if x.is_cuda:
+        index = _current_device()
+        y = _lib.calls().linear(x, weight, bias, slope, residual, _ACTS.get(act, -1), out_dtype, index, _current_stream(index))
+        if y is not None:
+            return y
     dev = _check_tensors(op, x, weight, bias, slope, residual)
     shape = _linear_shape(op, x, weight, residual)
     N, K = weight.shape
@@ -358,6 +375,13 @@ def _block_norm_eager(x, residual, slot_weights, norm, weight, bias, eps, gate, 
                       next_eps, out_dtype, next_dtype):
     """(out, next), None for a next that is not asked for."""
     op = "block_norm"
+    if x.is_cuda:
+        index = _current_device()
+        both = _lib.calls().block_norm(x, residual, slot_weights, _NORMS.get(norm, -1), weight, bias, eps, gate, _GATE_ACTS.get(gate_act, -1),
+                                       scale, _NORMS.get(next_norm, -1), next_weight, next_bias, next_eps, out_dtype, next_dtype,
+                                       index, _current_stream(index))
+        if both is not None:
+            return both
     dev = _check_tensors(op, x, residual, slot_weights, weight, bias, gate, next_weight, next_bias)
     shape = _block_norm_shape(op, x, slot_weights)
     d = x.shape[-1]
@@ -424,6 +448,11 @@ def _route_empty(logits, k):
 
 def _route(logits, k, score, bias, groups, top_groups, renormalise, scale):
     op = "route"
+    if logits.is_cuda:
+        index = _current_device()
+        out = _lib.calls().route(logits, k, _SCORES.get(score, -1), bias, groups, top_groups, renormalise, scale, index, _current_stream(index))
+        if out is not None:
+            return out
     dev = _check_tensors(op, logits, bias)
     T, E = _route_shape(op, logits, k)
     if not 1 <= groups <= 64 or not 1 <= top_groups <= groups:
@@ -459,6 +488,12 @@ def _expert_shape(op, x, weight, order, offsets, k, rows, out):
 
 def _expert_linear(x, weight, order, offsets, k, bias, act, slope, rows, out, out_dtype):
     op = "expert_linear"
+    if x.is_cuda:
+        index = _current_device()
+        y = _lib.calls().expert_linear(x, weight, order, offsets, k, bias, _ACTS.get(act, -1), slope, _ROWS.get(rows, -1), _OUTS.get(out, -1),
+                                       out_dtype, index, _current_stream(index))
+        if y is not None:
+            return y
     dev = _check_tensors(op, x, weight, order, offsets, bias, slope)
     T, shape = _expert_shape(op, x, weight, order, offsets, k, rows, out)
     E, N, K = weight.shape

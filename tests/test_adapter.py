@@ -923,6 +923,79 @@ def test_streams_and_graphs():
 
 
 @pytest.mark.gpu
+def test_usual_calls_take_the_short_way_and_answer_the_same(monkeypatch):
+    g = gen(77)
+    x, w, b, e = randn(g, 9, 64, dtype=torch.bfloat16), randn(g, 40, 64, dtype=torch.bfloat16), randn(g, 40), randn(g, 5, 40, 64, dtype=torch.bfloat16)
+    res, slope, logits, lb = randn(g, 9, 40), randn(g, 40), randn(g, 9, 5), randn(g, 5, scale=0.1)
+    gates, sw, y3 = [None, randn(g, 64), randn(g, 9, 1), randn(g, 9, 64)], randn(g, 9, 3), randn(g, 9, 3, 64)
+    nw, nb = randn(g, 64), randn(g, 64)
+    r = adapter.route(logits, 2)
+    calls = [lambda: adapter.linear(x, w), lambda: adapter.linear(x.view(3, 3, 64), w, b, act="prelu", slope=slope, residual=res.view(3, 3, 40), out_dtype=torch.float16),
+             lambda: adapter.linear(x, w, w.new_zeros(40), act="gelu", residual=res.half()), lambda: adapter.linear(x[0], w, residual=res[0]),
+             lambda: adapter.linear(randn(gen(5), 130, 2048), randn(gen(6), 70, 2048)),
+             lambda: adapter.route(logits, 3, score="sigmoid", bias=lb, groups=5, top_groups=4, renormalise=False, scale=2), lambda: adapter.route(logits.half(), 1),
+             lambda: adapter.route(logits[:0], 2), lambda: adapter.route(randn(gen(8), 700, 40), 4),
+             lambda: adapter.expert_linear(x, e, r, act="silu"), lambda: adapter.expert_linear(x, e, r, randn(gen(3), 5, 40), out="slots", out_dtype=torch.float32),
+             lambda: adapter.expert_linear(torch.cat([x, x]), e, r, act="prelu", slope=randn(gen(4), 5, 40), rows="sorted")]
+    for gate in gates:
+        calls += [lambda gate=gate: adapter.block_norm(x, x.float(), norm="layer", weight=nw, bias=nb, gate=gate, gate_act="tanh", scale=0.5),
+                  lambda gate=gate: adapter.block_norm(y3, slot_weights=sw, norm="rms", gate=gate, next_norm="layer", next_weight=nw, next_dtype=torch.bfloat16, eps=0)]
+    calls += [lambda: adapter.block_norm(x, norm="none", next_norm="l2", out_dtype=torch.float32), lambda: adapter.block_norm(x[0], norm="l2")]
+    flat = lambda v: tuple(v) if isinstance(v, tuple) else (v,)
+    taken = []
+
+    class Counted:
+        def __getattr__(self, name):
+            def call(*args):
+                v = getattr(real, name)(*args)
+                taken.append(v is not None)
+                return v
+            return call
+
+    class Never:
+        def __getattr__(self, name):
+            return lambda *args: None
+
+    real = _lib.calls()
+    monkeypatch.setattr(_lib, "calls", lambda: Counted())
+    short = [flat(c()) for c in calls]
+    assert all(taken) and len(taken) == len(calls)
+    monkeypatch.setattr(_lib, "calls", lambda: Never())
+    for i, (c, got) in enumerate(zip(calls, short)):
+        want = flat(c())
+        assert len(want) == len(got)
+        for a, z in zip(got, want):
+            assert a.dtype == z.dtype and a.shape == z.shape and a.stride() == z.stride() and a.device == z.device and torch.equal(a, z), i
+            assert not a.requires_grad
+    monkeypatch.setattr(_lib, "calls", lambda: Counted())
+    taken.clear()
+    wide = randn(g, 9, 128, dtype=torch.bfloat16)
+    with torch.no_grad():
+        adapter.linear(x.clone().requires_grad_(), w)
+    assert taken == [True]
+    taken.clear()
+    adapter.linear(wide[:, :64], w)
+    adapter.linear(x[:0], w)
+    adapter.block_norm(x.t().contiguous().t())
+    adapter.route(logits.t().contiguous().t(), 2)
+    adapter.route(logits, 2, scale=torch.tensor(1.0).numpy()[()].astype("float64"))
+    adapter.expert_linear(wide[:, :64], e, r)
+    wrong = (lambda: adapter.linear(x, w.float()), lambda: adapter.linear(x, w[:, :63]), lambda: adapter.linear(x, w, b[:39]), lambda: adapter.linear(x, w, act="tanh"),
+                lambda: adapter.linear(x, w, act="prelu"), lambda: adapter.linear(x, w, slope=slope), lambda: adapter.linear(x, w, residual=res[:8]),
+                lambda: adapter.linear(x, w.cpu()), lambda: adapter.linear(x.double(), w.double()), lambda: adapter.linear(x, w, out_dtype=torch.int32),
+                lambda: adapter.linear(x.clone().requires_grad_(), w), lambda: adapter.block_norm(x, norm="max"), lambda: adapter.block_norm(x, weight=nw[:63]),
+                lambda: adapter.block_norm(x, norm="l2", weight=nw), lambda: adapter.block_norm(x, gate=randn(g, 9)), lambda: adapter.block_norm(x, x[:8]),
+                lambda: adapter.block_norm(x, slot_weights=sw), lambda: adapter.route(logits, 6), lambda: adapter.route(logits, 2, bias=lb.half()),
+                lambda: adapter.route(logits, 2, groups=5, top_groups=6), lambda: adapter.route(logits, 2, score="max"),
+                lambda: adapter.expert_linear(x[:8], e, r), lambda: adapter.expert_linear(x, e[:4], r), lambda: adapter.expert_linear(x, e, r, randn(g, 40)),
+                lambda: adapter.expert_linear(x, e, r, rows="all"))
+    for bad in wrong:
+        with pytest.raises(RuntimeError, match="fr_hip::"):
+            bad()
+    assert len(taken) == 6 + len(wrong) and not any(taken)
+
+
+@pytest.mark.gpu
 def test_dispatched_ops_answer_as_the_functions_do():
     """torch.ops.fr_hip goes through the dispatcher, the functions of adapter straight to the implementation."""
     g = gen(50)
