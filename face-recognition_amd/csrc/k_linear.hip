@@ -230,6 +230,13 @@ FR_DEV void tile_of_block(int block, int mtiles, int ntiles, int& mt, int& nt) {
 // The one barrier of a slice stands between its halves: there its last fragments have been read and the next slice has
 // landed, and behind it the DMA of slice s + ST goes into its buffer, spread over the second half's products (in one
 // burst it held up the waves that issue it).
+// What bounds it: a slice of a 256-tile is 2048 clocks of matrix instructions, as much LDS traffic (each wave's 128 x 64 outputs
+// read 24 KB of the two halves, 8 waves 192, and 64 KB are written), and takes 2390 to 2550, at the 1.3 to 1.8 GHz the card
+// holds under it; launch, first loads and epilogue are 10 us a tile, which a tile alone on its CU does not hide.
+// bf16: 8192 cubed 754 us (1459 TFLOP/s; the library 662), 16384 x 2048 x 8192 383 (1435; 348), with bias and residual 403;
+// 65536 x 4096 x 1024 520, with silu 540; experts 65536 slots x 4096 x 1024 with silu 624.  fp32 8192 cubed 7.73 ms (142 of
+// 154).  Other ways to a 256-tile: 16 x 16 x 32 instructions reach 2145 TFLOP/s from registers alone, 32 x 32 x 16 1868; 4 waves
+// of 128 x 128 read less LDS, but their 256 accumulators leave no registers to read ahead.
 // WHOLE false: rows of any alignment.  The chunks of slice s + ST go to registers in the second half of slice s and to LDS in
 // the first half of the next, where ST = 2 wants them by its barrier.
 template <typename T, int BM, int BN, int WM, int WN, int ST, bool WHOLE>
@@ -487,7 +494,8 @@ __global__ __launch_bounds__(64 * WM * WN, BM == 128 && BN == 128 && ST == 2 ? 4
     }
 }
 
-// The parts of a split K added in their order, then the epilogue: 8 outputs a thread.
+// The parts of a split K added in their order, then the epilogue: 8 outputs a thread.  Bound by its launch: 128 x 4096 outputs in
+// 8 parts, 4.5 us of the product's 17.
 __global__ __launch_bounds__(256) void gemm_join_kernel(GemmArgs a) {
     const int vecs = (a.N + 7) / 8;
     const long i = blockIdx.x * 256l + threadIdx.x, row = i / vecs;
@@ -513,7 +521,8 @@ __global__ __launch_bounds__(256) void gemm_join_kernel(GemmArgs a) {
 // of x; its NW waves take the slices of K in turn, each with a ring of R slices of its own in LDS, so that nothing waits but
 // a wave for its own oldest slice; the waves' sums meet in LDS, in their order, and one launch does it all.
 // The ring is filled by LDS-DMA in whole lines of 128 bytes: fragments straight from memory take 64 bytes of 16 rows an
-// instruction, which the address path carries at half the rate (16 x 4096 x 4096: 12 us).  Rows that are not whole 16-byte
+// instruction, which the address path carries at half the rate (16 x 4096 x 4096: 12 us; 24 rows this way 8.6 in f16, 4.0 TB/s
+// of weights, with 3.3 us of launch and first loads in it).  Rows that are not whole 16-byte
 // chunks (WHOLE false) go through registers instead.
 template <typename T, int MT, int NW, int R, bool WHOLE>
 __global__ __launch_bounds__(64 * NW) void gemm_rows_kernel(GemmArgs a) {
@@ -612,7 +621,9 @@ __global__ __launch_bounds__(64 * NW) void gemm_rows_kernel(GemmArgs a) {
 }
 
 // Any shape, any alignment: 64 x 64 outputs a block, 4 waves of 32 x 32, slices of 128 bytes of K through registers into
-// LDS.  Piece p of LDS row r lies at p ^ ((r >> 1) & 7): the 16 rows of a fragment read fall on different banks.
+// LDS.  Piece p of LDS row r lies at p ^ ((r >> 1) & 7): the 16 rows of a fragment read fall on different banks.  For what the
+// staged kernel does not take: gathered rows beyond its 32-bit offsets, rows of 8 MB, few odd rows (300 x 1001 x 1001 bf16 15 us,
+// bound by the latency of one slice after the other).
 template <typename T>
 __global__ __launch_bounds__(256) void gemm_any_kernel(GemmArgs a) {
     __shared__ __attribute__((aligned(16))) unsigned char lds[2][64 * 128];

@@ -269,6 +269,8 @@ FR_DEV void first_places(const RouteArgs& a, int* next, bool write, F n, G more)
 // is at most 4 steps of 2^-24 for a sigmoid (exp2's argument and result, the sum, the reciprocal) and 32 for a softmax
 // (the row's sum of up to 512 besides).  At 65536 x 256, biased sigmoids, 8 of 256 in 4 of 8 groups, one row in 500 goes
 // that way; with the expert's number in the scored keys too it was one in 50, which took more time than all the rest.
+// What bounds it: 1030 vector and 350 scalar instructions for 4 rows of 256 (the read alone would take 15 us of the 53 at
+// 65536 x 256); a wave is done after 32 us in the mean, 41 at most without a row done again, and such a row takes 8.5.
 template <int V, int LPR, int NE, int NB, bool SCORED>
 __global__ __launch_bounds__(512, 4) void route_choose_kernel(RouteArgs a) {
     __shared__ int count[RT_EMAX + 1];
@@ -436,7 +438,8 @@ __global__ __launch_bounds__(512, 4) void route_choose_kernel(RouteArgs a) {
     }
 }
 
-// counts[e][c] -> number of e's slots in the chunks before c; totals[e].  One block per expert, four chunks a thread.
+// counts[e][c] -> number of e's slots in the chunks before c; totals[e].  One block per expert, four chunks a thread: 4 us for
+// 256 x 1024, launch and latency.
 __global__ __launch_bounds__(256) void route_scan_kernel(RouteArgs a) {
     __shared__ int part[2][4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -463,7 +466,8 @@ __global__ __launch_bounds__(256) void route_scan_kernel(RouteArgs a) {
     if (threadIdx.x == 0) a.totals[blockIdx.x] = before;
 }
 
-// Places of a chunk's slots: first place of the expert + its slots in earlier chunks + earlier in this chunk.
+// Places of a chunk's slots: first place of the expert + its slots in earlier chunks + earlier in this chunk.  524288 slots of
+// 256 experts 8.4 us: 512 slots a wave, 64 at a time, each after the one before.
 __global__ __launch_bounds__(64) void route_place_kernel(RouteArgs a) {
     __shared__ int next[RT_EMAX + 1];
     const long s0 = (long)blockIdx.x * RT_ROWS * a.k;
