@@ -704,7 +704,7 @@ __global__ __launch_bounds__(256) void gemm_any_kernel(GemmArgs a) {
 template <typename T, int BM, int BN, int WM, int WN, int ST, bool WHOLE = true>
 int launch_tile(GemmArgs a, hipStream_t st) {
     const long mt = a.order ? a.M / BM + std::min<long>(a.M, a.E + 1) : (a.M + BM - 1) / BM;
-    a.n_tiles = (a.N + BN - 1) / BN;
+    a.n_tiles = (int)((a.N + (BN - 1l)) / BN);
     if (mt * a.n_tiles * a.splits >= (1l << 32) / (64 * WM * WN)) FR_FAIL(FR_ERR_UNSUPPORTED, "adapter product: more output tiles than a launch takes");
     const int lds = ST * (BM + BN) * 128;
     static_assert(WN * BM <= ST * (BM + BN), "the ring has room for the vectors that N ends in: 32 bytes a lane and row tile");
@@ -718,7 +718,7 @@ int launch_tile(GemmArgs a, hipStream_t st) {
 double tile_count(const GemmArgs& a, int bm, int bn) {
     const double some = a.order ? (double)std::min<long>(a.M, a.E) : 0;
     const double rows = a.order ? std::max((double)a.M / bm + 0.5 * some, some) : (double)((a.M + bm - 1) / bm);
-    return rows * ((a.N + bn - 1) / bn);
+    return rows * ((a.N + (bn - 1l)) / bn);
 }
 // Estimated time in us with tiles of bm x bn: `each` for a slice of 128 bytes of K and `fixed` for the rest of a tile, for every
 // tile of the fullest CU.  The constants are least squares over 90 shapes of 64 to 18 000 rows on one card (rms 3 % in fp32,
@@ -733,7 +733,7 @@ double tile_cost(const GemmArgs& a, int bm, int bn, double each16, double fixed1
 template <typename T, int MT, int NW, int R>
 int launch_rows(GemmArgs a, bool whole, hipStream_t st) {
     const long mt = (a.M + 16 * MT - 1) / (16 * MT);
-    a.n_tiles = (a.N + 15) / 16;
+    a.n_tiles = (int)((a.N + 15l) / 16);
     if (mt * a.n_tiles >= (1l << 32) / (64 * NW)) FR_FAIL(FR_ERR_UNSUPPORTED, "adapter product: more output tiles than a launch takes");
     const int lds = NW * R * (16 + 16 * MT) * 128;
     const dim3 grid((unsigned)(mt * a.n_tiles)), block(64 * NW);
@@ -748,7 +748,7 @@ int launch_rows(GemmArgs a, bool whole, hipStream_t st) {
 // K of a product whose 64-tiles leave most of the card idle is split into parts of at least 4 slices, up to two blocks a CU.
 // 128 x 4096 x 4096 bf16: 17 us, 20 in one part; K of fewer than 16 slices saves less than the second launch takes.
 int split_count(int64_t M, int N, int K, int type) {
-    const long slices = ((long)K * type_bytes(type) + 127) / 128, tiles = ((M + 63) / 64) * ((N + 63) / 64);
+    const long slices = ((long)K * type_bytes(type) + 127) / 128, tiles = ((M + 63) / 64) * ((N + 63l) / 64);
     if (M <= 64 || tiles > 160 || slices < 16) return 1;        // up to 64 rows: gemm_rows_kernel
     return (int)std::max(1l, std::min(std::min(slices / 4, 512 / tiles), 16l));
 }
@@ -799,7 +799,7 @@ int launch_gemm(GemmArgs a, hipStream_t st) {
         return alone ? launch_tile<T, 128, 128, 2, 4, 3>(a, st) : launch_tile<T, 128, 128, 2, 4, 2>(a, st);
     }
     const long mt = a.order ? a.M / 64 + std::min<long>(a.M, a.E + 1) : (a.M + 63) / 64;
-    a.n_tiles = (a.N + 63) / 64;
+    a.n_tiles = (int)((a.N + 63l) / 64);
     if (mt >= 1l << 24 || a.n_tiles >= 1 << 24) FR_FAIL(FR_ERR_UNSUPPORTED, "adapter product: more output tiles than a launch takes");
     hipLaunchKernelGGL((gemm_any_kernel<T>), dim3(a.n_tiles, (unsigned)std::min(mt, 65535l), (unsigned)((mt + 65534) / 65535)), dim3(256), 0, st, a);
     FR_LAUNCH_CHECK("gemm_any_kernel");

@@ -204,6 +204,19 @@ def test_c_entries_refuse_before_they_launch():
     assert expert(T=0) == 0
 
 
+@pytest.mark.parametrize("M, K", [(1, 1), (1, 8), (64, 1), (65, 8), (1, 512)])
+def test_c_entries_refuse_outputs_wider_than_a_launch(M, K):
+    """N of nearly 31 bits: the tiles are counted in 64 bits and refused before anything is launched."""
+    lib, at, need = _lib.lib(), 4096, C.c_size_t()
+    for N in (2 ** 31 - 1, 2 ** 31 - 8, 2 ** 31 - 64):
+        assert lib.fr_linear_workspace_bytes(M, N, K, _lib.FR_TYPE_BF16, C.byref(need)) == 0
+        assert need.value == 0
+        rc = lib.fr_linear(at, K, at, None, None, None, 0, at, M, N, K, 1, 1, 1, 1, 0, None, 0, None)
+        assert rc != 0 and b"tiles" in lib.fr_last_error()
+        rc = lib.fr_expert_linear(at, 0, at, None, None, at, at, at, 0, M, 1, 1, N, K, 1, 1, 1, 0, None)
+        assert rc != 0 and b"tiles" in lib.fr_last_error()
+
+
 @pytest.mark.gpu
 def test_plans_refuse_the_new_activations():
     w = torch.zeros(8, 8, 1, 1)
@@ -972,7 +985,10 @@ def test_usual_calls_take_the_short_way_and_answer_the_same(monkeypatch):
     wide = randn(g, 9, 128, dtype=torch.bfloat16)
     with torch.no_grad():
         adapter.linear(x.clone().requires_grad_(), w)
-    assert taken == [True]
+    with torch.inference_mode():
+        y = adapter.linear(x, w)
+        assert y.is_inference() and torch.equal(y, short[0][0])
+    assert taken == [True, True]
     taken.clear()
     adapter.linear(wide[:, :64], w)
     adapter.linear(x[:0], w)
