@@ -389,9 +389,15 @@ __global__ __launch_bounds__(512, 4) void route_choose_kernel(RouteArgs a) {
                 wins += here;
             }
             const unsigned pop = here ? ~0u : 0u;            // the winner's next key moves up: one bit select a key
+            if (V <= 8 || a.k <= 8) {                        // no more than k + 1 rounds: nothing behind the ninth key becomes a head
 #pragma unroll
-            for (int v = 0; v + 1 < V; ++v) key[v] = (key[v + 1] & pop) | (key[v] & ~pop);
-            key[V - 1] &= ~pop;
+                for (int v = 0; v < (V <= 8 ? V - 1 : 8); ++v) key[v] = (key[v + 1] & pop) | (key[v] & ~pop);
+                if (V <= 8) key[V - 1] &= ~pop;
+            } else {
+#pragma unroll
+                for (int v = 0; v + 1 < V; ++v) key[v] = (key[v + 1] & pop) | (key[v] & ~pop);
+                key[V - 1] &= ~pop;
+            }
         }
         {
             const unsigned x = (unsigned)__shfl((int)mine, max(lane - 1, base), 64) & ~MASK, y = mine & ~MASK;
