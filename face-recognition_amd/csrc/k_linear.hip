@@ -770,25 +770,25 @@ int launch_gemm(GemmArgs a, hipStream_t st) {
         return launch_rows<T, 4, 4, 3>(a, whole, st);
     }
     // rows of any alignment, us against gemm_any_kernel: 16384 x 2048 x 4097 bf16 455 and 723, 3001 x 2047 x 2049 68 and 90;
-    // a 64-tile alone on its CU has its chunks sooner there (300 x 1001 x 1001: 18 and 15)
+    // a 64-tile alone on its CU has its chunks sooner there (300 x 1001 x 1001: 18 and 15), but for K in parts
     const double tiles64 = tile_count(a, 64, 64);
-    if (near && (whole || tiles64 > 256)) {
+    const int splits = a.partial ? split_count(a.M, a.N, a.K, Elem<T>::BYTES == 4 ? FR_TYPE_F32 : FR_TYPE_BF16) : 1;
+    if (near && (whole || tiles64 > 256 || splits > 1)) {
         const bool alone = tile_count(a, 128, 128) <= 256;
         const double c256 = tile_cost<T>(a, 256, 256, 1.10, 5.5, 7.29, 9.0), c64 = tile_cost<T>(a, 64, 64, 0.195, 0.3, 0.535, 0.3);
         const double c128 = alone ? tile_cost<T>(a, 128, 128, 0.412, 0.0, 1.85, 0.8) : tile_cost<T>(a, 128, 128, 0.474, 0.9, 1.91, 1.8);
         const double c12864 = tile_cost<T>(a, 128, 64, 0.296, 0.8, 0.99, 1.1);
-        if (!whole) return c128 <= c64 ? launch_tile<T, 128, 128, 2, 4, 2, false>(a, st) : launch_tile<T, 64, 64, 2, 2, 2, false>(a, st);
-        const int splits = a.partial ? split_count(a.M, a.N, a.K, Elem<T>::BYTES == 4 ? FR_TYPE_F32 : FR_TYPE_BF16) : 1;
         if (splits > 1) {
             const long slices = (rowb + 127) / 128;
             a.split_slices = (int)((slices + splits - 1) / splits);
             a.splits = (int)((slices + a.split_slices - 1) / a.split_slices);
-            const int rc = launch_tile<T, 64, 64, 2, 2, 3>(a, st);
+            const int rc = whole ? launch_tile<T, 64, 64, 2, 2, 3>(a, st) : launch_tile<T, 64, 64, 2, 2, 2, false>(a, st);
             if (rc) return rc;
             hipLaunchKernelGGL(gemm_join_kernel, dim3((unsigned)((a.M * ((a.N + 7) / 8) + 255) / 256)), dim3(256), 0, st, a);
             FR_LAUNCH_CHECK("gemm_join_kernel");
             return FR_OK;
         }
+        if (!whole) return c128 <= c64 ? launch_tile<T, 128, 128, 2, 4, 2, false>(a, st) : launch_tile<T, 64, 64, 2, 2, 2, false>(a, st);
         // an expert's few rows are one tile of any height: 5 rows, 2 of 32 experts, 512 -> 2048: 7.0 us by 64-tiles, 10.8 by 128
         const bool few = a.order && a.M <= 32 * std::min<long>(a.M, a.E);
         if (!few && c256 <= std::min(c128, std::min(c12864, c64))) return launch_tile<T, 256, 256, 2, 4, 2>(a, st);

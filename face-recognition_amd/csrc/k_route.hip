@@ -368,12 +368,16 @@ __global__ __launch_bounds__(512, 4) void route_choose_kernel(RouteArgs a) {
                 doubt = !(least - most > 2.f * slack * fmaxf(1.f, fabsf(least))) && row_max<LPR>(b1) > -INFINITY;
             }
         }
+        // without a bias 16-bit logits order as their scores do and leave room for the expert's number: equal ones need no care
+        constexpr unsigned NUMBER = RT_EMAX - 1;
+        const bool by_logit = SCORED && a.type != FR_TYPE_F32 && !a.bias;
         unsigned key[V];                                     // up to that of -inf: not to be chosen
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            unsigned u = __float_as_uint(f[v]);
+            unsigned u = __float_as_uint(by_logit ? l[v] + 0.f : f[v]);
             u ^= (unsigned)((int)u >> 31) | 0x80000000u;
-            key[v] = ((u & ~MASK) | (MASK - (unsigned)(SCORED ? v : e0 + v))) & kept;
+            if (by_logit) key[v] = ((u & ~NUMBER) | (NUMBER - min((unsigned)(e0 + v), NUMBER))) & kept;
+            else key[v] = ((u & ~MASK) | (MASK - (unsigned)(SCORED ? v : e0 + v))) & kept;
         }
         constexpr unsigned LEAST = 0x007FFFFFu | MASK;
         sort_down<V>(key);
@@ -385,7 +389,7 @@ __global__ __launch_bounds__(512, 4) void route_choose_kernel(RouteArgs a) {
             if (rl == j) mine = top;
             const bool here = key[0] == top && top;
             if constexpr (SCORED) {
-                if (here && j < a.k) chosen[r * a.k + j] = e0 + (int)(MASK - (top & MASK));
+                if (here && j < a.k) chosen[r * a.k + j] = by_logit ? (int)(NUMBER - (top & NUMBER)) : e0 + (int)(MASK - (top & MASK));
                 wins += here;
             }
             const unsigned pop = here ? ~0u : 0u;            // the winner's next key moves up: one bit select a key
@@ -403,11 +407,17 @@ __global__ __launch_bounds__(512, 4) void route_choose_kernel(RouteArgs a) {
             const unsigned x = (unsigned)__shfl((int)mine, max(lane - 1, base), 64) & ~MASK, y = mine & ~MASK;
             bool close = false;                              // this lane's key to the one before
             if constexpr (!SCORED) close = a.type == FR_TYPE_F32 && x == y;
-            else {
+            else if (by_logit) {
+                // but for logits whose neighbours in their type may have the same score in doubles, which the lower expert wins:
+                // sigmoids next to 1 (steps of 2^-6 times e^-30 still show), scores below e^-600, logits below 2^-30
+                const unsigned w = mine & ~NUMBER;
+                const float t = __uint_as_float(w & 0x80000000u ? w ^ 0x80000000u : ~w);
+                close = t > (a.score == FR_SCORE_SOFTMAX ? INFINITY : 30.f) || t - m < -600.f || (t != 0.f && fabsf(t) < 0x1p-30f);
+            } else {
                 const float fx = __uint_as_float(x & 0x80000000u ? x ^ 0x80000000u : ~x), fy = __uint_as_float(y & 0x80000000u ? y ^ 0x80000000u : ~y);
                 close = !(fx - fy > slack * fmaxf(1.f, fabsf(fx)) + 2.f * DROP * fmaxf(fabsf(fx), fabsf(fy)));
             }
-            unsigned flag = close && mine && rl > 0 && rl <= a.k;
+            unsigned flag = close && mine && (rl > 0 || by_logit) && rl <= a.k;
             // equal keys of two lanes win the same round: more wins than keys
             if constexpr (SCORED) flag |= row_addu<LPR>(wins) != row_addu<LPR>(mine && rl <= a.k ? 1u : 0u);
             doubt |= row_maxu<LPR>(flag) != 0;
@@ -492,7 +502,7 @@ void launch_choose(const RouteArgs& a, hipStream_t st) {
     const dim3 grid(a.chunks), block(64 * waves);
     const size_t lds = (size_t)waves * NE * 64 * sizeof(double);
     if (a.bias || a.groups > 1) hipLaunchKernelGGL((route_choose_kernel<V, LPR, NE, 4, true>), grid, block, lds, st, a);
-    else hipLaunchKernelGGL((route_choose_kernel<V, LPR, NE, NB, false>), grid, block, lds, st, a);
+    else if constexpr (LPR < 64) hipLaunchKernelGGL((route_choose_kernel<V, LPR, NE, NB, false>), grid, block, lds, st, a);      // 64 lanes: groups
 }
 
 }  // namespace

@@ -641,6 +641,20 @@ def test_route_few_rows(e, k, t):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("e, k, groups, top", [(204, 8, 4, 4), (16, 4, 2, 1), (64, 6, 8, 3), (500, 10, 20, 7), (480, 5, 32, 32)])
+def test_route_equal_logits_in_groups(kind, score, e, k, groups, top):
+    """16-bit logits without a bias: many equal ones; ones that differ and have the same score in doubles; masks."""
+    g, kw = gen(e + k), dict(score=score, groups=groups, top_groups=top)
+    x = randn(g, 70, e, dtype=TYPES[kind])
+    for what, l in (("random", x), ("few values", (x.float() * 2).round().to(x.dtype) / 2), ("near 1", x + 25), ("at 1", x * 4 + 60), ("low", x * 30 - 590),
+                    ("tiny", x * 1e-7 if kind == "f16" else x * 1e-30), ("some tiny", torch.where(x > 0.5, x * (1e-6 if kind == "f16" else 1e-20), x.abs() * -3)),
+                    ("zeros", torch.where(x > 0, 0.0, -0.0).to(x.dtype)), ("wide", x * 300), ("masked", x.masked_fill(randn(g, 70, e) > 0.3, -math.inf))):
+        check_route(l, k, what=(kind, score, e, what), **kw)
+
+
+@pytest.mark.gpu
 def test_route_nothing():
     got = adapter.route(torch.zeros(0, 12, device="cuda"), 3)
     assert got.weights.shape == got.experts.shape == (0, 3) and got.order.shape == (0,) and got.offsets.tolist() == [0] * 13
@@ -788,6 +802,20 @@ def test_linear_every_tile(kind, m, k, n):
     x, w, b, res = randn(g, m, k, dtype=dt), randn(g, n, k, dtype=dt, scale=k ** -0.5), randn(g, n), randn(g, m, n, dtype=dt)
     want = oa.linear(x, w, b, residual=res, name="relu")
     close(adapter.linear(x, w, b, residual=res, act="relu"), want, linear_tol(x, w, b, res, want, dt), (kind, m, k, n))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("m, k, n", [(156, 3937, 200), (65, 1025, 70), (300, 2051, 129), (90, 1333, 1000)])
+def test_linear_odd_rows_in_parts(kind, m, k, n):
+    """Rows of any alignment whose K is split over parts."""
+    g, dt = gen(m + k), TYPES[kind]
+    x, w, b, res = randn(g, m, k, dtype=dt), randn(g, n, k, dtype=dt, scale=k ** -0.5), randn(g, n), randn(g, m, n, dtype=dt)
+    want = oa.linear(x, w, b, residual=res, name="silu")
+    close(adapter.linear(x, w, b, residual=res, act="silu"), want, linear_tol(x, w, b, res, want, dt), (kind, m, k, n))
+    wide = torch.randn(m, k + 3, device="cuda", generator=g).to(dt)[:, 1:k + 1]
+    want = oa.linear(wide, w)
+    close(adapter.linear(wide, w), want, linear_tol(wide, w, None, None, want, dt), "apart")
 
 
 @pytest.mark.gpu
