@@ -770,15 +770,17 @@ int launch_gemm(GemmArgs a, hipStream_t st) {
         return launch_rows<T, 4, 4, 3>(a, whole, st);
     }
     // rows of any alignment, us against gemm_any_kernel: 16384 x 2048 x 4097 bf16 455 and 723, 3001 x 2047 x 2049 68 and 90;
-    // a 64-tile alone on its CU has its chunks sooner there (300 x 1001 x 1001: 18 and 15), but for K in parts
+    // a 64-tile alone on its CU has its chunks sooner there (300 x 1001 x 1001: 18 and 15, in parts of K 16), but for
+    // a long K in parts (554 x 242 x 1461 f32 45 and 22, 156 x 1024 x 7874 f16 73 and 21)
     const double tiles64 = tile_count(a, 64, 64);
     const int splits = a.partial ? split_count(a.M, a.N, a.K, Elem<T>::BYTES == 4 ? FR_TYPE_F32 : FR_TYPE_BF16) : 1;
-    if (near && (whole || tiles64 > 256 || splits > 1)) {
+    const bool parts = splits > 1 && (whole || rowb >= 24 * 128);
+    if (near && (whole || tiles64 > 256 || parts)) {
         const bool alone = tile_count(a, 128, 128) <= 256;
         const double c256 = tile_cost<T>(a, 256, 256, 1.10, 5.5, 7.29, 9.0), c64 = tile_cost<T>(a, 64, 64, 0.195, 0.3, 0.535, 0.3);
         const double c128 = alone ? tile_cost<T>(a, 128, 128, 0.412, 0.0, 1.85, 0.8) : tile_cost<T>(a, 128, 128, 0.474, 0.9, 1.91, 1.8);
         const double c12864 = tile_cost<T>(a, 128, 64, 0.296, 0.8, 0.99, 1.1);
-        if (splits > 1) {
+        if (parts) {
             const long slices = (rowb + 127) / 128;
             a.split_slices = (int)((slices + splits - 1) / splits);
             a.splits = (int)((slices + a.split_slices - 1) / a.split_slices);

@@ -261,18 +261,23 @@ FR_DEV void first_places(const RouteArgs& a, int* next, bool write, F n, G more)
 
 // A row takes LPR > k lanes, a lane up to V experts of one group, in index order over the lanes.  A lane sorts its keys, and
 // the k best (and one more, for the doubt) are maxima over the row of the lanes' heads.  Keys are unique in their lane: f32
-// in unsigned order, the low NB bits replaced by an index (greater for lower
-// ones).  Unscored rows (no bias, one group) order by the logits themselves and put the expert's number there: unique in
-// the row, ties need no care, and with 16-bit logits nothing is lost.  Scored rows put the place in the lane there, 4 bits.
+// in unsigned order, the low bits replaced by an index (greater for lower ones).
+// BY_LOGIT (no bias, one group): the logits themselves, with the expert's number in NB bits: unique in the row, ties need no
+// care, and with 16-bit logits nothing is lost.
+// BY_LOGIT_IN_GROUPS (no bias, 16 bits): the same key; only the groups are compared by their scores.  By scores, whose equal
+// ones made nearly every row a doubtful one, 171 x 204, 8 of 204 in 4 groups, took 59 us, and takes 24.
+// BY_SCORE: score and bias, with the place in the lane in NB = 4 bits.
 // A row is done again by the whole wave in doubles where f32 cannot vouch for the choice: where two neighbours in the order
 // (or the groups on either side of the cut) are no further apart than the bits dropped and the error of their scores, which
 // is at most 4 steps of 2^-24 for a sigmoid (exp2's argument and result, the sum, the reciprocal) and 32 for a softmax
 // (the row's sum of up to 512 besides).  At 65536 x 256, biased sigmoids, 8 of 256 in 4 of 8 groups, one row in 500 goes
 // that way; with the expert's number in the scored keys too it was one in 50, which took more time than all the rest.
-// What bounds it: 1030 vector and 350 scalar instructions for 4 rows of 256 (the read alone would take 15 us of the 53 at
+// What bounds it: 970 vector and 370 scalar instructions for 4 rows of 256 (the read alone would take 15 us of the 51 at
 // 65536 x 256); a wave is done after 32 us in the mean, 41 at most without a row done again, and such a row takes 8.5.
-template <int V, int LPR, int NE, int NB, bool SCORED>
+enum { BY_LOGIT, BY_SCORE, BY_LOGIT_IN_GROUPS };
+template <int V, int LPR, int NE, int NB, int ORDER>
 __global__ __launch_bounds__(512, 4) void route_choose_kernel(RouteArgs a) {
+    constexpr bool SCORED = ORDER != BY_LOGIT, by_logit = ORDER == BY_LOGIT_IN_GROUPS;
     __shared__ int count[RT_EMAX + 1];
     __shared__ int chosen[RT_ROWS * RT_KMAX];
     __shared__ float bias[SCORED ? RT_EMAX + V : 1];
@@ -368,9 +373,7 @@ __global__ __launch_bounds__(512, 4) void route_choose_kernel(RouteArgs a) {
                 doubt = !(least - most > 2.f * slack * fmaxf(1.f, fabsf(least))) && row_max<LPR>(b1) > -INFINITY;
             }
         }
-        // without a bias 16-bit logits order as their scores do and leave room for the expert's number: equal ones need no care
         constexpr unsigned NUMBER = RT_EMAX - 1;
-        const bool by_logit = SCORED && a.type != FR_TYPE_F32 && !a.bias;
         unsigned key[V];                                     // up to that of -inf: not to be chosen
 #pragma unroll
         for (int v = 0; v < V; ++v) {
@@ -407,7 +410,7 @@ __global__ __launch_bounds__(512, 4) void route_choose_kernel(RouteArgs a) {
             const unsigned x = (unsigned)__shfl((int)mine, max(lane - 1, base), 64) & ~MASK, y = mine & ~MASK;
             bool close = false;                              // this lane's key to the one before
             if constexpr (!SCORED) close = a.type == FR_TYPE_F32 && x == y;
-            else if (by_logit) {
+            else if constexpr (by_logit) {
                 // but for logits whose neighbours in their type may have the same score in doubles, which the lower expert wins:
                 // sigmoids next to 1 (steps of 2^-6 times e^-30 still show), scores below e^-600, logits below 2^-30
                 const unsigned w = mine & ~NUMBER;
@@ -501,8 +504,9 @@ void launch_choose(const RouteArgs& a, hipStream_t st) {
     const int waves = a.chunks > 512 ? 4 : (int)std::max(1l, std::min(8l, needed));
     const dim3 grid(a.chunks), block(64 * waves);
     const size_t lds = (size_t)waves * NE * 64 * sizeof(double);
-    if (a.bias || a.groups > 1) hipLaunchKernelGGL((route_choose_kernel<V, LPR, NE, 4, true>), grid, block, lds, st, a);
-    else if constexpr (LPR < 64) hipLaunchKernelGGL((route_choose_kernel<V, LPR, NE, NB, false>), grid, block, lds, st, a);      // 64 lanes: groups
+    if (a.groups > 1 && !a.bias && a.type != FR_TYPE_F32) hipLaunchKernelGGL((route_choose_kernel<V, LPR, NE, 4, BY_LOGIT_IN_GROUPS>), grid, block, lds, st, a);
+    else if (a.bias || a.groups > 1) hipLaunchKernelGGL((route_choose_kernel<V, LPR, NE, 4, BY_SCORE>), grid, block, lds, st, a);
+    else if constexpr (LPR < 64) hipLaunchKernelGGL((route_choose_kernel<V, LPR, NE, NB, BY_LOGIT>), grid, block, lds, st, a);      // 64 lanes: groups
 }
 
 }  // namespace
