@@ -517,21 +517,26 @@ __global__ __launch_bounds__(256) void gemm_join_kernel(GemmArgs a) {
     finish8(a, row, n, columns(a, n, have, 0, false), v, false);
 }
 
-// Few rows: the weights are read once and are nearly all there is to read.  A block takes 16 weight rows and up to 16 MT rows
+// Few rows, of one matrix or of each expert: the weights are read once and are nearly all there is to read.  A block takes 16 weight rows and up to 16 MT rows
 // of x; its NW waves take the slices of K in turn, each with a ring of R slices of its own in LDS, so that nothing waits but
 // a wave for its own oldest slice; the waves' sums meet in LDS, in their order, and one launch does it all.
 // The ring is filled by LDS-DMA in whole lines of 128 bytes: fragments straight from memory take 64 bytes of 16 rows an
 // instruction, which the address path carries at half the rate (16 x 4096 x 4096: 12 us; 24 rows this way 8.6 in f16, 4.0 TB/s
 // of weights, with 3.3 us of launch and first loads in it).  Rows that are not whole 16-byte
 // chunks (WHOLE false) go through registers instead.
-template <typename T, int MT, int NW, int R, bool WHOLE>
+template <typename T, int MT, int NW, int R, bool WHOLE, bool EXPERTS>
 __global__ __launch_bounds__(64 * NW) void gemm_rows_kernel(GemmArgs a) {
     constexpr int ROWS = 16 + 16 * MT, DPS = ROWS / 8, SLOT = ROWS * 128;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int li = lane & 15, lg = lane >> 4;
     const int nt = blockIdx.x % a.n_tiles, mt = blockIdx.x / a.n_tiles, n0 = nt * 16;
-    const long r0 = (long)mt * 16 * MT, r1 = min(r0 + 16 * MT, a.M), rowb = (long)a.K * Elem<T>::BYTES;
+    long r0 = (long)mt * 16 * MT, r1 = min(r0 + 16 * MT, a.M);
+    int expert = 0;
+    if constexpr (EXPERTS)
+        if (!expert_tile(a, mt, 16 * MT, scan_experts(a, 0, 16 * MT), expert, r0, r1)) return;
+    const bool none = EXPERTS && expert == a.E;
+    const long nbase = (long)expert * a.N, rowb = (long)a.K * Elem<T>::BYTES;
     f32x4 acc[MT];
 #pragma unroll
     for (int j = 0; j < MT; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -544,10 +549,10 @@ __global__ __launch_bounds__(64 * NW) void gemm_rows_kernel(GemmArgs a) {
 #pragma unroll
     for (int d = 0; d < DPS; ++d) {
         const int r = 8 * d + (lane >> 3);
-        src[d] = (d < 2 ? reinterpret_cast<const unsigned char*>(a.w) + (long)min(n0 + r, a.N - 1) * rowb
-                        : reinterpret_cast<const unsigned char*>(a.x) + min(r0 + r - 16, r1 - 1) * a.ldx * Elem<T>::BYTES) + kx[d & 1];
+        src[d] = (d < 2 ? reinterpret_cast<const unsigned char*>(a.w) + ((none ? 0 : nbase) + min(n0 + r, a.N - 1)) * rowb
+                        : reinterpret_cast<const unsigned char*>(a.x) + (EXPERTS ? x_row(a, min(r0 + r - 16, r1 - 1)) : min(r0 + r - 16, r1 - 1)) * a.ldx * Elem<T>::BYTES) + kx[d & 1];
     }
-    const int slices = (int)((rowb + 127) / 128), mine = (slices - wave + NW - 1) / NW;    // <= 0: more waves than slices
+    const int slices = none ? 0 : (int)((rowb + 127) / 128), mine = (slices - wave + NW - 1) / NW;    // <= 0: more waves than slices
     auto multiply = [&](const unsigned char* slot) __attribute__((always_inline)) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -615,9 +620,9 @@ __global__ __launch_bounds__(64 * NW) void gemm_rows_kernel(GemmArgs a) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) { v.v[e] += lo[e]; v.v[4 + e] += hi[e]; }
     }
-    const long row = r0 + 16 * j + i;
+    const long at = r0 + 16 * j + i, row = at >= r1 ? -1 : EXPERTS ? out_row(a, at) : at;
     const int n = n0 + half * 8;
-    if (row < r1 && n < a.N) finish8(a, row, n, columns(a, n, min(8, a.N - n), 0, false), v, false);
+    if (row >= 0 && n < a.N) finish8(a, row, n, columns(a, n, min(8, a.N - n), nbase, none), v, none);
 }
 
 // Any shape, any alignment: 64 x 64 outputs a block, 4 waves of 32 x 32, slices of 128 bytes of K through registers into
@@ -730,17 +735,17 @@ double tile_cost(const GemmArgs& a, int bm, int bn, double each16, double fixed1
     return ceil(tile_count(a, bm, bn) / 256) * (((long)a.K * Elem<T>::BYTES + 127) / 128 * (f32 ? each32 : each16) + (f32 ? fixed32 : fixed16));
 }
 
-template <typename T, int MT, int NW, int R>
+template <typename T, int MT, int NW, int R, bool EXPERTS = false>
 int launch_rows(GemmArgs a, bool whole, hipStream_t st) {
-    const long mt = (a.M + 16 * MT - 1) / (16 * MT);
+    const long mt = EXPERTS ? a.M / (16 * MT) + std::min<long>(a.M, a.E + 1) : (a.M + 16 * MT - 1) / (16 * MT);
     a.n_tiles = (int)((a.N + 15l) / 16);
     if (mt * a.n_tiles >= (1l << 32) / (64 * NW)) FR_FAIL(FR_ERR_UNSUPPORTED, "adapter product: more output tiles than a launch takes");
     const int lds = NW * R * (16 + 16 * MT) * 128;
     const dim3 grid((unsigned)(mt * a.n_tiles)), block(64 * NW);
     if (whole) {
-        FR_BIG_LDS_ONCE((gemm_rows_kernel<T, MT, NW, R, true>), lds);
-        hipLaunchKernelGGL((gemm_rows_kernel<T, MT, NW, R, true>), grid, block, lds, st, a);
-    } else hipLaunchKernelGGL((gemm_rows_kernel<T, MT, NW, 1, false>), grid, block, lds / R, st, a);
+        FR_BIG_LDS_ONCE((gemm_rows_kernel<T, MT, NW, R, true, EXPERTS>), lds);
+        hipLaunchKernelGGL((gemm_rows_kernel<T, MT, NW, R, true, EXPERTS>), grid, block, lds, st, a);
+    } else hipLaunchKernelGGL((gemm_rows_kernel<T, MT, NW, 1, false, EXPERTS>), grid, block, lds / R, st, a);
     FR_LAUNCH_CHECK("gemm_rows_kernel");
     return FR_OK;
 }
@@ -769,6 +774,16 @@ int launch_gemm(GemmArgs a, hipStream_t st) {
         if (a.M <= 32 || f32) return launch_rows<T, 2, 8, 3>(a, whole, st);
         return launch_rows<T, 4, 4, 3>(a, whole, st);
     }
+    // experts with few rows each, by the few blocks of one round (fp32: two, its tiles walk K at half the pace), us against
+    // 64-tiles: 7 rows of 13 experts x 384 x 2432, 168 blocks, bf16 6.9 and 11, fp32 8.9 and 45; 512 blocks 10 % slower in bf16,
+    // 10 to 50 % faster in fp32, 1024 half as fast and equal; odd rows, against gemm_any_kernel, 1134 blocks 13 and 42
+    const long some = std::min<long>(a.M, a.E);
+    const bool few = a.order && a.M <= 32 * some;
+    if (few && (rowb >= 1024 || !whole)) {
+        const int rows = a.M <= 8 * some ? 16 : 32;
+        if (tile_count(a, rows, 16) <= (!whole ? 2048 : Elem<T>::BYTES == 4 ? 512 : 256))
+            return rows == 16 ? launch_rows<T, 1, 8, 4, true>(a, whole, st) : launch_rows<T, 2, 8, 3, true>(a, whole, st);
+    }
     // rows of any alignment, us against gemm_any_kernel: 16384 x 2048 x 4097 bf16 455 and 723, 3001 x 2047 x 2049 68 and 90;
     // a 64-tile alone on its CU has its chunks sooner there (300 x 1001 x 1001: 18 and 15, in parts of K 16), but for
     // a long K in parts (554 x 242 x 1461 f32 45 and 22, 156 x 1024 x 7874 f16 73 and 21)
@@ -792,7 +807,6 @@ int launch_gemm(GemmArgs a, hipStream_t st) {
         }
         if (!whole) return c128 <= c64 ? launch_tile<T, 128, 128, 2, 4, 2, false>(a, st) : launch_tile<T, 64, 64, 2, 2, 2, false>(a, st);
         // an expert's few rows are one tile of any height: 5 rows, 2 of 32 experts, 512 -> 2048: 7.0 us by 64-tiles, 10.8 by 128
-        const bool few = a.order && a.M <= 32 * std::min<long>(a.M, a.E);
         if (!few && c256 <= std::min(c128, std::min(c12864, c64))) return launch_tile<T, 256, 256, 2, 4, 2>(a, st);
         if (!few && c12864 <= std::min(c128, c64)) return launch_tile<T, 128, 64, 4, 2, 3>(a, st);
         // a deeper ring for a tile alone on its CU, more tiles at a time for others: 2048 cubed bf16 (128-tiles) 20 us, 26 with

@@ -830,6 +830,24 @@ def test_expert_linear_every_tile(kind, t, e, k, d, n):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("rows, out", [("tokens", "slots"), ("sorted", "sorted")])
+@pytest.mark.parametrize("t, e, k, d, n", [(1, 3, 1, 520, 9), (7, 13, 1, 2432, 40), (9, 70, 2, 1032, 17), (40, 8, 4, 1023, 33), (33, 2, 1, 512, 130), (90, 130, 3, 515, 8),
+                                           (100, 8, 2, 1032, 70), (60, 4, 1, 2051, 24)])
+def test_expert_linear_few_rows(kind, rows, out, t, e, k, d, n):
+    g, dt = gen(t + e + d), TYPES[kind]
+    for lost in (0.0, 0.4, 1.0):
+        r = choose(g, t, e, k, lost)
+        x = randn(g, t if rows == "tokens" else t * k, d, dtype=dt)
+        w, b = randn(g, e, n, d, dtype=dt, scale=d ** -0.5), randn(g, e, n)
+        check_expert(x, w, r, b, act="hsigmoid" if lost else "gelu", rows=rows, out=out, what=(kind, t, e, k, d, n, lost))
+    lies = adapter.Routing(r.weights, r.experts, torch.randint(-5, t * k + 5, (t * k,), generator=g, device="cuda", dtype=torch.int32),
+                           torch.randint(-9, 2 * t * k + 9, (e + 1,), generator=g, device="cuda", dtype=torch.int32))
+    adapter.expert_linear(x, w, lies, b, rows=rows, out=out)
+    torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("e", [62, 63, 64, 65, 127, 128, 200])
 @pytest.mark.parametrize("t, k", [(2, 1), (90, 7), (1500, 3)])
 def test_expert_linear_many_experts(e, t, k):
