@@ -784,7 +784,7 @@ int launch_gemm(GemmArgs a, hipStream_t st) {
         if (tile_count(a, rows, 16) <= (!whole ? 2048 : Elem<T>::BYTES == 4 ? 512 : 256))
             return rows == 16 ? launch_rows<T, 1, 8, 4, true>(a, whole, st) : launch_rows<T, 2, 8, 3, true>(a, whole, st);
     }
-    // rows of any alignment, us against gemm_any_kernel: 16384 x 2048 x 4097 bf16 455 and 723, 3001 x 2047 x 2049 68 and 90;
+    // rows of any alignment, us against gemm_any_kernel: 16384 x 2048 x 4097 bf16 440 and 723, 3001 x 2047 x 2049 58 and 90;
     // a 64-tile alone on its CU has its chunks sooner there (300 x 1001 x 1001: 18 and 15, in parts of K 16), but for
     // a long K in parts (554 x 242 x 1461 f32 45 and 22, 156 x 1024 x 7874 f16 73 and 21)
     const double tiles64 = tile_count(a, 64, 64);
