@@ -367,10 +367,15 @@ __global__ __launch_bounds__(512, 4) void route_choose_kernel(RouteArgs a) {
             }
             const bool keep = g < a.groups && rank < a.top_groups;
             kept = keep ? ~0u : 0u;
-            if (a.top_groups < a.groups) {                   // sums of two: twice the error
-                const float least = -row_max<LPR>(keep ? -sum : -INFINITY), most = row_max<LPR>(!keep && g < a.groups ? sum : -INFINITY);
+            if (a.top_groups < a.groups) {
+                // Where the sum may lie: a key is off by its score's error and its rounding, relative to its own size (the sum of
+                // two large keys of either sign may be small), and both sums and bounds round again: at most 7 (softmax 35) steps
+                // of 2^-24 of the keys' sizes, which slack covers.  A sum beyond f32's range is at least its greatest number.
+                const float err = slack * (fmaxf(1.f, fabsf(g1)) + (per > 1 ? fmaxf(1.f, fabsf(g2)) : 0.f));
+                const float lo = fminf(sum, 0x1.fffffep127f) - err, hi = sum > -INFINITY ? sum + err : -INFINITY;
+                const float least = -row_max<LPR>(keep ? -lo : -INFINITY), most = row_max<LPR>(!keep && g < a.groups ? hi : -INFINITY);
                 // a row without any eligible expert needs no second look
-                doubt = !(least - most > 2.f * slack * fmaxf(1.f, fabsf(least))) && row_max<LPR>(b1) > -INFINITY;
+                doubt = !(least > most) && row_max<LPR>(b1) > -INFINITY;
             }
         }
         constexpr unsigned NUMBER = RT_EMAX - 1;
