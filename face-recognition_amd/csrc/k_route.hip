@@ -71,6 +71,10 @@ FR_DEV float raw_weight(const RouteArgs& a, float l, float top, float m, float z
     return 1.f / (1.f + expf(-l));
 }
 
+// A group's key from its best two: of fewer than two eligible experts -inf, also where the one has a bias of +inf (inf - inf would
+// be a NaN, which no rank counts).
+template <typename T> FR_DEV T group_sum(T best, T second, int per) { return per == 1 ? best : second > -INFINITY ? best + second : (T)-INFINITY; }
+
 FR_DEV double dpp_step(double v, int ctrl) {                // ctrl is a constant at every call
     const unsigned long long u = __builtin_bit_cast(unsigned long long, v);
     unsigned lo, hi;
@@ -166,7 +170,7 @@ FR_DEV void choose_exact(const RouteArgs& a, long row, double* keys, int* chosen
             g2 = fmax(fmin(g1, o1), fmax(g2, o2));
             g1 = fmax(g1, o1);
         }
-        const double sum = per > 1 ? g1 + g2 : g1;           // right in the first lane of each group
+        const double sum = group_sum(g1, g2, per);           // right in the first lane of each group
         int rank = 0;
 #pragma unroll 1
         for (int o = 0; o < a.groups; ++o) {
@@ -359,7 +363,7 @@ __global__ __launch_bounds__(512, 4) void route_choose_kernel(RouteArgs a) {
                 g2 = fmaxf(fminf(g1, o1), fmaxf(g2, o2));
                 g1 = fmaxf(g1, o1);
             }
-            const float sum = per > 1 ? g1 + g2 : g1;
+            const float sum = group_sum(g1, g2, per);
             int rank = 0;
             for (int o = 0; o < a.groups; ++o) {
                 const float v = __shfl(sum, base + o * LG, 64);

@@ -258,9 +258,10 @@ int fr_block_norm(const void* x, int x_type, int slots, const float* slot_weight
 /* Routing of T rows to k of E experts, from logits [T][E] of logits_type.
  * score = softmax over the row (FR_SCORE_SOFTMAX) or sigmoid (FR_SCORE_SIGMOID); key = score + bias[e] (fp32 or NULL; the
  * bias moves the choice, not the weights).  groups > 1: experts in `groups` equal runs, a group's key = the sum of its best
- * two keys (its one key where groups == E), only the best top_groups groups stay.  Then the best k keys, ties to the lower
- * index; keys are ordered as exact scores are (decided in 64 bits where 32 cannot tell them apart).  A logit (or bias) that
- * is -inf or NaN masks its expert; slots that find no expert get expert -1 and weight 0.
+ * two keys (its one key where groups == E; -inf where fewer than two of its experts are eligible), only the best top_groups
+ * groups stay.  Then the best k keys, ties to the lower index; a bias of +inf puts its expert before all others.  Keys are
+ * ordered as exact scores are (decided in 64 bits where 32 cannot tell them apart).  A logit (or bias) that is -inf or NaN
+ * masks its expert; slots that find no expert get expert -1 and weight 0.
  * weights [T][k] fp32: the chosen scores, divided by their sum if renormalise, times scale.  experts [T][k] int32, best first.
  * order [T*k] int32: slot numbers t*k + j sorted by expert, stable; the slots without an expert come last.
  * offsets [E+1] int32: expert e's slots are order[offsets[e] .. offsets[e+1]).

@@ -30,3 +30,29 @@ def test_route_groups_whose_best_two_cancel(score, big, e, groups, top, k):
     # the large keys in some groups only: their error is no reason to doubt the others, and is one where they stand at the cut
     mixed = torch.where(torch.arange(e, device="cuda") < e // 2, bias, randn(g, e, scale=0.1))
     check_route(apart, k, score=score, bias=mixed, groups=groups, top_groups=top, what=("mixed", score, big, e))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("kind", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("e, groups, top, k", [(8, 4, 2, 3), (64, 8, 3, 6), (100, 5, 4, 2)])
+def test_route_bias_of_infinity_in_groups(score, kind, e, groups, top, k):
+    """+inf puts an expert first; alone in its group it leaves the group without a best two, as any other bias does."""
+    g, per = gen(e), e // groups
+    logits = randn(g, 70, e, dtype=kind)
+    bias = randn(g, e, scale=0.1)
+    bias[1], bias[per + 1] = math.inf, math.inf
+    logits[::2, 0], logits[::2, 2:per] = -math.inf, -math.inf  # expert 1 is alone in its group
+    logits[5, per + 1] = math.nan
+    got = adapter.route(logits, k, score=score, bias=bias, groups=groups, top_groups=top)
+    for r in range(70):
+        chosen = {x // per for x in got.experts[r].tolist() if x >= 0}
+        assert len(chosen) <= top
+    finite = bias.clone()
+    finite[1], finite[per + 1] = 2e6, 1e6                      # the same order: scores are at most 1, the lower of two infinities first
+    alone = finite.clone()
+    alone[1] = 0.0                                             # the sum of a lone expert is -inf whatever its bias
+    for rows, b in ((slice(0, None, 2), alone), (slice(1, None, 2), finite)):
+        w, ex, _, _ = oa.route(logits[rows], k, score, b, groups, top)
+        assert torch.equal(got.experts[rows].cpu(), ex), rows
+        assert float((got.weights[rows].cpu().double() - w).abs().max()) < (128 + e) * 2.0 ** -24
