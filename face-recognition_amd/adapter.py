@@ -19,6 +19,7 @@ their tensors' device, allocate with torch's caching allocator, synchronise noth
 """
 from __future__ import annotations
 
+import functools
 from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
@@ -26,15 +27,17 @@ import torch
 from . import ops as _ops
 
 
-_EAGER = {"linear": _ops._linear, "block_norm": _ops._block_norm_eager, "route": _ops._route, "expert_linear": _ops._expert_linear}
+_DIRECT = {name: functools.partial(impl, direct=True) for name, impl in
+           (("linear", _ops._linear), ("block_norm", _ops._block_norm_eager), ("route", _ops._route), ("expert_linear", _ops._expert_linear))}
 
 
 def _op(name: str, x: torch.Tensor):
-    """The operator for a call on ``x``: its implementation itself for an eager call on a plain tensor (the dispatcher takes
-    as long as the smallest kernels run), ``torch.ops.fr_hip`` for whatever traces or stands in for one."""
+    """The operator for a call on ``x``: its implementation itself for an eager call on plain tensors (the dispatcher takes
+    as long as the smallest kernels run), ``torch.ops.fr_hip`` for whatever traces or stands in for one.  The first look is at
+    ``x``; what the other arguments hold is seen by the implementation, which turns to ``torch.ops.fr_hip`` too."""
     kind = type(x)
     if (kind is torch.Tensor or kind is torch.nn.Parameter) and not torch.compiler.is_compiling():
-        return _EAGER[name]
+        return _DIRECT[name]
     return getattr(torch.ops.fr_hip, name)
 
 

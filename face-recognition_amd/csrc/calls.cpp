@@ -1,7 +1,8 @@
 // Host side of the adapter operators' usual calls: contiguous tensors of the current device.  On a few rows the GPU is done in
 // 3 to 6 us, and checking the arguments in Python and handing them over through ctypes took 9 (route: 12); here it is 4.6 (7.1).
 // Each function checks what its Python counterpart in ops.py checks and answers None where anything is not as usual (a view,
-// another device, a gradient, a bad argument): the counterpart then takes the call, or says what is wrong with it.  There is
+// another device, a gradient, a bad argument): the counterpart then takes the call, or says what is wrong with it.  Where the
+// dispatcher has more to do than to find the GPU's kernel it answers NotImplemented, before it looks at anything else.  There is
 // no kernel here: the entries of include/fr_hip.h are bound by address.
 #include <Python.h>
 
@@ -11,6 +12,7 @@
 #include <ATen/core/Tensor.h>
 #include <ATen/core/grad_mode.h>
 #include <ATen/ops/empty.h>
+#include <c10/core/DispatchKeySet.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -40,6 +42,19 @@ int type_of(at::ScalarType t) {
     }
 }
 
+// Whether a tensor is more than memory on one device: a subclass, a negative bit, a batch of a transform, a zero without memory.  Its
+// key set says so; the keys a plain one has are those of its backend, of autograd (which refuses or does nothing) and of autocast
+// (which has no rule for these operators).
+bool interposed(PyObject* const* args, Py_ssize_t count) {
+    static const uint64_t plain = c10::full_backend_mask | c10::DispatchKeySet(c10::DispatchKey::Dense).raw_repr() |
+                                  c10::autograd_dispatch_keyset_with_ADInplaceOrView.raw_repr() | c10::autocast_dispatch_keyset.raw_repr();
+    for (Py_ssize_t i = 0; i < count; ++i) {
+        if (!THPVariable_Check(args[i])) continue;
+        if (!THPVariable_CheckExact(args[i]) || (THPVariable_Unpack(args[i]).key_set().raw_repr() & ~plain)) return true;
+    }
+    return false;
+}
+
 // The arguments of a call.  `usual` turns false at the first that is not.
 struct Call {
     PyObject* const* args;
@@ -51,7 +66,7 @@ struct Call {
         if (args[i] == Py_None) return nullptr;
         if (!THPVariable_CheckExact(args[i])) { usual = false; return nullptr; }
         const at::Tensor& t = THPVariable_Unpack(args[i]);
-        if (!t.defined() || !t.is_cuda() || t.layout() != at::kStrided || !t.has_storage() || t.get_device() != device || !t.is_contiguous() || t.is_neg() ||
+        if (!t.defined() || !t.is_cuda() || t.layout() != at::kStrided || !t.has_storage() || t.get_device() != device || !t.is_contiguous() ||
             (t.requires_grad() && at::GradMode::is_enabled())) {
             usual = false;
             return nullptr;
@@ -109,11 +124,13 @@ PyObject* failed(const char* name, int rc) {
 
 #define USUAL(ok) do { if (!(ok)) Py_RETURN_NONE; } while (0)
 #define ARGUMENTS(n) do { if (count != (n)) return PyErr_Format(PyExc_TypeError, "%d arguments expected", n); } while (0)
+#define DIRECT() do { if (interposed(args, count)) Py_RETURN_NOTIMPLEMENTED; } while (0)
 
 // linear(x, weight, bias, slope, residual, act, out_dtype, device, stream)
 PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t count) {
     HANDLE_TH_ERRORS
     ARGUMENTS(9);
+    DIRECT();
     Call c{args, (int)PyLong_AsLong(args[7])};
     void* stream = PyLong_AsVoidPtr(args[8]);
     const at::Tensor *x = c.needed(0), *w = c.needed(1), *bias = c.tensor(2), *slope = c.tensor(3), *res = c.tensor(4);
@@ -152,6 +169,7 @@ PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t count) {
 PyObject* block_norm(PyObject*, PyObject* const* args, Py_ssize_t count) {
     HANDLE_TH_ERRORS
     ARGUMENTS(18);
+    DIRECT();
     Call c{args, (int)PyLong_AsLong(args[16])};
     void* stream = PyLong_AsVoidPtr(args[17]);
     const at::Tensor *x = c.needed(0), *res = c.tensor(1), *slots = c.tensor(2), *w = c.tensor(4), *b = c.tensor(5), *gate = c.tensor(7),
@@ -212,6 +230,7 @@ PyObject* block_norm(PyObject*, PyObject* const* args, Py_ssize_t count) {
 PyObject* route(PyObject*, PyObject* const* args, Py_ssize_t count) {
     HANDLE_TH_ERRORS
     ARGUMENTS(10);
+    DIRECT();
     Call c{args, (int)PyLong_AsLong(args[8])};
     void* stream = PyLong_AsVoidPtr(args[9]);
     const at::Tensor *logits = c.needed(0), *bias = c.tensor(3);
@@ -250,6 +269,7 @@ PyObject* route(PyObject*, PyObject* const* args, Py_ssize_t count) {
 PyObject* expert_linear(PyObject*, PyObject* const* args, Py_ssize_t count) {
     HANDLE_TH_ERRORS
     ARGUMENTS(13);
+    DIRECT();
     Call c{args, (int)PyLong_AsLong(args[11])};
     void* stream = PyLong_AsVoidPtr(args[12]);
     const at::Tensor *x = c.needed(0), *w = c.needed(1), *order = c.needed(2), *offsets = c.needed(3), *bias = c.tensor(5), *slope = c.tensor(7);

@@ -298,13 +298,17 @@ def _linear_shape(op, x, weight, residual):
 
 
 # Each of the four first offers its call to csrc/calls.cpp, which takes the usual ones (plain contiguous tensors on the current
-# device) with a third of the host's time; the rest, and every wrong one, is dealt with here.
-def _linear(x, weight, bias, slope, residual, act, out_dtype):
+# device) with a third of the host's time; the rest, and every wrong one, is dealt with here.  ``direct``: the call has not been
+# through the dispatcher; where that has something to do (csrc/calls.cpp says NotImplemented) the call is made through it.
+def _linear(x, weight, bias, slope, residual, act, out_dtype, direct=False):
     op = "linear"
     if x.is_cuda:
         index = _current_device()
         y = _lib.calls().linear(x, weight, bias, slope, residual, _ACTS.get(act, -1), out_dtype, index, _current_stream(index))
-        if y is not None:
+        if y is NotImplemented:
+            if direct:
+                return torch.ops.fr_hip.linear(x, weight, bias, slope, residual, act, out_dtype)
+        elif y is not None:
             return y
     dev = _check_tensors(op, x, weight, bias, slope, residual)
     shape = _linear_shape(op, x, weight, residual)
@@ -372,15 +376,19 @@ def _affine(op, what, norm, weight, bias, d):
 
 
 def _block_norm_eager(x, residual, slot_weights, norm, weight, bias, eps, gate, gate_act, scale, next_norm, next_weight, next_bias,
-                      next_eps, out_dtype, next_dtype):
-    """(out, next), None for a next that is not asked for."""
+                      next_eps, out_dtype, next_dtype, direct=False):
+    """(out, next), None (through the dispatcher: a tensor without elements) for a next that is not asked for."""
     op = "block_norm"
     if x.is_cuda:
         index = _current_device()
         both = _lib.calls().block_norm(x, residual, slot_weights, _NORMS.get(norm, -1), weight, bias, eps, gate, _GATE_ACTS.get(gate_act, -1),
                                        scale, _NORMS.get(next_norm, -1), next_weight, next_bias, next_eps, out_dtype, next_dtype,
                                        index, _current_stream(index))
-        if both is not None:
+        if both is NotImplemented:
+            if direct:
+                return torch.ops.fr_hip.block_norm(x, residual, slot_weights, norm, weight, bias, eps, gate, gate_act, scale, next_norm,
+                                                   next_weight, next_bias, next_eps, out_dtype, next_dtype)
+        elif both is not None:
             return both
     dev = _check_tensors(op, x, residual, slot_weights, weight, bias, gate, next_weight, next_bias)
     shape = _block_norm_shape(op, x, slot_weights)
@@ -446,12 +454,15 @@ def _route_empty(logits, k):
             logits.new_empty(E + 1, dtype=i32))
 
 
-def _route(logits, k, score, bias, groups, top_groups, renormalise, scale):
+def _route(logits, k, score, bias, groups, top_groups, renormalise, scale, direct=False):
     op = "route"
     if logits.is_cuda:
         index = _current_device()
         out = _lib.calls().route(logits, k, _SCORES.get(score, -1), bias, groups, top_groups, renormalise, scale, index, _current_stream(index))
-        if out is not None:
+        if out is NotImplemented:
+            if direct:
+                return torch.ops.fr_hip.route(logits, k, score, bias, groups, top_groups, renormalise, scale)
+        elif out is not None:
             return out
     dev = _check_tensors(op, logits, bias)
     T, E = _route_shape(op, logits, k)
@@ -486,13 +497,16 @@ def _expert_shape(op, x, weight, order, offsets, k, rows, out):
     return T, (T * k, weight.shape[1]) if out == "sorted" else (T, k, weight.shape[1])
 
 
-def _expert_linear(x, weight, order, offsets, k, bias, act, slope, rows, out, out_dtype):
+def _expert_linear(x, weight, order, offsets, k, bias, act, slope, rows, out, out_dtype, direct=False):
     op = "expert_linear"
     if x.is_cuda:
         index = _current_device()
         y = _lib.calls().expert_linear(x, weight, order, offsets, k, bias, _ACTS.get(act, -1), slope, _ROWS.get(rows, -1), _OUTS.get(out, -1),
                                        out_dtype, index, _current_stream(index))
-        if y is not None:
+        if y is NotImplemented:
+            if direct:
+                return torch.ops.fr_hip.expert_linear(x, weight, order, offsets, k, bias, act, slope, rows, out, out_dtype)
+        elif y is not None:
             return y
     dev = _check_tensors(op, x, weight, order, offsets, bias, slope)
     T, shape = _expert_shape(op, x, weight, order, offsets, k, rows, out)
