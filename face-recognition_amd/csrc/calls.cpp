@@ -8,11 +8,13 @@
 
 #include <string.h>
 
+#include <ATen/PythonTorchFunctionTLS.h>
 #include <ATen/core/LegacyTypeDispatch.h>
 #include <ATen/core/Tensor.h>
 #include <ATen/core/grad_mode.h>
 #include <ATen/ops/empty.h>
 #include <c10/core/DispatchKeySet.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -42,12 +44,15 @@ int type_of(at::ScalarType t) {
     }
 }
 
-// Whether a tensor is more than memory on one device: a subclass, a negative bit, a batch of a transform, a zero without memory.  Its
-// key set says so; the keys a plain one has are those of its backend, of autograd (which refuses or does nothing) and of autocast
-// (which has no rule for these operators).
+// Whether a tensor is more than memory on one device (a subclass, a negative bit, a batch of a transform, a zero without memory), or
+// the thread is in a tracer, a mode or a transform that has to see the operator.  The key sets of both say so; the keys of a plain
+// call are those of a backend, of autograd (which refuses or does nothing) and of autocast (which has no rule for these operators).
 bool interposed(PyObject* const* args, Py_ssize_t count) {
     static const uint64_t plain = c10::full_backend_mask | c10::DispatchKeySet(c10::DispatchKey::Dense).raw_repr() |
-                                  c10::autograd_dispatch_keyset_with_ADInplaceOrView.raw_repr() | c10::autocast_dispatch_keyset.raw_repr();
+                                  c10::autograd_dispatch_keyset_with_ADInplaceOrView.raw_repr() | c10::autocast_dispatch_keyset.raw_repr() |
+                                  c10::DispatchKeySet(c10::DispatchKey::BackendSelect).raw_repr();
+    const c10::impl::LocalDispatchKeySet thread = c10::impl::tls_local_dispatch_key_set();
+    if ((thread.included_.raw_repr() & ~thread.excluded_.raw_repr() & ~plain) || at::impl::torch_function_mode_enabled()) return true;
     for (Py_ssize_t i = 0; i < count; ++i) {
         if (!THPVariable_Check(args[i])) continue;
         if (!THPVariable_CheckExact(args[i]) || (THPVariable_Unpack(args[i]).key_set().raw_repr() & ~plain)) return true;

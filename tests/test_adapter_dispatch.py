@@ -122,3 +122,114 @@ def test_subclass_in_any_place(name):
         got = function(name, replaced(args, i, args[i].as_subclass(Seen)))
         assert any("fr_hip" in f and name in f for f in Seen.met), (name, i, Seen.met)
         same(tuple(t.as_subclass(torch.Tensor) for t in flat(got)), want, (name, i))
+
+
+# ---- threads in a tracer, a mode or a transform ------------------------------------------------------------------------
+
+class Counting(torch.utils._python_dispatch.TorchDispatchMode):
+    def __init__(self):
+        super().__init__()
+        self.met = []
+
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        self.met.append(str(func))
+        return func(*args, **(kwargs or {}))
+
+
+class CountingFunctions(torch.overrides.TorchFunctionMode):
+    def __init__(self):
+        super().__init__()
+        self.met = []
+
+    def __torch_function__(self, func, types, args=(), kwargs=None):
+        self.met.append(str(func))
+        return func(*args, **(kwargs or {}))
+
+
+def traced(name, args, run):
+    """``run`` on ``name`` as a function of its first argument, as make_fx and jit.trace take it."""
+    return lambda x: run(name, (x,) + args[1:])
+
+
+@pytest.mark.parametrize("name", OPS)
+def test_short_way_leaves_such_threads_to_the_dispatcher(name):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    args = arguments("cpu")[name]
+    said = []
+
+    def ask(x):
+        said.append(short(name, (x,) + args[1:]))
+        return x + 1
+
+    ask(args[0])
+    with torch.no_grad(), torch.autocast("cpu"):
+        ask(args[0])
+    with torch.inference_mode():
+        ask(args[0])
+    assert said == [None] * 3
+    said.clear()
+    for run in (lambda: make_fx(ask)(args[0]), lambda: torch.jit.trace(ask, args[0], check_trace=False), lambda: torch.func.vmap(ask)(args[0][None]),
+                lambda: torch.func.jvp(ask, (args[0],), (args[0],)), lambda: torch.func.grad(lambda x: ask(x).sum())(args[0])):
+        run()
+        assert said and all(a is NotImplemented for a in said), said
+        said.clear()
+    for mode in (Counting(), CountingFunctions()):
+        with mode:
+            ask(args[0])
+        assert said.pop() is NotImplemented
+    ask(args[0])
+    assert said == [None]                                      # and nothing of it stays behind
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", OPS)
+def test_tracers_record_the_operator(name):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    args, other = arguments("cuda")[name], arguments("cuda", 2)[name]
+    graph = make_fx(traced(name, args, function))(args[0])
+    assert any(f"fr_hip.{name}" in str(n.target) for n in graph.graph.nodes), graph.code
+    want = function(name, (other[0],) + args[1:])
+    same(graph(other[0]), want, name)
+    for kind in ("fake", "symbolic"):
+        graph = make_fx(traced(name, args, function), tracing_mode=kind, _allow_non_fake_inputs=True)(args[0])
+        assert any(f"fr_hip.{name}" in str(n.target) for n in graph.graph.nodes), graph.code
+        same(graph(other[0]), want, (name, kind))
+    script = torch.jit.trace(traced(name, args, function), args[0])
+    assert f"fr_hip::{name}" in str(script.graph)
+    same(script(other[0]), want, name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", OPS)
+def test_modes_see_the_operator(name):
+    args = arguments("cuda")[name]
+    want = function(name, args)
+    for mode in (Counting(), CountingFunctions()):
+        with mode:
+            got = function(name, args)
+        assert any("fr_hip" in f and name in f for f in mode.met), mode.met
+        same(got, want, name)
+
+
+@pytest.mark.gpu
+def test_maps_over_a_batch():
+    x, w = randn(gen(3), 5, 6, 16), randn(gen(4), 12, 16)
+    assert torch.equal(torch.func.vmap(lambda r: adapter.linear(r, w))(x), torch.stack([adapter.linear(r, w) for r in x]))
+    assert torch.equal(torch.func.vmap(adapter.block_norm)(x), torch.stack([adapter.block_norm(r) for r in x]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", OPS)
+def test_compiled_programs_hold_the_operator(name):
+    args, other = arguments("cuda")[name], arguments("cuda", 2)[name]
+    graphs = []
+
+    def backend(graph, inputs):
+        graphs.append(graph)
+        return graph.forward
+
+    torch._dynamo.reset()
+    compiled = torch.compile(traced(name, args, function), backend=backend, fullgraph=True)
+    same(compiled(other[0]), function(name, (other[0],) + args[1:]), name)
+    assert any(f"fr_hip.{name}" in str(n.target) for n in graphs[0].graph.nodes), graphs[0].code
+    torch._dynamo.reset()
