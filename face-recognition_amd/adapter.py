@@ -19,7 +19,6 @@ their tensors' device, allocate with torch's caching allocator, synchronise noth
 """
 from __future__ import annotations
 
-import functools
 from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
@@ -27,8 +26,7 @@ import torch
 from . import ops as _ops
 
 
-_DIRECT = {name: functools.partial(impl, direct=True) for name, impl in
-           (("linear", _ops._linear), ("block_norm", _ops._block_norm_eager), ("route", _ops._route), ("expert_linear", _ops._expert_linear))}
+_DIRECT = {"linear": _ops._linear, "block_norm": _ops._block_norm_eager, "route": _ops._route, "expert_linear": _ops._expert_linear}
 
 
 def _op(name: str, x: torch.Tensor):

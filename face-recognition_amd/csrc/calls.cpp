@@ -72,7 +72,7 @@ struct Call {
         if (!THPVariable_CheckExact(args[i])) { usual = false; return nullptr; }
         const at::Tensor& t = THPVariable_Unpack(args[i]);
         if (!t.defined() || !t.is_cuda() || t.layout() != at::kStrided || !t.has_storage() || t.get_device() != device || !t.is_contiguous() ||
-            (t.requires_grad() && at::GradMode::is_enabled())) {
+            (t.requires_grad() && at::GradMode::is_enabled()) || t._fw_grad(0).defined()) {
             usual = false;
             return nullptr;
         }

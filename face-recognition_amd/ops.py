@@ -22,6 +22,7 @@ import functools
 from typing import Dict, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -43,6 +44,7 @@ _defs.define("expert_linear(Tensor x, Tensor weight, Tensor order, Tensor offset
              "str rows, str out, ScalarType? out_dtype) -> Tensor")
 _impl = torch.library.Library(_NS, "IMPL", "CUDA")
 _meta = torch.library.Library(_NS, "IMPL", "Meta")
+_autograd = torch.library.Library(_NS, "IMPL", "Autograd")
 
 # (plan handle | 0 for search, device index, stream handle) -> scratch.  Keyed by STREAM as well: two calls enqueued
 # on different streams can overlap on the GPU, and a workspace shared between them (the same model on two streams,
@@ -214,18 +216,21 @@ def _type(op, what, dtype):
     return code
 
 
-def _check_tensors(op, first, *others):
-    """One device, and no gradient asked for: the kernels have no backward pass, and a result that silently cuts the graph
-    would be a wrong one."""
-    dev, index = first.device, first.get_device()
-    grad = first.requires_grad
-    for t in others:
-        if t is not None:
-            if t.get_device() != index or (index < 0 and t.device != dev):
-                _fail(op, f"all tensors on {dev}: got one on {t.device}")
-            grad = grad or t.requires_grad
-    if grad and torch.is_grad_enabled():
+def _no_gradient(op, *tensors):
+    """The kernels have no backward pass and carry no tangents, and a result that silently cuts the graph would be a wrong one."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         _fail(op, "inference only: call it under torch.no_grad() or on detached tensors")
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        _fail(op, "inference only: a tensor has a forward-mode tangent")
+
+
+def _check_tensors(op, first, *others):
+    """One device, and no gradient asked for."""
+    dev, index = first.device, first.get_device()
+    for t in others:
+        if t is not None and (t.get_device() != index or (index < 0 and t.device != dev)):
+            _fail(op, f"all tensors on {dev}: got one on {t.device}")
+    _no_gradient(op, first, *others)
     return dev
 
 
@@ -298,18 +303,23 @@ def _linear_shape(op, x, weight, residual):
 
 
 # Each of the four first offers its call to csrc/calls.cpp, which takes the usual ones (plain contiguous tensors on the current
-# device) with a third of the host's time; the rest, and every wrong one, is dealt with here.  ``direct``: the call has not been
-# through the dispatcher; where that has something to do (csrc/calls.cpp says NotImplemented) the call is made through it.
-def _linear(x, weight, bias, slope, residual, act, out_dtype, direct=False):
+# device) with a third of the host's time; the rest, and every wrong one, is dealt with here.  ``way`` says where the call comes from.
+# _DIRECT: not through the dispatcher; where that has something to do (csrc/calls.cpp says NotImplemented) it goes there.
+# _ABOVE: the dispatcher, before autograd; no answer (None) unless the short way has one.  _BELOW: the dispatcher, as the kernel.
+_DIRECT, _ABOVE, _BELOW = 0, 1, 2
+
+
+def _linear(x, weight, bias, slope, residual, act, out_dtype, way=_DIRECT):
     op = "linear"
     if x.is_cuda:
         index = _current_device()
         y = _lib.calls().linear(x, weight, bias, slope, residual, _ACTS.get(act, -1), out_dtype, index, _current_stream(index))
-        if y is NotImplemented:
-            if direct:
-                return torch.ops.fr_hip.linear(x, weight, bias, slope, residual, act, out_dtype)
-        elif y is not None:
+        if y is not None and y is not NotImplemented:
             return y
+        if y is NotImplemented and way == _DIRECT:
+            return torch.ops.fr_hip.linear(x, weight, bias, slope, residual, act, out_dtype)
+    if way == _ABOVE:
+        return None
     dev = _check_tensors(op, x, weight, bias, slope, residual)
     shape = _linear_shape(op, x, weight, residual)
     N, K = weight.shape
@@ -376,7 +386,7 @@ def _affine(op, what, norm, weight, bias, d):
 
 
 def _block_norm_eager(x, residual, slot_weights, norm, weight, bias, eps, gate, gate_act, scale, next_norm, next_weight, next_bias,
-                      next_eps, out_dtype, next_dtype, direct=False):
+                      next_eps, out_dtype, next_dtype, way=_DIRECT):
     """(out, next), None (through the dispatcher: a tensor without elements) for a next that is not asked for."""
     op = "block_norm"
     if x.is_cuda:
@@ -384,12 +394,13 @@ def _block_norm_eager(x, residual, slot_weights, norm, weight, bias, eps, gate, 
         both = _lib.calls().block_norm(x, residual, slot_weights, _NORMS.get(norm, -1), weight, bias, eps, gate, _GATE_ACTS.get(gate_act, -1),
                                        scale, _NORMS.get(next_norm, -1), next_weight, next_bias, next_eps, out_dtype, next_dtype,
                                        index, _current_stream(index))
-        if both is NotImplemented:
-            if direct:
-                return torch.ops.fr_hip.block_norm(x, residual, slot_weights, norm, weight, bias, eps, gate, gate_act, scale, next_norm,
-                                                   next_weight, next_bias, next_eps, out_dtype, next_dtype)
-        elif both is not None:
+        if both is not None and both is not NotImplemented:
             return both
+        if both is NotImplemented and way == _DIRECT:
+            return torch.ops.fr_hip.block_norm(x, residual, slot_weights, norm, weight, bias, eps, gate, gate_act, scale, next_norm,
+                                               next_weight, next_bias, next_eps, out_dtype, next_dtype)
+    if way == _ABOVE:
+        return None
     dev = _check_tensors(op, x, residual, slot_weights, weight, bias, gate, next_weight, next_bias)
     shape = _block_norm_shape(op, x, slot_weights)
     d = x.shape[-1]
@@ -430,9 +441,12 @@ def _block_norm_eager(x, residual, slot_weights, norm, weight, bias, eps, gate, 
 
 
 def _block_norm(x, residual, slot_weights, norm, weight, bias, eps, gate, gate_act, scale, next_norm, next_weight, next_bias,
-                next_eps, out_dtype, next_dtype):
-    out, nxt = _block_norm_eager(x, residual, slot_weights, norm, weight, bias, eps, gate, gate_act, scale, next_norm, next_weight,
-                                 next_bias, next_eps, out_dtype, next_dtype)
+                next_eps, out_dtype, next_dtype, way=_DIRECT):
+    both = _block_norm_eager(x, residual, slot_weights, norm, weight, bias, eps, gate, gate_act, scale, next_norm, next_weight,
+                             next_bias, next_eps, out_dtype, next_dtype, way)
+    if both is None:
+        return None
+    out, nxt = both
     return out, x.new_empty(0, dtype=next_dtype or out.dtype) if nxt is None else nxt      # the op's schema has two results
 
 
@@ -454,16 +468,17 @@ def _route_empty(logits, k):
             logits.new_empty(E + 1, dtype=i32))
 
 
-def _route(logits, k, score, bias, groups, top_groups, renormalise, scale, direct=False):
+def _route(logits, k, score, bias, groups, top_groups, renormalise, scale, way=_DIRECT):
     op = "route"
     if logits.is_cuda:
         index = _current_device()
         out = _lib.calls().route(logits, k, _SCORES.get(score, -1), bias, groups, top_groups, renormalise, scale, index, _current_stream(index))
-        if out is NotImplemented:
-            if direct:
-                return torch.ops.fr_hip.route(logits, k, score, bias, groups, top_groups, renormalise, scale)
-        elif out is not None:
+        if out is not None and out is not NotImplemented:
             return out
+        if out is NotImplemented and way == _DIRECT:
+            return torch.ops.fr_hip.route(logits, k, score, bias, groups, top_groups, renormalise, scale)
+    if way == _ABOVE:
+        return None
     dev = _check_tensors(op, logits, bias)
     T, E = _route_shape(op, logits, k)
     if not 1 <= groups <= 64 or not 1 <= top_groups <= groups:
@@ -497,17 +512,18 @@ def _expert_shape(op, x, weight, order, offsets, k, rows, out):
     return T, (T * k, weight.shape[1]) if out == "sorted" else (T, k, weight.shape[1])
 
 
-def _expert_linear(x, weight, order, offsets, k, bias, act, slope, rows, out, out_dtype, direct=False):
+def _expert_linear(x, weight, order, offsets, k, bias, act, slope, rows, out, out_dtype, way=_DIRECT):
     op = "expert_linear"
     if x.is_cuda:
         index = _current_device()
         y = _lib.calls().expert_linear(x, weight, order, offsets, k, bias, _ACTS.get(act, -1), slope, _ROWS.get(rows, -1), _OUTS.get(out, -1),
                                        out_dtype, index, _current_stream(index))
-        if y is NotImplemented:
-            if direct:
-                return torch.ops.fr_hip.expert_linear(x, weight, order, offsets, k, bias, act, slope, rows, out, out_dtype)
-        elif y is not None:
+        if y is not None and y is not NotImplemented:
             return y
+        if y is NotImplemented and way == _DIRECT:
+            return torch.ops.fr_hip.expert_linear(x, weight, order, offsets, k, bias, act, slope, rows, out, out_dtype)
+    if way == _ABOVE:
+        return None
     dev = _check_tensors(op, x, weight, order, offsets, bias, slope)
     T, shape = _expert_shape(op, x, weight, order, offsets, k, rows, out)
     E, N, K = weight.shape
@@ -543,10 +559,28 @@ _impl.impl("cosine_pairs", _cosine_pairs)
 _impl.impl("l2norm_bf16", _l2norm_bf16)
 _impl.impl("topk_search", _topk_search)
 _impl.impl("topk_merge", _topk_merge)
-_impl.impl("linear", _linear)
-_impl.impl("block_norm", _block_norm)
-_impl.impl("route", _route)
-_impl.impl("expert_linear", _expert_linear)
+
+
+def _register(name, impl):
+    """The kernel, and above it, for the calls that the short way does not take, the refusal of gradients: it has to stand where
+    the dispatcher still sees them, as below autograd a transform's tensors (torch.func.grad, jvp) have neither gradient nor tangent."""
+    op = getattr(torch.ops.fr_hip, name).default
+
+    def above(keys, *args):
+        if type(args[0]) is torch.Tensor:                     # nothing that only stands in for one
+            out = impl(*args, _ABOVE)
+            if out is not None:
+                return out
+        _no_gradient(name, *(a for a in args if isinstance(a, torch.Tensor)))
+        with torch._C._AutoDispatchBelowAutograd():
+            return op.redispatch(keys & torch._C._after_autograd_keyset, *args)
+
+    _autograd.impl(name, above, with_keyset=True)
+    _impl.impl(name, lambda *args: impl(*args, _BELOW))
+
+
+for _name_impl in (("linear", _linear), ("block_norm", _block_norm), ("route", _route), ("expert_linear", _expert_linear)):
+    _register(*_name_impl)
 
 # shape functions (tracing / torch.export)
 _meta.impl("embed", lambda x, plan, c, h, w: x.new_empty(_out_shape(x.shape[0], c, h, w), dtype=torch.float32))

@@ -233,3 +233,70 @@ def test_compiled_programs_hold_the_operator(name):
     same(compiled(other[0]), function(name, (other[0],) + args[1:]), name)
     assert any(f"fr_hip.{name}" in str(n.target) for n in graphs[0].graph.nodes), graphs[0].code
     torch._dynamo.reset()
+
+
+# ---- gradients ---------------------------------------------------------------------------------------------------------
+
+def refused(call, words):
+    with pytest.raises(RuntimeError, match="inference only") as e:
+        call()
+    assert words in str(e.value)
+
+
+def refuses_gradients(name, args, call):
+    """``call(args)`` says no to a gradient or a tangent of any of its tensors, by whatever way it is asked for."""
+    from torch.autograd import forward_ad
+    for i in tensors(args):
+        t = args[i]
+        if not t.is_floating_point():
+            continue
+        one = lambda v, i=i: call(replaced(args, i, v))
+        refused(lambda: one(t.clone().requires_grad_()), "no_grad")
+        with torch.no_grad():
+            assert not any(y.requires_grad for y in flat(one(t.clone().requires_grad_())))
+        with forward_ad.dual_level():
+            refused(lambda: one(forward_ad.make_dual(t, torch.ones_like(t))), "tangent")
+            with torch.no_grad():                              # which does not turn these off
+                refused(lambda: one(forward_ad.make_dual(t, torch.ones_like(t))), "tangent")
+            one(t)                                             # another's level is no reason
+        refused(lambda: torch.func.jvp(one, (t,), (torch.ones_like(t),)), "tangent")
+        refused(lambda: torch.func.vjp(one, t), "no_grad")
+        refused(lambda: torch.func.grad(lambda v: flat(one(v))[0].sum())(t), "no_grad")
+
+
+@pytest.mark.parametrize("name", OPS)
+def test_dispatched_gradients_are_refused(name):
+    """Through the dispatcher, on tensors without data."""
+    args = tuple(a.to("meta") if isinstance(a, torch.Tensor) else a for a in arguments("cpu")[name])
+    refuses_gradients(name, args, lambda a: getattr(torch.ops.fr_hip, name)(*a))
+
+
+@pytest.mark.parametrize("name", OPS)
+def test_direct_tangents_are_refused(name):
+    from torch.autograd import forward_ad
+    args = arguments("cpu")[name]
+    impl = {"linear": ops._linear, "block_norm": ops._block_norm, "route": ops._route, "expert_linear": ops._expert_linear}[name]
+    with forward_ad.dual_level():
+        for i in tensors(args):
+            if args[i].is_floating_point():
+                refused(lambda: impl(*replaced(args, i, forward_ad.make_dual(args[i], args[i]))), "tangent")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", OPS)
+def test_gradients_and_tangents_are_refused_on_the_gpu(name):
+    args = arguments("cuda")[name]
+    refuses_gradients(name, args, lambda a: function(name, a))
+    refuses_gradients(name, args, lambda a: getattr(torch.ops.fr_hip, name)(*a))
+
+
+@pytest.mark.parametrize("name", OPS)
+def test_fake_tensors_need_no_gpu(name):
+    """Shapes of GPU tensors that only stand in for some, through the functions and the dispatched operators."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    real = arguments("cpu")[name]
+    with FakeTensorMode():
+        args = tuple(torch.empty(a.shape, dtype=a.dtype, device="cuda") if isinstance(a, torch.Tensor) else a for a in real)
+        for got in (function(name, args), getattr(torch.ops.fr_hip, name)(*args)):
+            assert all(y.is_cuda for y in flat(got))
+        refused(lambda: getattr(torch.ops.fr_hip, name)(*replaced(args, 0, args[0].requires_grad_())), "no_grad")
