@@ -282,15 +282,20 @@ def _rows(t, width):
     return t.contiguous(), width
 
 
-def _vector(op, what, t, n, dtypes):
-    if t is None:
-        return None
-    if t.shape != (n,) or t.dtype not in dtypes:
-        _fail(op, f"{what} is [{n}] of {' or '.join(str(d)[6:] for d in dtypes)}: got {t.dtype} {tuple(t.shape)}")
-    return t.contiguous()
+def _check_of(op, what, t, shape, *dtypes):
+    if t is not None and (t.shape != shape or t.dtype not in dtypes):
+        _fail(op, f"{what} is {list(shape)} of {' or '.join(str(d)[6:] for d in dtypes)}: got {t.dtype} {tuple(t.shape)}")
 
 
-def _linear_shape(op, x, weight, residual):
+def _whole(t):
+    return None if t is None else t.contiguous()
+
+
+# The checks of an operator's arguments, of tensors with and without data alike.
+def _check_linear(x, weight, bias, slope, residual, act, out_dtype):
+    """(device, shape of the result, codes of x's type, of out_dtype and of act)."""
+    op = "linear"
+    dev = _check_tensors(op, x, weight, bias, slope, residual)
     xs, ws = x.shape, weight.shape
     if len(xs) < 1 or len(ws) != 2 or xs[-1] != ws[1] or ws[1] < 1 or ws[0] < 1:
         _fail(op, f"expected x [..., K] and weight [N, K]: got {tuple(xs)} and {tuple(ws)}")
@@ -299,7 +304,23 @@ def _linear_shape(op, x, weight, residual):
     shape = xs[:-1] + ws[:1]
     if residual is not None and residual.shape != shape:
         _fail(op, f"residual is {tuple(shape)}: got {tuple(residual.shape)}")
-    return shape
+    kind, code = _check_product(op, x, weight, bias, slope, ws[:1], act)
+    if residual is not None:
+        _type(op, "residual", residual.dtype)
+    return dev, shape, kind, kind if out_dtype is None else _type(op, "out_dtype", out_dtype), code
+
+
+def _check_product(op, x, weight, bias, slope, shape, act):
+    """What the two products have in common: (code of x's type, of act)."""
+    kind = _type(op, "x", x.dtype)
+    if weight.dtype != x.dtype:
+        _fail(op, f"x and weight have one type: got {x.dtype} and {weight.dtype}")
+    code = _name(op, _ACTS, act, "act")
+    if (slope is not None) != (code == _lib.FR_ACT_PRELU):
+        _fail(op, "slope belongs to act='prelu', and only to it")
+    _check_of(op, "bias", bias, shape, x.dtype, torch.float32)
+    _check_of(op, "slope", slope, shape, torch.float32)
+    return kind, code
 
 
 # Each of the four first offers its call to csrc/calls.cpp, which takes the usual ones (plain contiguous tensors on the current
@@ -310,7 +331,6 @@ _DIRECT, _ABOVE, _BELOW = 0, 1, 2
 
 
 def _linear(x, weight, bias, slope, residual, act, out_dtype, way=_DIRECT):
-    op = "linear"
     if x.is_cuda:
         index = _current_device()
         y = _lib.calls().linear(x, weight, bias, slope, residual, _ACTS.get(act, -1), out_dtype, index, _current_stream(index))
@@ -320,75 +340,71 @@ def _linear(x, weight, bias, slope, residual, act, out_dtype, way=_DIRECT):
             return torch.ops.fr_hip.linear(x, weight, bias, slope, residual, act, out_dtype)
     if way == _ABOVE:
         return None
-    dev = _check_tensors(op, x, weight, bias, slope, residual)
-    shape = _linear_shape(op, x, weight, residual)
+    dev, shape, kind, out_type, code = _check_linear(x, weight, bias, slope, residual, act, out_dtype)
     N, K = weight.shape
-    dtype = x.dtype
-    kind = _type(op, "x", dtype)
-    if weight.dtype != dtype:
-        _fail(op, f"x and weight have one type: got {dtype} and {weight.dtype}")
-    code = _name(op, _ACTS, act, "act")
-    if (slope is not None) != (act == "prelu"):
-        _fail(op, "slope belongs to act='prelu', and only to it")
-    bias_type, res_type, ldr = kind, kind, 0
-    bias_ptr = slope_ptr = res_ptr = ws_ptr = None
-    if bias is not None:
-        bias = _vector(op, "bias", bias, N, (dtype, torch.float32))
-        bias_type, bias_ptr = _TYPES[bias.dtype], bias.data_ptr()
-    if slope is not None:
-        slope = _vector(op, "slope", slope, N, (torch.float32,))
-        slope_ptr = slope.data_ptr()
-    if out_dtype is None or out_dtype == dtype:
-        out, out_type = x.new_empty(shape), kind
-    else:
-        out_type = _type(op, "out_dtype", out_dtype)
-        out = x.new_empty(shape, dtype=out_dtype)
-    if residual is not None:
-        res_type = _type(op, "residual", residual.dtype)
-        residual, ldr = _rows(residual, N)
-        res_ptr = residual.data_ptr()
+    out = x.new_empty(shape, dtype=out_dtype or x.dtype)
     M = out.numel() // N
     if M == 0:
         return out
     x, ldx = _rows(x, K)
-    weight = weight.contiguous()
+    weight, bias, slope = weight.contiguous(), _whole(bias), _whole(slope)
+    res_type, ldr = kind, 0
+    if residual is not None:
+        res_type = _TYPES[residual.dtype]
+        residual, ldr = _rows(residual, N)
     need = _scratch_bytes("fr_linear_workspace_bytes", M, N, K, kind)
-    if need:
-        ws = x.new_empty(need, dtype=torch.uint8)
-        ws_ptr = ws.data_ptr()
-    _call("fr_linear", dev, x.data_ptr(), ldx, weight.data_ptr(), bias_ptr, slope_ptr, res_ptr, ldr, out.data_ptr(),
-          M, N, K, kind, bias_type, res_type, out_type, code, ws_ptr, need)
+    ws = x.new_empty(need, dtype=torch.uint8) if need else None
+    _call("fr_linear", dev, x.data_ptr(), ldx, weight.data_ptr(), _ptr(bias), _ptr(slope), _ptr(residual), ldr, out.data_ptr(),
+          M, N, K, kind, kind if bias is None else _TYPES[bias.dtype], res_type, out_type, code, _ptr(ws), need)
     return out
 
 
-def _block_norm_shape(op, x, slot_weights):
-    least = 1 if slot_weights is None else 2
-    if x.dim() < least or x.shape[-1] < 1:
+def _check_block_norm(x, residual, slot_weights, norm, weight, bias, gate, gate_act, next_norm, next_weight, next_bias, out_dtype, next_dtype):
+    """(device, shape of the results, their dtypes, the gate's strides along rows and columns, codes of norm, next_norm and gate_act)."""
+    op = "block_norm"
+    dev = _check_tensors(op, x, residual, slot_weights, weight, bias, gate, next_weight, next_bias)
+    if x.dim() < (1 if slot_weights is None else 2) or x.shape[-1] < 1:
         _fail(op, f"expected x [..., d], or [..., slots, d] with slot_weights: got {tuple(x.shape)}")
-    if x.shape[-1] > 16384:
-        _fail(op, f"d is at most 16384: got {x.shape[-1]}")
-    if slot_weights is None:
-        return x.shape
-    if x.shape[-2] >= 1 << 31:
-        _fail(op, "slots have to fit 31 bits")
-    if slot_weights.shape != x.shape[:-1] or slot_weights.dtype != torch.float32 or x.shape[-2] < 1:
-        _fail(op, f"slot_weights is float32 {tuple(x.shape[:-1])}: got {slot_weights.dtype} {tuple(slot_weights.shape)}")
-    return x.shape[:-2] + x.shape[-1:]
-
-
-def _affine(op, what, norm, weight, bias, d):
-    if weight is None and bias is None:
-        return None, None
-    if norm not in (_lib.FR_NORM_RMS, _lib.FR_NORM_LAYER):
-        _fail(op, f"{what}weight and {what}bias belong to the rms and layer norms")
-    f32 = (torch.float32,)
-    return _vector(op, what + "weight", weight, d, f32), _vector(op, what + "bias", bias, d, f32)
+    d, shape = x.shape[-1], x.shape
+    if d > 16384:
+        _fail(op, f"d is at most 16384: got {d}")
+    if slot_weights is not None:
+        if x.shape[-2] >= 1 << 31:
+            _fail(op, "slots have to fit 31 bits")
+        if slot_weights.shape != x.shape[:-1] or slot_weights.dtype != torch.float32 or x.shape[-2] < 1:
+            _fail(op, f"slot_weights is float32 {tuple(x.shape[:-1])}: got {slot_weights.dtype} {tuple(slot_weights.shape)}")
+        shape = x.shape[:-2] + x.shape[-1:]
+    norm, next_norm = _name(op, _NORMS, norm, "norm"), _name(op, _NORMS, next_norm, "next_norm")
+    for what, code, w, b in (("", norm, weight, bias), ("next_", next_norm, next_weight, next_bias)):
+        if (w is not None or b is not None) and code not in (_lib.FR_NORM_RMS, _lib.FR_NORM_LAYER):
+            _fail(op, f"{what}weight and {what}bias belong to the rms and layer norms")
+        _check_of(op, what + "weight", w, (d,), torch.float32)
+        _check_of(op, what + "bias", b, (d,), torch.float32)
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    next_dtype = out_dtype if next_dtype is None else next_dtype
+    for what, dtype in (("out_dtype", out_dtype), ("next_dtype", next_dtype), ("x", x.dtype)):
+        _type(op, what, dtype)
+    if residual is not None:
+        if residual.shape != shape:
+            _fail(op, f"residual is {tuple(shape)}: got {tuple(residual.shape)}")
+        _type(op, "residual", residual.dtype)
+    strides = 0, 0
+    if gate is not None:
+        _type(op, "gate", gate.dtype)
+        if gate.shape == (d,):
+            strides = 0, 1
+        elif gate.shape == shape:
+            strides = d, 1
+        elif gate.shape == shape[:-1] + (1,):
+            strides = 1, 0
+        else:
+            _fail(op, f"gate is [{d}], {tuple(shape[:-1]) + (1,)} or {tuple(shape)}: got {tuple(gate.shape)}")
+    return dev, shape, out_dtype, next_dtype, strides, norm, next_norm, _name(op, _GATE_ACTS, gate_act, "gate_act")
 
 
 def _block_norm_eager(x, residual, slot_weights, norm, weight, bias, eps, gate, gate_act, scale, next_norm, next_weight, next_bias,
                       next_eps, out_dtype, next_dtype, way=_DIRECT):
     """(out, next), None (through the dispatcher: a tensor without elements) for a next that is not asked for."""
-    op = "block_norm"
     if x.is_cuda:
         index = _current_device()
         both = _lib.calls().block_norm(x, residual, slot_weights, _NORMS.get(norm, -1), weight, bias, eps, gate, _GATE_ACTS.get(gate_act, -1),
@@ -401,42 +417,20 @@ def _block_norm_eager(x, residual, slot_weights, norm, weight, bias, eps, gate, 
                                                next_weight, next_bias, next_eps, out_dtype, next_dtype)
     if way == _ABOVE:
         return None
-    dev = _check_tensors(op, x, residual, slot_weights, weight, bias, gate, next_weight, next_bias)
-    shape = _block_norm_shape(op, x, slot_weights)
+    dev, shape, out_dtype, next_dtype, (gate_ldt, gate_ldc), norm, next_norm, gate_act = _check_block_norm(
+        x, residual, slot_weights, norm, weight, bias, gate, gate_act, next_norm, next_weight, next_bias, out_dtype, next_dtype)
     d = x.shape[-1]
-    norm, next_norm = _name(op, _NORMS, norm, "norm"), _name(op, _NORMS, next_norm, "next_norm")
-    weight, bias = _affine(op, "", norm, weight, bias, d)
-    next_weight, next_bias = _affine(op, "next_", next_norm, next_weight, next_bias, d)
-    out_dtype = x.dtype if out_dtype is None else out_dtype
-    next_dtype = out_dtype if next_dtype is None else next_dtype
-    out_type, next_type, x_type = _type(op, "out_dtype", out_dtype), _type(op, "next_dtype", next_dtype), _type(op, "x", x.dtype)
-    res_type = gate_type = gate_ldt = gate_ldc = 0
-    if residual is not None:
-        if residual.shape != shape:
-            _fail(op, f"residual is {tuple(shape)}: got {tuple(residual.shape)}")
-        res_type, residual = _type(op, "residual", residual.dtype), residual.contiguous()
-    if gate is not None:
-        gate_type = _type(op, "gate", gate.dtype)
-        if gate.shape == (d,):
-            gate, gate_ldc = gate.contiguous(), 1
-        elif gate.shape == shape:
-            gate, gate_ldt, gate_ldc = gate.contiguous(), d, 1
-        elif gate.shape == shape[:-1] + (1,):
-            gate, gate_ldt = gate.contiguous(), 1
-        else:
-            _fail(op, f"gate is [{d}], {tuple(shape[:-1]) + (1,)} or {tuple(shape)}: got {tuple(gate.shape)}")
-    gate_act = _name(op, _GATE_ACTS, gate_act, "gate_act")
     out = x.new_empty(shape, dtype=out_dtype)
     nxt = x.new_empty(shape, dtype=next_dtype) if next_norm else None
     T = out.numel() // d
     if T == 0:
         return out, nxt
     slots = 0 if slot_weights is None else x.shape[-2]
-    x = x.contiguous()
-    slot_weights = None if slot_weights is None else slot_weights.contiguous()
-    _call("fr_block_norm", dev, x.data_ptr(), x_type, slots, _ptr(slot_weights), T, d, norm, _ptr(weight), _ptr(bias), eps,
-          _ptr(gate), gate_type, gate_ldt, gate_ldc, gate_act, scale, _ptr(residual), res_type, out.data_ptr(), out_type,
-          next_norm, _ptr(next_weight), _ptr(next_bias), next_eps, _ptr(nxt), next_type)
+    x, residual, slot_weights, weight, bias, gate, next_weight, next_bias = map(_whole, (x, residual, slot_weights, weight, bias, gate, next_weight, next_bias))
+    _call("fr_block_norm", dev, x.data_ptr(), _TYPES[x.dtype], slots, _ptr(slot_weights), T, d, norm, _ptr(weight), _ptr(bias), eps,
+          _ptr(gate), 0 if gate is None else _TYPES[gate.dtype], gate_ldt, gate_ldc, gate_act, scale,
+          _ptr(residual), 0 if residual is None else _TYPES[residual.dtype], out.data_ptr(), _TYPES[out_dtype],
+          next_norm, _ptr(next_weight), _ptr(next_bias), next_eps, _ptr(nxt), _TYPES[next_dtype])
     return out, nxt
 
 
@@ -450,15 +444,26 @@ def _block_norm(x, residual, slot_weights, norm, weight, bias, eps, gate, gate_a
     return out, x.new_empty(0, dtype=next_dtype or out.dtype) if nxt is None else nxt      # the op's schema has two results
 
 
-def _route_shape(op, logits, k):
+def _check_route(logits, k, score, bias, groups, top_groups):
+    """(device, codes of the logits' type and of score)."""
+    op = "route"
+    dev = _check_tensors(op, logits, bias)
     if logits.dim() != 2 or logits.shape[1] < 1:
         _fail(op, f"expected logits [T, E]: got {tuple(logits.shape)}")
-    T, E = logits.shape
+    E = logits.shape[1]
     if E > 512:
         _fail(op, f"at most 512 experts: got {E}")
     if not 1 <= k <= min(E, 16):
         _fail(op, f"1 <= k <= 16 of {E} experts: got {k}")
-    return T, E
+    if logits.shape[0] >= 1 << 30 or logits.shape[0] * k >= 1 << 31:
+        _fail(op, f"T has to fit 30 bits and T * k 31: got {logits.shape[0]} and k = {k}")
+    if not 1 <= groups <= 64 or not 1 <= top_groups <= groups or E % groups:
+        _fail(op, f"1 <= top_groups <= groups <= 64, groups dividing {E}: got {top_groups} of {groups}")
+    if top_groups * (E // groups) < k:
+        _fail(op, f"{top_groups} of {groups} groups hold fewer than {k} experts")
+    kind = _type(op, "logits", logits.dtype)
+    _check_of(op, "bias", bias, (E,), torch.float32)
+    return dev, kind, _name(op, _SCORES, score, "score")
 
 
 def _route_empty(logits, k):
@@ -469,7 +474,6 @@ def _route_empty(logits, k):
 
 
 def _route(logits, k, score, bias, groups, top_groups, renormalise, scale, way=_DIRECT):
-    op = "route"
     if logits.is_cuda:
         index = _current_device()
         out = _lib.calls().route(logits, k, _SCORES.get(score, -1), bias, groups, top_groups, renormalise, scale, index, _current_stream(index))
@@ -479,14 +483,9 @@ def _route(logits, k, score, bias, groups, top_groups, renormalise, scale, way=_
             return torch.ops.fr_hip.route(logits, k, score, bias, groups, top_groups, renormalise, scale)
     if way == _ABOVE:
         return None
-    dev = _check_tensors(op, logits, bias)
-    T, E = _route_shape(op, logits, k)
-    if not 1 <= groups <= 64 or not 1 <= top_groups <= groups:
-        _fail(op, f"1 <= top_groups <= groups <= 64: got {top_groups} of {groups}")
-    kind = _type(op, "logits", logits.dtype)
-    score = _name(op, _SCORES, score, "score")
-    bias = _vector(op, "bias", bias, E, (torch.float32,))
-    logits = logits.contiguous()
+    dev, kind, score = _check_route(logits, k, score, bias, groups, top_groups)
+    T, E = logits.shape
+    logits, bias = logits.contiguous(), _whole(bias)
     need = _scratch_bytes("fr_route_workspace_bytes", T, E, k)
     out = _route_empty(logits, k)
     ws = logits.new_empty(need, dtype=torch.uint8) if need else None
@@ -495,7 +494,10 @@ def _route(logits, k, score, bias, groups, top_groups, renormalise, scale, way=_
     return out
 
 
-def _expert_shape(op, x, weight, order, offsets, k, rows, out):
+def _check_expert_linear(x, weight, order, offsets, k, bias, act, slope, rows, out, out_dtype):
+    """(device, shape of the result, codes of x's type, of out_dtype and of act)."""
+    op = "expert_linear"
+    dev = _check_tensors(op, x, weight, order, offsets, bias, slope)
     if x.dim() != 2 or weight.dim() != 3 or x.shape[1] != weight.shape[2] or min(weight.shape) < 1:
         _fail(op, f"expected x [rows, K] and weight [E, N, K]: got {tuple(x.shape)} and {tuple(weight.shape)}")
     if rows not in ("tokens", "sorted") or out not in ("sorted", "slots"):
@@ -509,11 +511,12 @@ def _expert_shape(op, x, weight, order, offsets, k, rows, out):
     T = order.shape[0] // k
     if x.shape[0] != (T if rows == "tokens" else T * k):
         _fail(op, f"rows={rows!r} takes {T if rows == 'tokens' else T * k} rows of x: got {x.shape[0]}")
-    return T, (T * k, weight.shape[1]) if out == "sorted" else (T, k, weight.shape[1])
+    kind, code = _check_product(op, x, weight, bias, slope, weight.shape[:2], act)
+    shape = (T * k, weight.shape[1]) if out == "sorted" else (T, k, weight.shape[1])
+    return dev, shape, kind, kind if out_dtype is None else _type(op, "out_dtype", out_dtype), code
 
 
 def _expert_linear(x, weight, order, offsets, k, bias, act, slope, rows, out, out_dtype, way=_DIRECT):
-    op = "expert_linear"
     if x.is_cuda:
         index = _current_device()
         y = _lib.calls().expert_linear(x, weight, order, offsets, k, bias, _ACTS.get(act, -1), slope, _ROWS.get(rows, -1), _OUTS.get(out, -1),
@@ -524,32 +527,16 @@ def _expert_linear(x, weight, order, offsets, k, bias, act, slope, rows, out, ou
             return torch.ops.fr_hip.expert_linear(x, weight, order, offsets, k, bias, act, slope, rows, out, out_dtype)
     if way == _ABOVE:
         return None
-    dev = _check_tensors(op, x, weight, order, offsets, bias, slope)
-    T, shape = _expert_shape(op, x, weight, order, offsets, k, rows, out)
+    dev, shape, kind, out_type, code = _check_expert_linear(x, weight, order, offsets, k, bias, act, slope, rows, out, out_dtype)
     E, N, K = weight.shape
-    kind = _type(op, "x", x.dtype)
-    if weight.dtype != x.dtype:
-        _fail(op, f"x and weight have one type: got {x.dtype} and {weight.dtype}")
-    act = _name(op, _ACTS, act, "act")
-    if (slope is not None) != (act == _lib.FR_ACT_PRELU):
-        _fail(op, "slope belongs to act='prelu', and only to it")
-    if bias is not None:
-        if bias.shape != (E, N) or bias.dtype not in (x.dtype, torch.float32):
-            _fail(op, f"bias is [{E}, {N}] of x's type or float32: got {bias.dtype} {tuple(bias.shape)}")
-        bias = bias.contiguous()
-    if slope is not None:
-        if slope.shape != (E, N) or slope.dtype != torch.float32:
-            _fail(op, f"slope is float32 [{E}, {N}]: got {slope.dtype} {tuple(slope.shape)}")
-        slope = slope.contiguous()
-    out_dtype = x.dtype if out_dtype is None else out_dtype
-    y = x.new_empty(shape, dtype=out_dtype)
-    out_type = _type(op, "out_dtype", out_dtype)
+    y = x.new_empty(shape, dtype=out_dtype or x.dtype)
+    T = order.shape[0] // k
     if T == 0:
         return y
-    x, weight, order, offsets = x.contiguous(), weight.contiguous(), order.contiguous(), offsets.contiguous()
+    x, weight, order, offsets, bias, slope = map(_whole, (x, weight, order, offsets, bias, slope))
     _call("fr_expert_linear", dev, x.data_ptr(), int(rows == "sorted"), weight.data_ptr(), _ptr(bias), _ptr(slope), order.data_ptr(),
           offsets.data_ptr(), y.data_ptr(), int(out == "slots"), T, k, E, N, K, kind, kind if bias is None else _TYPES[bias.dtype],
-          out_type, act)
+          out_type, code)
     return y
 
 
@@ -595,22 +582,23 @@ _meta.impl("topk_merge", lambda s, i, k: (s.new_empty((s.shape[1], k), dtype=tor
 
 
 def _meta_linear(x, weight, bias, slope, residual, act, out_dtype):
-    return x.new_empty(_linear_shape("linear", x, weight, residual), dtype=out_dtype or x.dtype)
+    return x.new_empty(_check_linear(x, weight, bias, slope, residual, act, out_dtype)[1], dtype=out_dtype or x.dtype)
 
 
 def _meta_block_norm(x, residual, slot_weights, norm, weight, bias, eps, gate, gate_act, scale, next_norm, next_weight, next_bias,
                      next_eps, out_dtype, next_dtype):
-    shape, out_dtype = _block_norm_shape("block_norm", x, slot_weights), out_dtype or x.dtype
-    return x.new_empty(shape, dtype=out_dtype), x.new_empty(shape if next_norm != "none" else 0, dtype=next_dtype or out_dtype)
+    _, shape, out_dtype, next_dtype, *_ = _check_block_norm(x, residual, slot_weights, norm, weight, bias, gate, gate_act, next_norm, next_weight,
+                                                            next_bias, out_dtype, next_dtype)
+    return x.new_empty(shape, dtype=out_dtype), x.new_empty(shape if next_norm != "none" else 0, dtype=next_dtype)
 
 
 def _meta_route(logits, k, score, bias, groups, top_groups, renormalise, scale):
-    _route_shape("route", logits, k)
+    _check_route(logits, k, score, bias, groups, top_groups)
     return _route_empty(logits, k)
 
 
 def _meta_expert_linear(x, weight, order, offsets, k, bias, act, slope, rows, out, out_dtype):
-    return x.new_empty(_expert_shape("expert_linear", x, weight, order, offsets, k, rows, out)[1], dtype=out_dtype or x.dtype)
+    return x.new_empty(_check_expert_linear(x, weight, order, offsets, k, bias, act, slope, rows, out, out_dtype)[1], dtype=out_dtype or x.dtype)
 
 
 _meta.impl("linear", _meta_linear)

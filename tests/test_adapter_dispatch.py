@@ -300,3 +300,29 @@ def test_fake_tensors_need_no_gpu(name):
         for got in (function(name, args), getattr(torch.ops.fr_hip, name)(*args)):
             assert all(y.is_cuda for y in flat(got))
         refused(lambda: getattr(torch.ops.fr_hip, name)(*replaced(args, 0, args[0].requires_grad_())), "no_grad")
+
+
+# ---- tensors without data ----------------------------------------------------------------------------------------------
+
+def refusals():
+    """Every refusal that the functions are tested for, and some that stand in the C entries."""
+    import test_adapter as ta
+    base = {"linear": dict(x=torch.zeros(2, 8), weight=torch.zeros(4, 8), **ta.LINEAR), "block_norm": dict(x=torch.zeros(2, 8), **ta.NORM),
+            "route": dict(logits=torch.zeros(2, 8), **ta.ROUTE), "expert_linear": dict(x=torch.zeros(2, 8), weight=torch.zeros(3, 4, 8), **ta.EXPERT)}
+    for name, test in zip(OPS, (ta.test_linear_refuses, ta.test_block_norm_refuses, ta.test_route_refuses, ta.test_expert_linear_refuses)):
+        for change, words in test.pytestmark[0].args[1]:
+            if words != "all tensors on":                      # all of these are on one device
+                yield name, base[name], change, words
+    for change, words in ((dict(groups=3), "groups"), (dict(groups=8, top_groups=1), "fewer than"), (dict(logits=torch.zeros(1, 8).expand(1 << 30, 8)), "30 bits"),
+                          (dict(logits=torch.zeros(1, 8).expand((1 << 28) + 1, 8), k=8), "30 bits")):
+        yield "route", base["route"], change, words
+
+
+@pytest.mark.parametrize("name, base, change, words", list(refusals()))
+def test_tensors_without_data_meet_the_same_checks(name, base, change, words):
+    def moved(kw):
+        return {n: v.to("meta") if isinstance(v, torch.Tensor) else v for n, v in kw.items()}
+    op = getattr(torch.ops.fr_hip, name)
+    op(**moved(base))
+    with pytest.raises(RuntimeError, match=words):
+        op(**moved({**base, **change}))
