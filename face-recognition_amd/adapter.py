@@ -96,7 +96,8 @@ def expert_linear(x: torch.Tensor, weight: torch.Tensor, routing: Routing, bias:
     """``act(row @ weight[e].T + bias[e])`` for every slot of ``routing``: weight [E, N, K], bias [E, N].  rows="tokens"
     takes x [T, K] (each row once per expert it chose), rows="sorted" x [T * k, K] in the order's positions;
     out="sorted" answers [T * k, N] in those positions, out="slots" [T, k, N] by slot, ready for ``block_norm``'s
-    slot_weights.  Slots without an expert get zero rows."""
+    slot_weights.  Slots without an expert get zero rows.  The tables are taken as ``route`` gives them: nothing is written
+    for an entry of the order that names no slot."""
     _need_gpu(x, "expert_linear")
     return _op("expert_linear", x)(x, weight, routing.order, routing.offsets, routing.experts.shape[1], bias, act, slope,
                                           rows, out, out_dtype)

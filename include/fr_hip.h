@@ -276,7 +276,9 @@ int fr_route(const void* logits, int logits_type, int64_t T, int E, int k, int s
 /* out = act(row x w[e]^T + bias[e]) for every routed slot, e the slot's expert; order / offsets as fr_route writes them for T*k slots.
  * w [E][N][K], bias [E][N] or NULL, slope fp32 [E][N] for FR_ACT_PRELU.  rows_sorted 0: x [T][K], slot s takes row s / k;
  * rows_sorted 1: x [T*k][K], position p of the order takes row p.  out_slots 0: out [T*k][N] in the order's positions;
- * out_slots 1: out row = slot number.  Slots without an expert get zero rows.  An order entry outside [0, T*k) is skipped. */
+ * out_slots 1: out row = slot number.  Slots without an expert get zero rows.  An order entry outside [0, T*k) is skipped: nothing is
+ * written for its position (rows_sorted 1 with out_slots 0 does not read the order); the same goes for positions that the
+ * offsets leave out.  Offsets outside [0, T*k] are taken as its nearer end. */
 int fr_expert_linear(const void* x, int rows_sorted, const void* w, const void* bias, const float* slope,
                      const int32_t* order, const int32_t* offsets, void* out, int out_slots,
                      int64_t T, int k, int E, int N, int K, int type, int bias_type, int out_type, int act, void* stream);

@@ -56,3 +56,60 @@ def test_route_bias_of_infinity_in_groups(score, kind, e, groups, top, k):
         w, ex, _, _ = oa.route(logits[rows], k, score, b, groups, top)
         assert torch.equal(got.experts[rows].cpu(), ex), rows
         assert float((got.weights[rows].cpu().double() - w).abs().max()) < (128 + e) * 2.0 ** -24
+
+
+# ---- expert_linear -----------------------------------------------------------------------------------------------------
+
+def expert_entry(x, w, order, offsets, k, rows_sorted, out_slots, out):
+    """The C entry, into memory of the caller's."""
+    from face_recognition_amd import _lib, ops
+    E, N, K = w.shape
+    _lib.check(_lib.lib().fr_expert_linear(x.data_ptr(), rows_sorted, w.data_ptr(), None, None, order.data_ptr(), offsets.data_ptr(), out.data_ptr(), out_slots,
+                                           order.numel() // k, k, E, N, K, ops._TYPES[x.dtype], ops._TYPES[x.dtype], ops._TYPES[out.dtype], 0,
+                                           torch.cuda.current_stream().cuda_stream), "fr_expert_linear")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows_sorted, out_slots", [(0, 0), (0, 1), (1, 0), (1, 1)])
+@pytest.mark.parametrize("t, e, k, d, n", [(5, 8, 2, 512, 40), (9, 70, 2, 515, 17), (300, 3, 2, 65, 70), (300, 3, 2, 128, 70), (1500, 2, 2, 256, 264), (4000, 2, 1, 65, 520)])
+def test_expert_linear_order_entries_that_lie_are_skipped(kind, rows_sorted, out_slots, t, e, k, d, n):
+    """Few rows, rows of any alignment, small and large tiles: nothing is written for such an entry, and nothing outside the output."""
+    g, P, MARK = gen(t + d), t * k, 7.0
+    ex = torch.randint(0, e, (t, k), generator=g, device="cuda", dtype=torch.int32)
+    ex[torch.rand(t, k, generator=g, device="cuda") < 0.2] = -1
+    order, offsets = oa.routing_of(ex, e)
+    x, w = randn(g, P if rows_sorted else t, d, dtype=kind), randn(g, e, n, d, dtype=kind)
+    room = 4096
+
+    def run(order):
+        memory = torch.full((2 * room + P * n,), MARK, dtype=kind, device="cuda")
+        out = memory[room:room + P * n]
+        expert_entry(x, w, order, offsets, k, rows_sorted, out_slots, out)
+        torch.cuda.synchronize()
+        assert (memory[:room] == MARK).all() and (memory[-room:] == MARK).all()
+        return out.view(P, n)
+
+    want = run(order)
+    lies = order.clone()
+    at = torch.randperm(P, generator=g, device="cuda")[:max(2, P // 7)]
+    lies[at] = torch.tensor([P, -1, 1 << 30, -(1 << 31)], device="cuda", dtype=torch.int32)[torch.arange(at.numel(), device="cuda") % 4]
+    if out_slots:
+        want[order[at].long()] = MARK
+    elif not rows_sorted:
+        want[at] = MARK
+    assert torch.equal(run(lies), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t, e, k, d, n", [(5, 8, 2, 512, 40), (9, 70, 2, 515, 17), (300, 3, 2, 65, 70), (1500, 2, 2, 256, 264)])
+def test_expert_linear_offsets_that_lie_write_nothing_outside(t, e, k, d, n):
+    g, P, MARK, room = gen(t + d), t * k, 7.0, 4096
+    x, w = randn(g, t, d, dtype=torch.bfloat16), randn(g, e, n, d, dtype=torch.bfloat16)
+    order = torch.randperm(P, generator=g, device="cuda").to(torch.int32)
+    for _ in range(6):
+        offsets = torch.randint(-P, 3 * P, (e + 1,), generator=g, device="cuda", dtype=torch.int32)
+        memory = torch.full((2 * room + P * n,), MARK, dtype=torch.bfloat16, device="cuda")
+        expert_entry(x, w, order, offsets, k, 0, 0, memory[room:room + P * n])
+        torch.cuda.synchronize()
+        assert (memory[:room] == MARK).all() and (memory[-room:] == MARK).all()
