@@ -856,6 +856,7 @@ int launch_type(int type, const GemmArgs& a, hipStream_t st) {
 
 extern "C" int fr_linear_workspace_bytes(int64_t M, int N, int K, int type, size_t* out_bytes) {
     if (!out_bytes || M < 0 || N <= 0 || K <= 0 || !type_ok(type)) FR_FAIL(FR_ERR_ARG, "fr_linear_workspace_bytes: bad shape or type");
+    if (M >= 1ll << 40) FR_FAIL(FR_ERR_UNSUPPORTED, "fr_linear_workspace_bytes: M does not fit 40 bits");
     const int splits = split_count(M, N, K, type);
     *out_bytes = splits > 1 ? (size_t)splits * M * N * 4 : 0;
     return FR_OK;
@@ -866,6 +867,7 @@ extern "C" int fr_linear(const void* x, int64_t ldx, const void* w, const void* 
                          int type, int bias_type, int res_type, int out_type, int act,
                          void* workspace, size_t workspace_bytes, void* stream) {
     if (M < 0 || N <= 0 || K <= 0 || ldx < 0 || (residual && ldr < 0)) FR_FAIL(FR_ERR_ARG, "fr_linear: bad shape");
+    if (M >= 1ll << 40) FR_FAIL(FR_ERR_UNSUPPORTED, "fr_linear: M does not fit 40 bits");
     if (!type_ok(type) || !type_ok(out_type) || (bias && bias_type != type && bias_type != FR_TYPE_F32) || (residual && !type_ok(res_type)))
         FR_FAIL(FR_ERR_ARG, "fr_linear: unknown element type (bias: the operands' type or fp32)");
     if (act < FR_ACT_NONE || act > FR_ACT_SILU) FR_FAIL(FR_ERR_ARG, "fr_linear: unknown activation");
@@ -886,7 +888,7 @@ extern "C" int fr_expert_linear(const void* x, int rows_sorted, const void* w, c
                                 const int32_t* order, const int32_t* offsets, void* out, int out_slots,
                                 int64_t T, int k, int E, int N, int K, int type, int bias_type, int out_type, int act, void* stream) {
     if (T < 0 || k <= 0 || E <= 0 || N <= 0 || K <= 0) FR_FAIL(FR_ERR_ARG, "fr_expert_linear: bad shape");
-    if (T * k > 0x7FFFFFFFll) FR_FAIL(FR_ERR_UNSUPPORTED, "fr_expert_linear: T * k does not fit 31 bits");
+    if (T > 0x7FFFFFFFll / k) FR_FAIL(FR_ERR_UNSUPPORTED, "fr_expert_linear: T * k does not fit 31 bits");
     if (!type_ok(type) || !type_ok(out_type) || (bias && bias_type != type && bias_type != FR_TYPE_F32))
         FR_FAIL(FR_ERR_ARG, "fr_expert_linear: unknown element type (bias: the operands' type or fp32)");
     if (act < FR_ACT_NONE || act > FR_ACT_SILU) FR_FAIL(FR_ERR_ARG, "fr_expert_linear: unknown activation");

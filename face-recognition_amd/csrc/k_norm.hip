@@ -202,6 +202,7 @@ extern "C" int fr_block_norm(const void* x, int x_type, int slots, const float* 
                              int next_norm, const float* next_weight, const float* next_bias, float next_eps,
                              void* next_out, int next_type, void* stream) {
     if (T < 0 || d <= 0 || d > 16384 || slots < 0) FR_FAIL(FR_ERR_ARG, "fr_block_norm: bad shape (1 <= d <= 16384)");
+    if (T >= 1ll << 40) FR_FAIL(FR_ERR_UNSUPPORTED, "fr_block_norm: T does not fit 40 bits");
     if (norm < 0 || norm > FR_NORM_L2 || next_norm < 0 || next_norm > FR_NORM_L2) FR_FAIL(FR_ERR_ARG, "fr_block_norm: unknown norm");
     if (gate_act < 0 || gate_act > FR_GATE_TANH) FR_FAIL(FR_ERR_ARG, "fr_block_norm: unknown gate activation");
     if (!type_ok(x_type) || (gate && !type_ok(gate_type)) || (residual && !type_ok(res_type)) || (out && !type_ok(out_type)) ||

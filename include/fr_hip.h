@@ -223,8 +223,8 @@ int fr_topk_merge_packed(const void* packed, int P, int64_t Q, int k,
 
 /* ---- adapter operators (no counterpart in the reference) ------------------------------------------------------------
  * A residual block over embedding rows: products with their epilogue, norms fused with gate, scale and residual, and the
- * mixture form of both (a router and its experts' products).  Inference only.  All row-major; matrices may start at any
- * address their element type allows; statistics, sums and epilogues are fp32, results are rounded once. */
+ * mixture form of both (a router and its experts' products).  Inference only.  All row-major, fewer than 2^40 rows; matrices
+ * may start at any address their element type allows; statistics, sums and epilogues are fp32, results are rounded once. */
 
 /* out[m][n] = act(sum_k x[m][k] w[n][k] + bias[n]) + residual[m][n].
  * x [M][K] (row stride ldx), w [N][K] contiguous, both of type `type` (fp32 products are exact fp32 MFMA, not split);

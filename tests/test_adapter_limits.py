@@ -113,3 +113,22 @@ def test_expert_linear_offsets_that_lie_write_nothing_outside(t, e, k, d, n):
         expert_entry(x, w, order, offsets, k, 0, 0, memory[room:room + P * n])
         torch.cuda.synchronize()
         assert (memory[:room] == MARK).all() and (memory[-room:] == MARK).all()
+
+
+# ---- counts that wrap --------------------------------------------------------------------------------------------------
+
+def test_c_entries_refuse_counts_that_wrap():
+    """Row counts whose products leave 64 bits are refused before anything is launched (there is no GPU here)."""
+    import ctypes as C
+    from face_recognition_amd import _lib
+    lib, at, need = _lib.lib(), 4096, C.c_size_t()
+
+    def refused(rc, words):
+        assert rc == -2 and words in lib.fr_last_error().decode(), (rc, lib.fr_last_error())
+
+    for T, k in ((1 << 30, 2), ((1 << 33) + 1, (1 << 31) - 1), (1 << 62, 4), ((1 << 62) + 1, 4), ((1 << 63) - 1, 2), ((1 << 61) + 5, 8)):
+        refused(lib.fr_expert_linear(at, 0, at, None, None, at, at, at, 0, T, k, 4, 8, 8, 1, 1, 1, 0, None), "31 bits")
+    for M in (1 << 40, 1 << 57, (1 << 63) - 1):
+        refused(lib.fr_linear(at, 8, at, None, None, None, 0, at, M, 8, 8, 1, 1, 1, 1, 0, None, 0, None), "40 bits")
+        refused(lib.fr_linear_workspace_bytes(M, 8, 4096, 1, C.byref(need)), "40 bits")
+        refused(lib.fr_block_norm(at, 1, 0, None, M, 8, 1, None, None, 1e-6, None, 1, 0, 1, 0, 1.0, None, 0, at, 1, 0, None, None, 1e-6, None, 1, None), "40 bits")
