@@ -54,8 +54,9 @@ bool interposed(PyObject* const* args, Py_ssize_t count) {
     const c10::impl::LocalDispatchKeySet thread = c10::impl::tls_local_dispatch_key_set();
     if ((thread.included_.raw_repr() & ~thread.excluded_.raw_repr() & ~plain) || at::impl::torch_function_mode_enabled()) return true;
     for (Py_ssize_t i = 0; i < count; ++i) {
-        if (!THPVariable_Check(args[i])) continue;
-        if (!THPVariable_CheckExact(args[i]) || (THPVariable_Unpack(args[i]).key_set().raw_repr() & ~plain)) return true;
+        PyObject* a = args[i];
+        if (a == Py_None || PyLong_Check(a) || PyFloat_Check(a) || THPDtype_Check(a) || !THPVariable_Check(a)) continue;     // the last one is slow for these
+        if (!THPVariable_CheckExact(a) || (THPVariable_Unpack(a).key_set().raw_repr() & ~plain)) return true;
     }
     return false;
 }

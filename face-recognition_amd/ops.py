@@ -218,10 +218,14 @@ def _type(op, what, dtype):
 
 def _no_gradient(op, *tensors):
     """The kernels have no backward pass and carry no tangents, and a result that silently cuts the graph would be a wrong one."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        _fail(op, "inference only: call it under torch.no_grad() or on detached tensors")
-    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
-        _fail(op, "inference only: a tensor has a forward-mode tangent")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                _fail(op, "inference only: call it under torch.no_grad() or on detached tensors")
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                _fail(op, "inference only: a tensor has a forward-mode tangent")
 
 
 def _check_tensors(op, first, *others):
@@ -283,7 +287,7 @@ def _rows(t, width):
 
 
 def _check_of(op, what, t, shape, *dtypes):
-    if t is not None and (t.shape != shape or t.dtype not in dtypes):
+    if t.shape != shape or t.dtype not in dtypes:
         _fail(op, f"{what} is {list(shape)} of {' or '.join(str(d)[6:] for d in dtypes)}: got {t.dtype} {tuple(t.shape)}")
 
 
@@ -318,8 +322,10 @@ def _check_product(op, x, weight, bias, slope, shape, act):
     code = _name(op, _ACTS, act, "act")
     if (slope is not None) != (code == _lib.FR_ACT_PRELU):
         _fail(op, "slope belongs to act='prelu', and only to it")
-    _check_of(op, "bias", bias, shape, x.dtype, torch.float32)
-    _check_of(op, "slope", slope, shape, torch.float32)
+    if bias is not None:
+        _check_of(op, "bias", bias, shape, x.dtype, torch.float32)
+    if slope is not None:
+        _check_of(op, "slope", slope, shape, torch.float32)
     return kind, code
 
 
@@ -342,7 +348,7 @@ def _linear(x, weight, bias, slope, residual, act, out_dtype, way=_DIRECT):
         return None
     dev, shape, kind, out_type, code = _check_linear(x, weight, bias, slope, residual, act, out_dtype)
     N, K = weight.shape
-    out = x.new_empty(shape, dtype=out_dtype or x.dtype)
+    out = x.new_empty(shape) if out_dtype is None else x.new_empty(shape, dtype=out_dtype)
     M = out.numel() // N
     if M == 0:
         return out
@@ -378,8 +384,10 @@ def _check_block_norm(x, residual, slot_weights, norm, weight, bias, gate, gate_
     for what, code, w, b in (("", norm, weight, bias), ("next_", next_norm, next_weight, next_bias)):
         if (w is not None or b is not None) and code not in (_lib.FR_NORM_RMS, _lib.FR_NORM_LAYER):
             _fail(op, f"{what}weight and {what}bias belong to the rms and layer norms")
-        _check_of(op, what + "weight", w, (d,), torch.float32)
-        _check_of(op, what + "bias", b, (d,), torch.float32)
+        if w is not None:
+            _check_of(op, what + "weight", w, (d,), torch.float32)
+        if b is not None:
+            _check_of(op, what + "bias", b, (d,), torch.float32)
     out_dtype = x.dtype if out_dtype is None else out_dtype
     next_dtype = out_dtype if next_dtype is None else next_dtype
     for what, dtype in (("out_dtype", out_dtype), ("next_dtype", next_dtype), ("x", x.dtype)):
@@ -462,7 +470,8 @@ def _check_route(logits, k, score, bias, groups, top_groups):
     if top_groups * (E // groups) < k:
         _fail(op, f"{top_groups} of {groups} groups hold fewer than {k} experts")
     kind = _type(op, "logits", logits.dtype)
-    _check_of(op, "bias", bias, (E,), torch.float32)
+    if bias is not None:
+        _check_of(op, "bias", bias, (E,), torch.float32)
     return dev, kind, _name(op, _SCORES, score, "score")
 
 
@@ -529,7 +538,7 @@ def _expert_linear(x, weight, order, offsets, k, bias, act, slope, rows, out, ou
         return None
     dev, shape, kind, out_type, code = _check_expert_linear(x, weight, order, offsets, k, bias, act, slope, rows, out, out_dtype)
     E, N, K = weight.shape
-    y = x.new_empty(shape, dtype=out_dtype or x.dtype)
+    y = x.new_empty(shape) if out_dtype is None else x.new_empty(shape, dtype=out_dtype)
     T = order.shape[0] // k
     if T == 0:
         return y
