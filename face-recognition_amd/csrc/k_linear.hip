@@ -231,8 +231,8 @@ FR_DEV void tile_of_block(int block, int mtiles, int ntiles, int& mt, int& nt) {
 // What bounds it: a slice of a 256-tile is 2048 clocks of matrix instructions, as much LDS traffic (each wave's 128 x 64 outputs
 // read 24 KB of the two halves, 8 waves 192, and 64 KB are written), and takes 2390 to 2550, at the 1.3 to 1.8 GHz the card
 // holds under it; launch, first loads and epilogue are 10 us a tile, which a tile alone on its CU does not hide.
-// bf16: 8192 cubed 754 us (1459 TFLOP/s; the library 662), 16384 x 2048 x 8192 383 (1435; 348), with bias and residual 403;
-// 65536 x 4096 x 1024 520, with silu 540; experts 65536 slots x 4096 x 1024 with silu 624.  fp32 8192 cubed 7.73 ms (142 of
+// bf16: 8192 cubed 754 us (1459 TFLOP/s; the library 662), 16384 x 2048 x 8192 383 (1435; 348), with bias and residual 401;
+// 65536 x 4096 x 1024 520, with silu 540; experts 65536 slots x 4096 x 1024 with silu 614.  fp32 8192 cubed 7.73 ms (142 of
 // 154).  Other ways to a 256-tile: 16 x 16 x 32 instructions reach 2145 TFLOP/s from registers alone, 32 x 32 x 16 1868; 4 waves
 // of 128 x 128 read less LDS, but their 256 accumulators leave no registers to read ahead.
 // WHOLE false: rows of any alignment.  The chunks of slice s + ST go to registers in the second half of slice s and to LDS in
@@ -751,9 +751,10 @@ double tile_count(const GemmArgs& a, int bm, int bn) {
     return rows * ((a.N + (bn - 1l)) / bn);
 }
 // Estimated time in us with tiles of bm x bn: `each` for a slice of 128 bytes of K and `fixed` for the rest of a tile, for every
-// tile of the fullest CU.  The constants are least squares over 90 shapes of 64 to 18 000 rows on one card (rms 3 % in fp32,
-// 13 to 15 % in 16 bits); what the rule picks took 1.5 % more than the best of all tiles there (fp32: 1.8 %), and in 16 bits
-// 0.79 of the time of the library's plain product (fp32: 1.03).
+// tile of the fullest CU.  The constants are least squares over some 90 shapes of 100 to 18 700 rows on one card, which
+// profiles/tuning/adapter_tiles.txt lists with every tile's time (rms 3 % in fp32, 13 to 16 % in 16 bits); what the rule picks takes
+// 1.4 % more than the best of all tiles there (fp32: 1.8 %), and 0.79 of the time of the library's plain product (fp32: 1.03; 0.82
+// and 0.99 where the library's time is not mostly the host's).
 template <typename T>
 double tile_cost(const GemmArgs& a, int bm, int bn, double each16, double fixed16, double each32, double fixed32) {
     constexpr bool f32 = std::is_same<T, float>::value;

@@ -169,8 +169,9 @@ FR_DEV void one_row(const NormArgs& a, long row, int col0, float (*part)[4], int
 
 // One row per wave (TPR = 64, 4 rows a block) or per block (TPR = 256).
 // VEC: d is a multiple of 8 and every tensor starts at a 16-byte address.
-// Bound by memory: 65536 x 512 bf16, gate, residual and unit rows out, moves its 268 MB in 53 us, 5.0 TB/s (a copy of 4 GiB: 4.85);
-// asking for the residual with the row changed nothing, a loop over rows inside the kernel cost a third.
+// Bound by memory: 65536 x 512 bf16, gate, residual and unit rows out, moves its 268 MB in 58 us a call over three inputs in turn,
+// 4.6 TB/s (a copy of 4 GiB: 4.8); 49 to 54 on one input, part of which stays in the cache.
+// Asking for the residual with the row changed nothing, a loop over rows inside the kernel cost a third.
 template <int TPR, int NV, bool VEC>
 __global__ __launch_bounds__(256) void block_norm_kernel(NormArgs a) {
     __shared__ float part[2][4];

@@ -276,8 +276,9 @@ FR_DEV void first_places(const RouteArgs& a, int* next, bool write, F n, G more)
 // is at most 4 steps of 2^-24 for a sigmoid (exp2's argument and result, the sum, the reciprocal) and 32 for a softmax
 // (the row's sum of up to 512 besides).  At 65536 x 256, biased sigmoids, 8 of 256 in 4 of 8 groups, one row in 500 goes
 // that way; with the expert's number in the scored keys too it was one in 50, which took more time than all the rest.
-// What bounds it: 970 vector and 370 scalar instructions for 4 rows of 256 (the read alone would take 15 us of the 51 at
-// 65536 x 256); a wave is done after 32 us in the mean, 41 at most without a row done again, and such a row takes 8.5.
+// What bounds it: 970 vector and 370 scalar instructions for 4 rows of 256.  At 65536 x 256 (traced by itself 50 us; the read alone
+// would take 15) vector instructions hold the SIMDs for two thirds of that, and a wave lives 40 us in the mean: the one round of
+// blocks waits for the waves with rows that doubles decide (about 120 rows, 8.5 us each, one after the other).
 enum { BY_LOGIT, BY_SCORE, BY_LOGIT_IN_GROUPS };
 template <int V, int LPR, int NE, int NB, int ORDER>
 __global__ __launch_bounds__(512, 4) void route_choose_kernel(RouteArgs a) {
@@ -466,7 +467,7 @@ __global__ __launch_bounds__(512, 4) void route_choose_kernel(RouteArgs a) {
     }
 }
 
-// counts[e][c] -> number of e's slots in the chunks before c; totals[e].  One block per expert, four chunks a thread: 4 us for
+// counts[e][c] -> number of e's slots in the chunks before c; totals[e].  One block per expert, four chunks a thread: 3 to 5 us for
 // 256 x 1024, launch and latency.
 __global__ __launch_bounds__(256) void route_scan_kernel(RouteArgs a) {
     __shared__ int part[2][4];
@@ -495,7 +496,7 @@ __global__ __launch_bounds__(256) void route_scan_kernel(RouteArgs a) {
 }
 
 // Places of a chunk's slots: first place of the expert + its slots in earlier chunks + earlier in this chunk.  524288 slots of
-// 256 experts 8.4 us: 512 slots a wave, 64 at a time, each after the one before.
+// 256 experts 8.6 us: 512 slots a wave, 64 at a time, each after the one before.
 __global__ __launch_bounds__(64) void route_place_kernel(RouteArgs a) {
     __shared__ int next[RT_EMAX + 1];
     const long s0 = (long)blockIdx.x * RT_ROWS * a.k;
@@ -505,8 +506,8 @@ __global__ __launch_bounds__(64) void route_place_kernel(RouteArgs a) {
     place_slots(a, next, slots, n, s0);
 }
 
-// Blocks of 8 waves while 4 would leave places for waves empty (256 CUs hold 1024 blocks of 4): 20000 x 512 62 us, 79 by 4;
-// 65536 x 256, all 1024 blocks at once, 66 us by 4, 69 by 8.
+// Blocks of 8 waves while 4 would leave places for waves empty (256 CUs hold 1024 blocks of 4), us a call of all three launches:
+// 20000 x 512 60 by 8, 73 by 4; 65536 x 256, whose 1024 blocks of 4 are there at once, 61 by 4, 62 by 8 (without groups 40 and 44).
 template <int V, int LPR, int NE, int NB>
 void launch_choose(const RouteArgs& a, hipStream_t st) {
     const long needed = (a.T * LPR + 63) / 64;                // of a single chunk

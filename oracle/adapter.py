@@ -74,7 +74,8 @@ def route(logits, k, score="softmax", bias=None, groups=1, top_groups=1, renorma
         key = [(v if plain else q + c) if l else -math.inf for v, q, c, l in zip(row, p, b, live)]
         if groups > 1:
             per = E // groups
-            best = [sum(sorted(key[g * per:(g + 1) * per])[-2:]) for g in range(groups)]
+            two = [sorted(key[g * per:(g + 1) * per])[-2:] for g in range(groups)]
+            best = [sum(v) if v[0] > -math.inf else -math.inf for v in two]      # of a lone expert too, whatever its bias
             keep = sorted(range(groups), key=lambda g: (-best[g], g))[:top_groups]
             key = [v if i // per in keep else -math.inf for i, v in enumerate(key)]
         pick = [i for i in sorted(range(E), key=lambda i: (-key[i], i))[:k] if key[i] > -math.inf]
