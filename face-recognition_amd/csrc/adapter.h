@@ -78,6 +78,9 @@ FR_DEV void store8t(void* base, long i, int type, const Vec8f& x) {
     }
 }
 
+// LDS written by other lanes of this wave is read behind it (a wave's LDS accesses are carried out in order).
+FR_DEV void wave_lds_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); __builtin_amdgcn_wave_barrier(); }
+
 // Sums over the lanes up to each lane.
 FR_DEV int scan_add(int v) {
     v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);          // 1, 2, 4 and 8 lanes back in a row of 16

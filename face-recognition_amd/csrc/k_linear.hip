@@ -205,9 +205,6 @@ FR_DEV void block_barrier() {                              // without the waits 
     __builtin_amdgcn_sched_barrier(0);
 }
 
-// LDS written by other lanes of this wave is read behind it (a wave's LDS accesses are carried out in order).
-FR_DEV void wave_lds_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); __builtin_amdgcn_wave_barrier(); }
-
 // Block -> output tile.  Blocks go to the 8 XCDs in turn and each XCD has its own L2: a contiguous run of tiles for each,
 // walked in groups of 4 row tiles by every n tile, so that the blocks of an XCD that run at the same time share their operands
 // (groups of 8: 4 % slower at 16384 x 2048 x 8192, equal at 8192 cubed; of 16: 15 % slower there).

@@ -18,9 +18,6 @@ struct RouteArgs {
     float scale;
 };
 
-// LDS written by other lanes of this wave is read behind it.
-FR_DEV void wave_lds_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); __builtin_amdgcn_wave_barrier(); }
-
 // ---- sums and maxima over the LPR lanes of a row, in every lane of it (all lanes of the wave take part) -----------------
 template <int CTRL> FR_DEV unsigned dpp(unsigned v) { return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true); }
 template <int LPR, typename F>
