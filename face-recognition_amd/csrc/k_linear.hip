@@ -94,9 +94,12 @@ FR_DEV int slot_at(const GemmArgs& a, long p) {
     const int s = a.order[p];
     return (unsigned)s < (unsigned)a.M ? s : -1;
 }
-// Row of x that slot s of the order multiplies (0 where there is none: its result goes nowhere), or the one of position p.
-FR_DEV long slot_row(const GemmArgs& a, int s) { return s < 0 ? 0 : __umulhi(2u * s, a.k_mul) >> a.k_shift; }     // s / k
-FR_DEV long x_row(const GemmArgs& a, long p) { return !a.order || a.rows_sorted ? p : slot_row(a, slot_at(a, p)); }
+// Row of x that position p of the order multiplies (0 where there is none: its result goes nowhere).
+FR_DEV long x_row(const GemmArgs& a, long p) {
+    if (!a.order || a.rows_sorted) return p;
+    const int s = slot_at(a, p);
+    return s < 0 ? 0 : __umulhi(2u * s, a.k_mul) >> a.k_shift;     // s / k
+}
 // Row of the output for position p of the order; -1: none, as the table names no slot (where neither side goes by slots it is not read).
 FR_DEV long out_row(const GemmArgs& a, long p) {
     if (!a.order || (a.rows_sorted && !a.out_slots)) return p;
@@ -267,33 +270,27 @@ __global__ __launch_bounds__(64 * WM * WN, BM == 128 && BN == 128 && ST == 2 ? 4
     const unsigned char* xbase = reinterpret_cast<const unsigned char*>(a.x) + (gather ? 0 : r0 * a.ldx * Elem<T>::BYTES) + k0;
     const unsigned char* wbase = reinterpret_cast<const unsigned char*>(a.w) + (none ? 0 : (nbase + n0) * pitch) + k0;
     unsigned off[DMA];                                       // x rows, then weight rows
-    int* lies = reinterpret_cast<int*>(smem + ST * BUF);     // [NW], of gathered rows: whether a wave met an entry of the order that names no slot
-    bool met = false;
 #pragma unroll
     for (int j = 0; j < WI; ++j) off[XI + j] = (unsigned)(min(8 * (wave + NW * j) + (lane >> 3), a.N - 1 - n0) * pitch) + kw;
 #pragma unroll
     for (int j = 0; j < XI; ++j) {
         const long p = min(r0 + 8 * (wave + NW * j) + (lane >> 3), r1 - 1);
-        long row = p - r0;
-        if (gather) {
-            const int s = slot_at(a, p);
-            met |= s < 0;
-            row = slot_row(a, s);
-        }
-        off[j] = (unsigned)(row * a.ldx * Elem<T>::BYTES) + kx;
+        off[j] = (unsigned)((gather ? x_row(a, p) : p - r0) * a.ldx * Elem<T>::BYTES) + kx;
     }
-    // A table that holds is not looked up again for rows in its own order; `lies` is written before the first barrier.
+    // Gathered rows in the order's positions: every wave looks over the tile's entries while its first loads are on their way, and
+    // the epilogue looks them up only where one names no slot (always: experts bulk 2 % slower).
     bool by_slot = a.order && a.out_slots;
-    auto tell = [&]() __attribute__((always_inline)) {
-        const bool any = __ballot(met) != 0;
-        if (gather && lane == 0) lies[wave] = any;
-    };
-    auto hear = [&]() __attribute__((always_inline)) {
-        if (!gather || a.out_slots) return;
-        int any = 0;
+    const bool look = gather && !a.out_slots;
+    int slots[BM / 64];
+    if (look)
 #pragma unroll
-        for (int q = 0; q < NW; ++q) any |= lies[q];
-        by_slot = __builtin_amdgcn_readfirstlane(any) != 0;
+        for (int q = 0; q < BM / 64; ++q) slots[q] = slot_at(a, min(r0 + 64 * q + lane, r1 - 1));
+    auto looked = [&]() __attribute__((always_inline)) {
+        if (!look) return;
+        bool lies = false;
+#pragma unroll
+        for (int q = 0; q < BM / 64; ++q) lies |= slots[q] < 0;
+        by_slot = __ballot(lies) != 0;
     };
     auto place = [&](int into, int d) __attribute__((always_inline)) {          // of instruction d in LDS
         return smem + into + (d < XI ? wave + NW * d : BM / 8 + wave + NW * (d - XI)) * 1024;
@@ -388,22 +385,17 @@ __global__ __launch_bounds__(64 * WM * WN, BM == 128 && BN == 128 && ST == 2 ? 4
             for (int s = 0; s < ST && s < slices; ++s) stage(s, s * BUF, 0, XI);
         } else
             for (int s = 0; s < ST && s < slices; ++s) stage(s, s * BUF, 0, DMA);
-        tell();
+        looked();
         if constexpr (!WHOLE) wait_counts<0, 0>();
-        if (slices >= ST) wait_counts<(ST == 2 ? XI : DMA) * (ST - 1), 0>();
-        else wait_counts<0, 0>();
+        if (slices >= ST) wait_counts<(ST == 2 ? XI : DMA) * (ST - 1), 15>();
+        else wait_counts<0, 15>();
         block_barrier();
-        hear();
 #pragma unroll
         for (int q = 0; q < TM + TN; ++q) fetch(0, 0, q);
         int s = 0;
         for (; s + ST < full; ++s) slice(s, true);
         for (; s < slices; ++s) slice(s, false);
-    } else {
-        tell();
-        __syncthreads();
-        hear();
-    }
+    } else looked();
 
     // epilogue, from the registers: vector q of x row 16 j + li is outputs n + 32 q .. + 7, a store 16 rows of 64 bytes (fp32: two
     // of 64).  Each choice of type or activation is made once for all vectors it concerns; a part's residuals are asked for
@@ -733,7 +725,7 @@ int launch_tile(GemmArgs a, hipStream_t st) {
     const long mt = a.order ? a.M / BM + std::min<long>(a.M, a.E + 1) : (a.M + BM - 1) / BM;
     a.n_tiles = (int)((a.N + (BN - 1l)) / BN);
     if (mt * a.n_tiles * a.splits >= (1l << 32) / (64 * WM * WN)) FR_FAIL(FR_ERR_UNSUPPORTED, "adapter product: more output tiles than a launch takes");
-    const int lds = ST * (BM + BN) * 128 + (a.order && !a.rows_sorted ? WM * WN * 4 : 0);      // gathered rows: `lies`
+    const int lds = ST * (BM + BN) * 128;
     static_assert(WN * BM <= ST * (BM + BN), "the ring has room for the vectors that N ends in: 32 bytes a lane and row tile");
     FR_BIG_LDS_ONCE((gemm_tile_kernel<T, BM, BN, WM, WN, ST, WHOLE>), lds);
     hipLaunchKernelGGL((gemm_tile_kernel<T, BM, BN, WM, WN, ST, WHOLE>), dim3((unsigned)(mt * a.n_tiles * a.splits)), dim3(64 * WM * WN), lds, st, a);
